@@ -86,7 +86,9 @@ typedef enum slm_role {
     SLM_ROLE_MOMENT2_F32 = 3      /* optimizer/adamw-m2.f32 */
 } slm_role;
 
-typedef enum slm_dtype { SLM_DTYPE_F32 = 0, SLM_DTYPE_BF16 = 1 } slm_dtype;
+/* SLM_DTYPE_F16 is a gradient-list type (slm_grad_view); the flat entry points
+ * take f32 and bf16. */
+typedef enum slm_dtype { SLM_DTYPE_F32 = 0, SLM_DTYPE_BF16 = 1, SLM_DTYPE_F16 = 2 } slm_dtype;
 typedef enum slm_memory { SLM_MEMORY_DEVICE = 0, SLM_MEMORY_HOST = 1 } slm_memory;
 typedef enum slm_nonfinite_policy {
     SLM_NONFINITE_SKIP = 0,  /* skip the update, state bit-unchanged, halve a dynamic scale */
@@ -402,6 +404,106 @@ typedef struct slm_norm_result {
 } slm_norm_result;
 int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_scale,
                           float max_grad_norm, slm_norm_result* out_device, void* stream);
+
+/* ---- gradient lists -------------------------------------------------------------
+ * No counterpart in the reference, whose graph hands back one flat gradient
+ * (src/model/accelerator/full_model.rs:172-201).  A list names the tensors a
+ * backward pass leaves behind -- many, of several types, contiguous or rows
+ * with a pitch (columns of a fused projection's gradient), at any address that
+ * is aligned to their element -- and takes them as they lie: norm, clipping,
+ * accumulation into the flat f32 buffer, and the optimizer step.
+ *
+ * A list borrows its tensors: they must stay allocated while the list or work
+ * enqueued with it uses them.  It is immutable but for slm_grad_list_bind, so
+ * calls with it may run at the same time on several streams or in several
+ * captured graphs, each with its own workspace and results; all but
+ * slm_grad_list_create and _destroy may be captured.  Elements are counted in
+ * row-major order, tensor after tensor.
+ *
+ * Norm: with u = g / loss_scale in f32, each tensor is cut into units of
+ * consecutive elements (a power of two between 4,096 and 2^30, so that a list
+ * has about 8,192 of them at most); a unit's squares are added by the tree of
+ * the flat norm (8 at a time pairwise in f32, then f64), and its partials in a
+ * fixed order in f64.  The result does not depend on the device or the run,
+ * only on the tensors' sizes.  The tree restarts at every tensor, so the sum
+ * can differ from the flat norm's in the last bits of the f64; both are
+ * within 3e-7 relative of the exact sum while the squares are normal f32
+ * numbers (|u| above 1e-19; a square above 3e38 is infinite, and counts as a
+ * non-finite gradient). */
+typedef struct slm_grad_view {
+  const void* data;     /* device memory, aligned to the element */
+  uint64_t rows, columns;
+  uint64_t row_stride;  /* elements from one row to the next, >= columns */
+  int32_t dtype;        /* slm_dtype */
+} slm_grad_view;
+typedef struct slm_grad_list slm_grad_list;
+typedef enum slm_norm_kind {
+    SLM_NORM_L2 = 0,  /* sqrt of the sum of squares */
+    SLM_NORM_MAX = 1  /* the largest magnitude */
+} slm_norm_kind;
+/* Written to device memory.  When a gradient is inf or NaN or the sum
+ * overflows: nonfinite 1, clip_scale 0. */
+typedef struct slm_list_norm {
+    float norm;        /* of all gradients divided by the loss scale */
+    float clip_scale;  /* min(max_norm / norm, 1); 1 when the norm is 0 */
+    float max_abs;     /* the largest magnitude after unscaling */
+    float nonfinite;   /* 0 or 1 */
+} slm_list_norm;
+
+/* The list of n >= 1 tensors on `device`.  Tensors without elements are allowed
+ * (their data is not looked at).  Addresses must lie in that device's memory
+ * (SLM_ERR_INVALID_ARGUMENT otherwise). */
+int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
+                         slm_grad_list** out);
+/* Waits for the device's outstanding work, then frees the list. */
+int slm_grad_list_destroy(slm_grad_list* list);
+uint64_t slm_grad_list_elements(const slm_grad_list* list);
+/* Bytes of device workspace of one norm or clip call. */
+uint64_t slm_grad_list_workspace_bytes(const slm_grad_list* list);
+/* Points the list at new addresses (same sizes, types and strides), in stream
+ * order: for gradients that are allocated anew every step.  Calls enqueued
+ * on other streams must be ordered against it by the caller. */
+int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n, void* stream);
+
+/* The norm of the list.  result_device, and where they are not NULL
+ * tensor_norms_device and tensor_max_device (n floats each: every tensor's own
+ * norm of that kind and largest magnitude; 0 for a tensor without elements)
+ * and sum_squares_device (the f64 sum of squares), receive the results in
+ * stream order.  workspace_device: slm_grad_list_workspace_bytes(list) bytes,
+ * 16-byte aligned, not shared with a call that may run at the same time. */
+int slm_grad_list_norm(const slm_grad_list* list, float loss_scale, float max_norm, int kind,
+                       slm_list_norm* result_device, float* tensor_norms_device,
+                       float* tensor_max_device, double* sum_squares_device,
+                       void* workspace_device, uint64_t workspace_bytes, void* stream);
+/* The norm, and every gradient divided by the loss scale and multiplied by the
+ * clip scale (each in f32, rounded once more to the output's type, nearest
+ * even), written to `out` -- a list of tensors of the same sizes, of any type
+ * and layout -- or in place when out is NULL or the list itself.  Nothing is
+ * written when a gradient is not finite.  Output tensors that share elements
+ * with each other, or with a gradient other than the same one in the same
+ * layout and type, are refused. */
+int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, float loss_scale,
+                       float max_norm, int kind, slm_list_norm* result_device,
+                       float* tensor_norms_device, float* tensor_max_device,
+                       double* sum_squares_device, void* workspace_device,
+                       uint64_t workspace_bytes, void* stream);
+/* slm_grad_accumulate from a list: acc_device (n == the list's elements, f32,
+ * 16-byte aligned) += the list's values, tensor after tensor, or with overwrite
+ * = them. */
+int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint64_t n,
+                             int overwrite, void* stream);
+/* slm_opt_step, slm_opt_norm_pass and slm_opt_norm_pass_accumulate with the
+ * gradients in a list whose tensors are the handle's parameters in order and
+ * size (E1_PARAMETER_LAYOUT_MISMATCH otherwise).  A ZeRO-1 handle refuses them.
+ * After slm_opt_norm_pass_list the list must live, unbound, until the update
+ * pass has run. */
+int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
+                      slm_step_result* out, void* stream);
+int slm_opt_norm_pass_list(slm_opt_handle* h, const slm_grad_list* list,
+                           const slm_step_config* cfg, void* stream);
+int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
+                                      const slm_grad_list* list, int overwrite,
+                                      const slm_step_config* cfg, void* stream);
 
 /* ---- loss scaler ------------------------------------------------------------- */
 int slm_opt_set_loss_scale(slm_opt_handle* h, float scale, uint32_t good_steps);

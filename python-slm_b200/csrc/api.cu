@@ -175,6 +175,11 @@ int allocate_state(slm_opt_handle* h, uint64_t w16_elems) {
           "upload tile table");
   const DeviceScaler sc{65536.0f, 0u};
   SLM_TRY(cudaMemcpy(h->d_scaler, &sc, sizeof(sc), cudaMemcpyHostToDevice), "upload scaler");
+  if (!h->sharded()) {
+    SLM_TRY(cudaMalloc(&h->d_list_partials, list_partial_bytes(h->offsets)),
+            "cudaMalloc list partials");
+    h->grid_list_update = list_update_grid(h->device);
+  }
 #undef SLM_TRY
   h->grid_norm = norm_partials_grid(h->device);
   h->grid_norm_bulk = norm_bulk_grid(h->device);
@@ -453,6 +458,16 @@ int slmopt::phase_mark(slm_opt_handle* h, cudaStream_t s) {
   return h->cuda(cudaEventRecord(t.ev[t.marks++], s), "phase timing");
 }
 
+int slmopt::finish_step(slm_opt_handle* h, slm_step_result* out, cudaStream_t s) {
+  h->pending = true;
+  h->pending_stream = s;
+  if (!out) return SLM_OK;
+  DeviceStepState ds;
+  if (int st = read_state(h, s, &ds)) return st;
+  h->pending = false;
+  return finish_result(h, ds, out);
+}
+
 void slmopt::phase_end(slm_opt_handle* h, int kind) {
   PhaseTimer& t = h->timer;
   if (!t.enabled) return;
@@ -604,6 +619,7 @@ int slm_opt_destroy(slm_opt_handle* h) {
   cudaFree(h->d_seq_carry);
   cudaFree(h->d_seq_ws);
   cudaFree(h->d_staging);
+  cudaFree(h->d_list_partials);
   for (int k = 0; k < slm_opt_handle::PinnedRing::kSlots; ++k) {
     if (h->ring.drained[k]) {
       cudaEventSynchronize(h->ring.drained[k]);
@@ -739,6 +755,7 @@ int slm_opt_norm_pass(slm_opt_handle* h, const void* grads, int dtype, int memor
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const void* dev = nullptr;
   h->pass_grads = nullptr;
+  h->pass_is_list = false;
   if ((st = stage_grads(h, grads, dtype, memory, s, &dev))) return st;
   if ((st = enqueue_norm(h, dev, dtype, cfg, s))) return st;
   h->pass_grads = dev;
@@ -814,6 +831,7 @@ int slm_opt_norm_pass_accumulate(slm_opt_handle* h, float* acc_device, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const void* dev = nullptr;
   h->pass_grads = nullptr;
+  h->pass_is_list = false;
   if ((st = stage_grads(h, micro, dtype, memory, s, &dev))) return st;
   const FinalizeParams fp = finalize_params(h, cfg);
   if ((st = h->cuda(launch_accumulate_norm(dtype, acc_device, dev, h->P, overwrite, h->n_chunks,
@@ -829,14 +847,16 @@ int slm_opt_norm_pass_accumulate(slm_opt_handle* h, float* acc_device, const voi
 
 int slm_opt_update_pass(slm_opt_handle* h, const slm_step_config* cfg, void* stream) {
   if (!h) return fail(SLM_ERR_INVALID_ARGUMENT, "NULL handle");
-  if (!h->pass_grads)
+  if (!h->pass_grads && !h->pass_is_list)
     return h->err(SLM_ERR_INVALID_ARGUMENT, "slm_opt_update_pass needs a preceding norm pass");
   int st = check_config(h, cfg);
   if (st) return st;
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, s);
+  st = h->pass_is_list ? enqueue_list_update(h, h->pass_list, cfg, s)
+                       : enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, s);
   h->pass_grads = nullptr;
+  h->pass_is_list = false;
   h->pending = true;
   h->pending_stream = s;
   return st;
@@ -861,13 +881,7 @@ int run_step(slm_opt_handle* h, const void* grads, int dtype, int memory,
     if ((st = phase_mark(h, s))) return st;
   }
   phase_end(h);
-  h->pending = true;
-  h->pending_stream = s;
-  if (!out) return SLM_OK;
-  DeviceStepState ds;
-  if ((st = read_state(h, s, &ds))) return st;
-  h->pending = false;
-  return finish_result(h, ds, out);
+  return finish_step(h, out, s);
 }
 
 int release_slot(slm_opt_handle* h, slm_opt_handle::UploadSlot* slot, cudaStream_t s) {

@@ -100,9 +100,13 @@ struct slm_opt_handle {
   int grid_norm = 0;       // resident blocks of the per-chunk tree kernels
   int grid_norm_bulk = 0;  // persistent grid of the bulk-copy norm pass
   int grid_update[2] = {0, 0};
+  int grid_list_update = 0;
+  void* d_list_partials = nullptr;  // norm partials of a gradient list over the table
   // Gradients seen by the last norm pass (consumed by the update pass).
   const void* pass_grads = nullptr;
   int pass_dtype = -1;
+  slmopt::GradListView pass_list{};  // of slm_opt_norm_pass_list, when pass_is_list
+  bool pass_is_list = false;
   cudaStream_t pending_stream = nullptr;
   bool pending = false;
   std::string last_error = "no error";
@@ -186,6 +190,15 @@ int build_table(slm_opt_handle* h, const slm_tensor_spec* table, uint32_t n_tens
 int check_config(slm_opt_handle* h, const slm_step_config* cfg);
 FinalizeParams finalize_params(const slm_opt_handle* h, const slm_step_config* cfg);
 int read_state(slm_opt_handle* h, cudaStream_t s, DeviceStepState* out);
+// A step is enqueued on s: waits for and returns its result when out != NULL.
+int finish_step(slm_opt_handle* h, slm_step_result* out, cudaStream_t s);
+// Gradient lists (gradlist_api.cu): the handle's partials, and the two passes
+// of a step on a list.
+uint64_t list_partial_bytes(const std::vector<uint64_t>& offsets);
+int enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
+                      cudaStream_t s);
+int enqueue_list_update(slm_opt_handle* h, const GradListView& list, const slm_step_config* cfg,
+                        cudaStream_t s);
 void fill_result(const DeviceStepState& s, slm_step_result* out);
 // ZeRO-1 pieces (zero1.cu).
 int zero1_step(slm_opt_handle* h, const void* grads, int dtype, int memory,

@@ -245,4 +245,95 @@ int norm_partials_grid(int device);
 int norm_bulk_grid(int device);
 int adamw_update_grid(int device, int dtype);
 
+// ---- gradient lists (gradlist.cu) ---------------------------------------------
+// A list is cut into units: at most `unit_elems` consecutive elements (row-major
+// order) of one tensor, so a unit never mixes tensors or types and its first
+// element's address depends on the tensor's alone.  A unit is one block's work
+// in the norm, clip and accumulate kernels and one f64 partial of the list's
+// fixed tree, which therefore restarts at every tensor.
+constexpr uint32_t kGradF32 = 0, kGradBf16 = 1, kGradF16 = 2;  // slm_dtype
+constexpr uint32_t kGradTypeMask = 3u;
+constexpr uint32_t kGradVector = 4u;   // every 8-element vector is one run on a 16-byte boundary
+constexpr uint32_t kGradPitched = 8u;  // rows are further apart than their columns
+struct __align__(16) GradTensor {
+  const void* ptr;
+  uint64_t elements;
+  uint64_t columns, row_stride;  // elements; only read when kGradPitched
+  uint64_t offset;               // flat position of the first element in the list
+  uint32_t first_unit;
+  uint32_t flags;
+};
+struct __align__(16) GradUnit {
+  const void* ptr;  // first element of the unit; of the tensor when kGradPitched
+  uint32_t count;   // elements, 1..unit_elems
+  uint32_t tensor;
+  uint32_t index;   // unit number within its tensor
+  uint32_t flags;
+  uint64_t offset;  // flat position of the unit's first element
+};
+static_assert(sizeof(GradTensor) == 48 && sizeof(GradUnit) == 32, "list tables");
+// The smallest and largest unit; between them the number of units stays near
+// kGradUnitsAimed, which bounds the partials a finalize has to add.
+constexpr uint32_t kGradUnitMin = 4096;
+constexpr uint32_t kGradUnitMax = 1u << 30;
+constexpr uint64_t kGradUnitsAimed = 8192;
+inline uint32_t grad_unit_elems(uint64_t total) {
+  uint32_t u = kGradUnitMin;
+  while (u < kGradUnitMax && total / u > kGradUnitsAimed) u *= 2;
+  return u;
+}
+struct GradListView {
+  const GradUnit* units;
+  const GradTensor* tensors;
+  uint32_t n_units, n_tensors;
+  uint32_t unit_elems;
+  uint64_t elements;
+};
+struct GradListOut {
+  float* result;         // norm, clip scale, largest magnitude, non-finite flag
+  float* tensor_norms;   // n_tensors, or NULL
+  float* tensor_max;     // n_tensors, or NULL
+  double* sum_squares;   // or NULL
+};
+// Per unit: f64 sum of squares and f32 bits of the largest magnitude (of the
+// stored values; the finalize unscales it).
+struct GradPartials {
+  double* sums;
+  uint32_t* tops;
+};
+cudaError_t launch_list_norm(const GradListView& list, float scale, const DeviceScaler* scaler,
+                             const GradPartials& part, cudaStream_t stream);
+cudaError_t launch_list_finalize(const GradListView& list, const GradPartials& part, float scale,
+                                 float max_norm, int kind, const GradListOut& out,
+                                 cudaStream_t stream);
+cudaError_t launch_list_clip(const GradListView& list, const GradListView& out, float scale,
+                             const float* result, bool in_place, cudaStream_t stream);
+cudaError_t launch_list_accumulate(const GradListView& list, float* acc, int overwrite,
+                                   cudaStream_t stream);
+// The last micro-batch: accumulates and forms the partials of the sums.
+cudaError_t launch_list_accumulate_norm(const GradListView& list, float* acc, int overwrite,
+                                        float scale, const DeviceScaler* scaler,
+                                        const GradPartials& part, cudaStream_t stream);
+// The handle's decision (clip, skip, scaler) from a list's partials.
+cudaError_t launch_list_decide(const GradListView& list, const GradPartials& part,
+                               DeviceScaler* scaler, DeviceStepState* st,
+                               const FinalizeParams& fp, cudaStream_t stream);
+// AdamW over the flat state with the gradients read from the list's tensors,
+// which are the state's tensors in order.
+cudaError_t launch_list_update(const GradListView& list, float* master, float* moment,
+                               float* variance, uint16_t* w16, const uint64_t* offsets,
+                               const uint8_t* decay, const uint32_t* tile_first,
+                               const AdamwParams& p, DeviceStepState* st, int grid,
+                               cudaStream_t stream);
+int list_update_grid(int device);
+// Points the list's tables at new first elements (tensors [begin, begin + n)).
+constexpr uint32_t kGradBindBatch = 256;
+struct GradBind {
+  const void* ptr[kGradBindBatch];
+  uint32_t flags[kGradBindBatch];
+};
+cudaError_t launch_list_bind(GradTensor* tensors, GradUnit* units, uint32_t n_units,
+                             uint32_t unit_elems, const GradBind& bind, uint32_t begin, uint32_t n,
+                             cudaStream_t stream);
+
 }  // namespace slmopt

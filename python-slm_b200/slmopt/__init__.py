@@ -7,6 +7,7 @@ tensor table, seeded synthetic inputs and the ZeRO-1 data-parallel driver.
 """
 from . import _lib
 from ._lib import SlmError, StepResult, load
+from .gradlist import GradientList, GradientNorm
 from .layout import GqaDimensions, TensorTable, weight_decay_for
 from .optimizer import ARTIFACTS, B200Adamw, B200TrainerBackend, StepOptions
 
@@ -16,6 +17,8 @@ __all__ = [
     "B200Adamw",
     "B200TrainerBackend",
     "GqaDimensions",
+    "GradientList",
+    "GradientNorm",
     "SlmError",
     "StepOptions",
     "StepResult",

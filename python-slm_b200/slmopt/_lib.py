@@ -45,6 +45,9 @@ ROLE_MOMENT2_F32 = 3
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
+NORM_L2 = 0
+NORM_MAX = 1
 MEMORY_DEVICE = 0
 MEMORY_HOST = 1
 NONFINITE_SKIP = 0
@@ -123,6 +126,29 @@ class ClipResult(ctypes.Structure):
     ]
 
 
+class GradView(ctypes.Structure):
+    """slm_grad_view: one tensor of a gradient list."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+        ("columns", ctypes.c_uint64),
+        ("row_stride", ctypes.c_uint64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class ListNorm(ctypes.Structure):
+    """slm_list_norm (written to device memory by the gradient-list calls)."""
+
+    _fields_ = [
+        ("norm", ctypes.c_float),
+        ("clip_scale", ctypes.c_float),
+        ("max_abs", ctypes.c_float),
+        ("nonfinite", ctypes.c_float),
+    ]
+
+
 NOALLOC_MAX_ELEMENTS = 268435456
 
 _P = ctypes.c_void_p
@@ -175,6 +201,18 @@ SIGNATURES = [
     ("slm_gradient_clip_scale", _I, [_P, _U64, _P, _P]),
     ("slm_gradient_clip_workspace_bytes", _U64, [_U64]),
     ("slm_gradient_clip_scale_ws", _I, [_P, _U64, _P, _U64, _P, _P]),
+    ("slm_grad_list_create", _I, [ctypes.POINTER(GradView), _U32, _I, ctypes.POINTER(_P)]),
+    ("slm_grad_list_destroy", _I, [_P]),
+    ("slm_grad_list_elements", _U64, [_P]),
+    ("slm_grad_list_workspace_bytes", _U64, [_P]),
+    ("slm_grad_list_bind", _I, [_P, ctypes.POINTER(_P), _U32, _P]),
+    ("slm_grad_list_norm", _I, [_P, _F, _F, _I, _P, _P, _P, _P, _P, _U64, _P]),
+    ("slm_grad_list_clip", _I, [_P, _P, _F, _F, _I, _P, _P, _P, _P, _P, _U64, _P]),
+    ("slm_grad_list_accumulate", _I, [_P, _P, _U64, _I, _P]),
+    ("slm_opt_step_list", _I, [_P, _P, ctypes.POINTER(StepConfig), ctypes.POINTER(StepResult),
+                               _P]),
+    ("slm_opt_norm_pass_list", _I, [_P, _P, ctypes.POINTER(StepConfig), _P]),
+    ("slm_opt_norm_pass_accumulate_list", _I, [_P, _P, _P, _I, ctypes.POINTER(StepConfig), _P]),
     ("slm_opt_set_loss_scale", _I, [_P, _F, _U32]),
     ("slm_opt_get_loss_scale", _I, [_P, ctypes.POINTER(_F), ctypes.POINTER(_U32)]),
     ("slm_canonical_learning_rate", _I, [_U64, ctypes.POINTER(_F)]),

@@ -1,0 +1,258 @@
+"""Gradients in many tensors: norm, clipping and accumulation without a flat copy.
+
+``GradientList`` names the tensors a backward pass leaves behind (CUDA tensors of
+one device, f32, bf16 or f16, contiguous or rows with a pitch) and runs the
+gradient-list entry points of the C ABI on them as they lie; ``B200Adamw.step``
+and its passes, and ``B200Trainer.process_batch``, take a list wherever they take
+a flat gradient tensor.  Every numeric operation runs in libslmopt.so.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import _lib
+
+_KINDS = {"l2": _lib.NORM_L2, "max": _lib.NORM_MAX}
+
+
+def _dtype_codes():
+    import torch
+
+    return {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
+            torch.float16: _lib.DTYPE_F16}
+
+
+def _rows(tensor) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a tensor whose elements, in row-major
+    order, are equally spaced runs; ValueError for any other layout."""
+    if tensor.is_contiguous():
+        n = tensor.numel()
+        return 1, n, n
+    dims = [(n, s) for n, s in zip(tensor.shape, tensor.stride()) if n != 1]
+    columns, inner = 1, len(dims)
+    while inner > 0 and dims[inner - 1][1] == columns:
+        columns *= dims[inner - 1][0]
+        inner -= 1
+    if inner == 0:
+        return 1, columns, columns
+    rows, stride = dims[inner - 1]
+    for n, s in reversed(dims[:inner - 1]):
+        if s != stride * rows:
+            raise ValueError("a gradient must be contiguous, or rows at one distance")
+        rows *= n
+    if stride < columns:
+        raise ValueError("a gradient's elements must not overlap")
+    return rows, columns, stride
+
+
+class GradientNorm:
+    """What a norm or clip call found, in device memory (reading a property that
+    is a tensor does not wait; ``read`` does).
+
+    ``values`` is one f32 tensor: the norm of all gradients divided by the loss
+    scale, the clip scale, the largest magnitude, 1.0 if a gradient or the norm
+    is not finite (the clip scale is then 0.0) else 0.0; and with per_tensor each
+    tensor's norm, then each tensor's largest magnitude."""
+
+    __slots__ = ("values", "_work", "_tensors")
+
+    def __init__(self, values, work, tensors: int):
+        self.values = values
+        self._work = work
+        self._tensors = tensors
+
+    @property
+    def norm(self):
+        return self.values[0]
+
+    @property
+    def clip_scale(self):
+        return self.values[1]
+
+    @property
+    def max_abs(self):
+        return self.values[2]
+
+    @property
+    def nonfinite(self):
+        return self.values[3]
+
+    @property
+    def sum_squares(self):
+        """The f64 sum of squares (0-d tensor): what ranks that hold different
+        tensors add up."""
+        return self._work[0]
+
+    @property
+    def tensor_norms(self):
+        if self.values.numel() == 4:
+            raise ValueError("the call was made without per_tensor")
+        return self.values[4:4 + self._tensors]
+
+    @property
+    def tensor_max(self):
+        if self.values.numel() == 4:
+            raise ValueError("the call was made without per_tensor")
+        return self.values[4 + self._tensors:]
+
+    def read(self) -> _lib.ListNorm:
+        """The four values on the host; waits for them."""
+        return _lib.ListNorm(*self.values[:4].tolist())
+
+
+class GradientList:
+    """Tensors whose norm, clipping, accumulation or step is wanted together.
+
+    The list holds references to the tensors.  Their storage is read at the
+    addresses of the last construction or ``bind``: after ``tensor.data = ...``
+    or a new backward pass that allocated new gradients, ``bind`` the new ones.
+    Work runs on ``stream`` (None: the legacy default stream) and is ordered
+    with the rest of that stream; the tensors must be ready there."""
+
+    def __init__(self, tensors):
+        import torch
+
+        self.lib = _lib.load()
+        self._h = None
+        self.tensors = tuple(tensors)
+        if not self.tensors:
+            raise ValueError("the list contains no tensors")
+        views = (_lib.GradView * len(self.tensors))()
+        codes = _dtype_codes()
+        self._shapes = []
+        first = self.tensors[0]
+        if not isinstance(first, torch.Tensor) or not first.is_cuda:
+            raise ValueError("gradients must be CUDA tensors")
+        self.device = first.device
+        for view, t in zip(views, self.tensors):
+            layout = self._layout(t)
+            view.data = t.data_ptr()
+            view.rows, view.columns, view.row_stride = layout[1:]
+            view.dtype = codes[t.dtype]
+            self._shapes.append(layout)
+        h = ctypes.c_void_p()
+        _lib.check(self.lib.slm_grad_list_create(views, len(self.tensors), self.device.index,
+                                                 ctypes.byref(h)))
+        self._h = h
+        self.elements = int(self.lib.slm_grad_list_elements(h))
+        self._work_bytes = int(self.lib.slm_grad_list_workspace_bytes(h))
+        self._work_doubles = 2 + (self._work_bytes + 7) // 8
+
+    def _layout(self, t):
+        import torch
+
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError("gradients must be CUDA tensors")
+        if t.device != self.device:
+            raise ValueError("gradients must be on one device")
+        if t.dtype not in _dtype_codes():
+            raise TypeError("gradients must be float32, bfloat16 or float16")
+        if t.is_conj() or t.is_neg():
+            raise ValueError("gradients must not be lazily negated views")
+        return (t.dtype, *_rows(t))
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self.lib.slm_grad_list_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    @property
+    def handle(self):
+        if not self._h:
+            raise ValueError("the list is closed")
+        return self._h
+
+    def bind(self, tensors, stream=None) -> None:
+        """Take other tensors of the same types, sizes and strides, in order."""
+        tensors = tuple(tensors)
+        if [self._layout(t) for t in tensors] != self._shapes:
+            raise ValueError("other tensors than the list's: types, sizes and strides must agree")
+        ptrs = (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+        _lib.check(self.lib.slm_grad_list_bind(self.handle, ptrs, len(tensors),
+                                               _stream_handle(stream)))
+        self.tensors = tensors
+
+    def norm(self, loss_scale: float = 1.0, max_norm: float = 1.0, kind: str = "l2",
+             per_tensor: bool = False, stream=None) -> GradientNorm:
+        """The norm ("l2", or "max": the largest magnitude) of all gradients
+        divided by loss_scale, and the clip scale min(max_norm / norm, 1)."""
+        return self._run(False, None, loss_scale, max_norm, kind, per_tensor, stream)
+
+    def clip(self, max_norm: float = 1.0, loss_scale: float = 1.0, kind: str = "l2", out=None,
+             per_tensor: bool = False, stream=None) -> GradientNorm:
+        """Divide by loss_scale and scale down to max_norm, in place or into the
+        tensors of the list ``out`` (same sizes, any type).  Nothing is written
+        when a gradient is inf or NaN."""
+        return self._run(True, out, loss_scale, max_norm, kind, per_tensor, stream)
+
+    def _run(self, write, out, loss_scale, max_norm, kind, per_tensor, stream) -> GradientNorm:
+        import torch
+
+        code = _KINDS.get(kind)
+        if code is None:
+            raise ValueError('kind must be "l2" or "max"')
+        n = len(self.tensors)
+        values = torch.empty(4 + (2 * n if per_tensor else 0), dtype=torch.float32,
+                             device=self.device)
+        # One allocation: the f64 sum of squares, then the workspace.
+        work = torch.empty(self._work_doubles, dtype=torch.float64, device=self.device)
+        s = _stream_handle(stream)
+        _use_on(values, work, s)
+        v, w = values.data_ptr(), work.data_ptr()
+        norms, tops = (v + 16, v + 16 + 4 * n) if per_tensor else (None, None)
+        if write:
+            st = self.lib.slm_grad_list_clip(self.handle, out.handle if out is not None else None,
+                                             loss_scale, max_norm, code, v, norms, tops, w, w + 16,
+                                             self._work_bytes, s)
+        else:
+            st = self.lib.slm_grad_list_norm(self.handle, loss_scale, max_norm, code, v, norms,
+                                             tops, w, w + 16, self._work_bytes, s)
+        _lib.check(st)
+        return GradientNorm(values, work, n)
+
+    def accumulate(self, acc, overwrite: bool = False, stream=None) -> None:
+        """acc (f32, one value per element, tensor after tensor) += the
+        gradients, or acc = the gradients."""
+        import torch
+
+        if not acc.is_cuda or acc.device != self.device or acc.dtype != torch.float32 or \
+                not acc.is_contiguous() or acc.numel() != self.elements:
+            raise ValueError("acc must be a contiguous f32 tensor on the list's device with one "
+                             "value per element")
+        _lib.check(self.lib.slm_grad_list_accumulate(self.handle, acc.data_ptr(), self.elements,
+                                                     1 if overwrite else 0,
+                                                     _stream_handle(stream)))
+
+
+def _stream_handle(stream) -> int | None:
+    if stream is None or isinstance(stream, int):
+        return stream
+    return int(stream.cuda_stream)  # torch.cuda.Stream
+
+
+def _use_on(values, work, stream: int | None) -> None:
+    """Tells torch's allocator when memory it gave for the current stream is used
+    on another one."""
+    import torch
+
+    handle = stream or 0
+    if torch.cuda.current_stream(values.device).cuda_stream != handle:
+        other = torch.cuda.ExternalStream(handle, device=values.device) if handle else \
+            torch.cuda.default_stream(values.device)
+        values.record_stream(other)
+        work.record_stream(other)

@@ -14,6 +14,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
+from .gradlist import GradientList, _stream_handle
 from .layout import GqaDimensions, TensorTable
 
 # Artifact roles and paths of the five-artifact codec (src/train/full_state.rs:27-36).
@@ -89,6 +90,16 @@ def _grad_pointer(grads):
         raise TypeError("gradients must be float32 or bfloat16")
     mem = _lib.MEMORY_DEVICE if grads.is_cuda else _lib.MEMORY_HOST
     return grads.data_ptr(), dt, mem, grads.numel(), grads
+
+
+class _DeviceArray:
+    """__cuda_array_interface__ of a handle's buffer; keeps the handle's owner alive."""
+
+    def __init__(self, owner, pointer: int, n: int, typestr: str):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"shape": (n,), "typestr": typestr, "version": 3,
+                                         "data": (pointer, False), "strides": None,
+                                         "stream": None}
 
 
 class B200Adamw:
@@ -168,6 +179,27 @@ class B200Adamw:
         self._check(self.lib.slm_opt_device_buffer(self._h, role, ctypes.byref(p)))
         return int(p.value)
 
+    def state_tensors(self) -> dict:
+        """The state's device buffers as CUDA tensors (views, not copies): master,
+        moment and variance in f32 (the handle's shard, if it is one rank's),
+        the P weights in bf16.  They are valid until the handle is closed; bf16
+        must stay RNE(master)."""
+        import torch
+
+        begin, length = ctypes.c_uint64(), ctypes.c_uint64()
+        self._check(self.lib.slm_opt_shard_range(self._h, ctypes.byref(begin),
+                                                 ctypes.byref(length)))
+        out = {}
+        for key, role, typestr in (("master", _lib.ROLE_MASTER_F32, "<f4"),
+                                   ("moment", _lib.ROLE_MOMENT1_F32, "<f4"),
+                                   ("variance", _lib.ROLE_MOMENT2_F32, "<f4"),
+                                   ("bf16", _lib.ROLE_PARAMETERS_BF16, "<i2")):
+            n = self.P if key == "bf16" else int(length.value)
+            t = torch.as_tensor(_DeviceArray(self, self.device_buffer(role), n, typestr),
+                                device=f"cuda:{self.device}")
+            out[key] = t.view(torch.bfloat16) if key == "bf16" else t
+        return out
+
     def validate(self) -> None:
         self._check(self.lib.slm_opt_validate_state(self._h))
 
@@ -203,11 +235,19 @@ class B200Adamw:
     # ---- the step ----------------------------------------------------------------------
     def step(self, grads, options: StepOptions | None = None, stream=None,
              wait: bool = True) -> _lib.StepResult | None:
-        """Fused step over P gradients (torch device tensor or host array).
+        """Fused step over P gradients (torch device tensor, host array, or a
+        GradientList of the table's tensors).
 
         With ``wait`` the call blocks and returns the StepResult (raising
         SlmError on a failed status); otherwise it only enqueues on ``stream``.
         """
+        if isinstance(grads, GradientList):
+            cfg = (options or StepOptions()).to_c()
+            res = _lib.StepResult() if wait else None
+            self._check(self.lib.slm_opt_step_list(self._h, grads.handle, ctypes.byref(cfg),
+                                                   ctypes.byref(res) if wait else None,
+                                                   _stream_handle(stream)))
+            return res
         ptr, dt, mem, n, keep = _grad_pointer(grads)
         if n != self.P:
             raise ValueError(f"expected {self.P} gradients, got {n}")
@@ -256,6 +296,11 @@ class B200Adamw:
     def norm_pass(self, grads, options: StepOptions | None = None, stream=None):
         """Enqueue the unscale / non-finite / norm / clip pass; returns the
         keep-alive object that must outlive the matching update_pass."""
+        if isinstance(grads, GradientList):
+            cfg = (options or StepOptions()).to_c()
+            self._check(self.lib.slm_opt_norm_pass_list(self._h, grads.handle, ctypes.byref(cfg),
+                                                        _stream_handle(stream)))
+            return grads
         ptr, dt, mem, n, keep = _grad_pointer(grads)
         if n != self.P:
             raise ValueError(f"expected {self.P} gradients, got {n}")
@@ -265,7 +310,11 @@ class B200Adamw:
         return keep
 
     def accumulate(self, acc, micro, overwrite: bool = False, stream=None) -> None:
-        """acc (device f32[P]) += micro (device f32 or bf16 [P]), or acc = micro."""
+        """acc (device f32[P]) += micro (device f32 or bf16 [P], or a
+        GradientList), or acc = micro."""
+        if isinstance(micro, GradientList):
+            micro.accumulate(acc, overwrite, stream)
+            return
         ptr, dt, mem, n, keep = _grad_pointer(micro)
         if mem != _lib.MEMORY_DEVICE or not acc.is_cuda:
             raise ValueError("accumulate works on device tensors")
@@ -278,6 +327,13 @@ class B200Adamw:
                              overwrite: bool = False, stream=None):
         """Last micro-batch: acc += micro fused with the norm pass over acc;
         follow with update_pass().  Returns the keep-alive for micro."""
+        if isinstance(micro, GradientList):
+            _check_accumulator(acc, self.P, self.device)
+            cfg = (options or StepOptions()).to_c()
+            self._check(self.lib.slm_opt_norm_pass_accumulate_list(
+                self._h, acc.data_ptr(), micro.handle, 1 if overwrite else 0, ctypes.byref(cfg),
+                _stream_handle(stream)))
+            return micro
         ptr, dt, mem, n, keep = _grad_pointer(micro)
         if n != self.P or acc.numel() != self.P:
             raise ValueError(f"expected {self.P} elements")
@@ -353,12 +409,13 @@ def gradient_clip_scale(gradients, stream=None, parallel: bool = True) -> tuple[
     return int(res.status), float(res.sum_squares), float(res.clip_scale)
 
 
-def _stream_handle(stream) -> int | None:
-    if stream is None:
-        return None
-    if isinstance(stream, int):
-        return stream
-    return int(stream.cuda_stream)  # torch.cuda.Stream
+def _check_accumulator(acc, n: int, device: int) -> None:
+    import torch
+
+    if not acc.is_cuda or acc.device.index != device or acc.dtype != torch.float32 or \
+            not acc.is_contiguous() or acc.numel() != n:
+        raise ValueError("acc must be a contiguous f32 tensor on the handle's device with one "
+                         "value per parameter")
 
 
 class B200TrainerBackend:
