@@ -420,16 +420,17 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * slm_grad_list_create and _destroy may be captured.  Elements are counted in
  * row-major order, tensor after tensor.
  *
- * Norm: with u = g / loss_scale in f32, each tensor is cut into units of
- * consecutive elements (a power of two between 4,096 and 2^30, so that a list
- * has about 8,192 of them at most); a unit's squares are added by the tree of
- * the flat norm (8 at a time pairwise in f32, then f64), and its partials in a
- * fixed order in f64.  The result does not depend on the device or the run,
- * only on the tensors' sizes.  The tree restarts at every tensor, so the sum
- * can differ from the flat norm's in the last bits of the f64; both are
- * within 3e-7 relative of the exact sum while the squares are normal f32
- * numbers (|u| above 1e-19; a square above 3e38 is infinite, and counts as a
- * non-finite gradient). */
+ * Norm: each tensor is cut into units of consecutive elements (a power of two
+ * between 4,096 and 2^30, so that a list has about 8,192 of them at most).
+ * Within a unit 8 consecutive values are squared and added in f32 (fused
+ * multiply-adds), and these sums in f64 by the flat norm's tree; the units'
+ * partials are added in f64 in a fixed order and divided by the loss scale
+ * squared.  The result does not depend on the device or the run, only on the
+ * tensors' sizes.  It is within 3e-7 relative of the exact sum, as the flat
+ * norm's is, but not the same bits (the tree restarts at every tensor).  The
+ * values are squared as they are stored for loss scales from 1 to 2^20, else
+ * times the power of two next to 1 / loss_scale; a square above 3e38 is
+ * infinite and counts as a non-finite gradient, one below 1e-38 loses bits. */
 typedef struct slm_grad_view {
   const void* data;     /* device memory, aligned to the element */
   uint64_t rows, columns;

@@ -19,26 +19,107 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 namespace slmopt {
 namespace {
 
 constexpr uint32_t kListThreads = 256;
-constexpr uint32_t kFinalThreads = 512;
+constexpr uint32_t kFinalThreads = 1024;
 
 // ---- element types ------------------------------------------------------------
-// Raw<T>: 8 elements as they lie in memory, kept packed while loads are in flight.
+template <uint32_t T>
+constexpr uint32_t kSize = T == kGradF32 ? 4u : 2u;
+template <uint32_t T>
+constexpr uint32_t kVecBytes = kVec * kSize<T>;  // a vector: 32 or 16 bytes, one load
+__device__ __forceinline__ uint32_t elem_bytes(uint32_t type) { return type == kGradF32 ? 4u : 2u; }
+
+template <uint32_t T>
+__device__ __forceinline__ float from_bits(uint32_t b) {
+  if constexpr (T == kGradF32)
+    return __uint_as_float(b);
+  else if constexpr (T == kGradBf16)
+    return __uint_as_float(b << 16);
+  else
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+}
+// Bits of element i.
+template <uint32_t T>
+__device__ __forceinline__ uint32_t elem_bits(const void* p, uint64_t i) {
+  if constexpr (T == kGradF32)
+    return static_cast<const uint32_t*>(p)[i];
+  else
+    return static_cast<const uint16_t*>(p)[i];
+}
+
+// 8 elements as they lie in memory, kept packed while loads are in flight.
 template <uint32_t T>
 struct Raw {
-  uint4 r;
-  __device__ __forceinline__ void zero() { r = make_uint4(0u, 0u, 0u, 0u); }
+  static constexpr uint32_t kWords = kVecBytes<T> / 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  // One load of a vector on its own size's boundary.
   __device__ __forceinline__ void load(const void* p) {
-    r = __ldcg(static_cast<const uint4*>(p));
+    if constexpr (T == kGradF32) {
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                     "=r"(w[6]), "=r"(w[7])
+                   : "l"(p)
+                   : "memory");
+    } else {
+      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                   : "l"(p)
+                   : "memory");
+    }
+  }
+  // A vector at any element's address: the 16-byte blocks that hold it (the
+  // neighbouring threads read the same blocks: L1), and its words shifted out.
+  // The caller makes sure that the blocks lie within the tensor.
+  __device__ __forceinline__ void load_shifted(const uint8_t* p) {
+    const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uint4* block = reinterpret_cast<const uint4*>(p - d);
+    constexpr uint32_t kBlocks = kWords / 4 + 1;
+    uint32_t b[kBlocks * 4];
+#pragma unroll
+    for (uint32_t i = 0; i < kBlocks; ++i) {
+      const uint4 r = block[i];
+      b[4 * i] = r.x;
+      b[4 * i + 1] = r.y;
+      b[4 * i + 2] = r.z;
+      b[4 * i + 3] = r.w;
+    }
+    // d bytes = (d / 8) pairs of words, (d / 4) % 2 words, (d / 2) % 2 halves.
+    if (d & 8u) {
+#pragma unroll
+      for (uint32_t i = 0; i < kWords + 2; ++i) b[i] = b[i + 2 < kBlocks * 4 ? i + 2 : i];
+    }
+    if (d & 4u) {
+#pragma unroll
+      for (uint32_t i = 0; i < kWords + 1; ++i) b[i] = b[i + 1];
+    }
+    const uint32_t bits = (d & 2u) * 8u;
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i)
+      w[i] = T == kGradF32 ? b[i] : __funnelshift_r(b[i], b[i + 1], bits);
+  }
+  __device__ __forceinline__ void set(uint32_t j, uint32_t bits) {
+    if constexpr (T == kGradF32)
+      w[j] = bits;
+    else
+      w[j / 2] = (j & 1u) ? (w[j / 2] & 0xffffu) | (bits << 16) : (w[j / 2] & 0xffff0000u) | bits;
   }
   __device__ __forceinline__ void unpack(float (&x)[8]) const {
-    if constexpr (T == kGradBf16) {
-      unpack_bf16x8(r, x);
+    if constexpr (T == kGradF32) {
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+    } else if constexpr (T == kGradBf16) {
+      unpack_bf16x8(make_uint4(w[0], w[1], w[2], w[3]), x);
     } else {
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
         __half2 h;
@@ -49,75 +130,31 @@ struct Raw {
       }
     }
   }
-  // Largest magnitude so far, two 16-bit lanes: without their sign, finite
-  // values, infinity and NaN order as integers.
+  // Largest magnitude so far (16-bit types: in two lanes): without their sign,
+  // finite values, infinity and NaN order as integers.
   __device__ __forceinline__ void top(uint32_t& m) const {
-    m = __vmaxu2(m, r.x & 0x7fff7fffu);
-    m = __vmaxu2(m, r.y & 0x7fff7fffu);
-    m = __vmaxu2(m, r.z & 0x7fff7fffu);
-    m = __vmaxu2(m, r.w & 0x7fff7fffu);
-  }
-};
-template <>
-struct Raw<kGradF32> {
-  uint4 a, b;
-  __device__ __forceinline__ void zero() { a = b = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void load(const void* p) {
-    a = __ldcg(static_cast<const uint4*>(p));
-    b = __ldcg(static_cast<const uint4*>(p) + 1);
-  }
-  __device__ __forceinline__ void unpack(float (&x)[8]) const {
-    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y);
-    x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-    x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y);
-    x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
-  }
-  __device__ __forceinline__ void top(uint32_t& m) const {
-    m = max(m, max(max(a.x & 0x7fffffffu, a.y & 0x7fffffffu),
-                   max(a.z & 0x7fffffffu, a.w & 0x7fffffffu)));
-    m = max(m, max(max(b.x & 0x7fffffffu, b.y & 0x7fffffffu),
-                   max(b.z & 0x7fffffffu, b.w & 0x7fffffffu)));
+    if constexpr (T == kGradF32) {
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
+    } else {
+      m = __vimax3_u16x2(m, w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
+      m = __vimax3_u16x2(m, w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu);
+    }
   }
 };
 
-__device__ __forceinline__ uint32_t elem_bytes(uint32_t type) { return type == kGradF32 ? 4u : 2u; }
-
-// Bits of |x| for element i, in the form Raw<T>::top keeps (16-bit types: the low lane).
-template <uint32_t T>
-__device__ __forceinline__ uint32_t elem_bits(const void* p, uint64_t i) {
-  if constexpr (T == kGradF32)
-    return static_cast<const uint32_t*>(p)[i];
-  else
-    return static_cast<const uint16_t*>(p)[i];
-}
-template <uint32_t T>
-__device__ __forceinline__ float from_bits(uint32_t b) {
-  if constexpr (T == kGradF32)
-    return __uint_as_float(b);
-  else if constexpr (T == kGradBf16)
-    return __uint_as_float(b << 16);
-  else
-    return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
-}
-
-// A thread's two 16-bit lanes (or one f32) of largest magnitude, as f32 bits.
+// A thread's largest magnitude as f32 bits.
 template <uint32_t T>
 __device__ __forceinline__ uint32_t top_f32(uint32_t m) {
-  if constexpr (T == kGradF32) {
+  if constexpr (T == kGradF32)
     return m;
-  } else {
-    const uint32_t h = max(m & 0xffffu, m >> 16);
-    return __float_as_uint(from_bits<T>(h)) & 0x7fffffffu;
-  }
+  else
+    return __float_as_uint(from_bits<T>(max(m & 0xffffu, m >> 16))) & 0x7fffffffu;
 }
 
-template <uint32_t T>
-constexpr uint32_t kSize = T == kGradF32 ? 4u : 2u;
-
-// Where a unit's elements lie.  `at(e)` is the address of element e of the unit
-// counted in row-major order; for a vector-aligned tensor, e a multiple of 8,
-// all 8 elements are one run.
-template <uint32_t T>
+// ---- where a unit's elements lie -------------------------------------------------
+// Element e of the unit in row-major order; a pitched tensor's rows are walked
+// with one division per run.
 struct Place {
   const uint8_t* base;
   uint64_t first;  // pitched: the unit's first element within its tensor
@@ -125,7 +162,7 @@ struct Place {
   bool pitched;
   __device__ __forceinline__ Place(const GradUnit& u, const GradTensor* tensors,
                                    uint32_t unit_elems)
-      : base(static_cast<const uint8_t*>(u.ptr)), first(0), columns(1), stride(0),
+      : base(static_cast<const uint8_t*>(u.ptr)), first(0), columns(0), stride(0),
         pitched((u.flags & kGradPitched) != 0u) {
     if (pitched) {
       const GradTensor* t = tensors + u.tensor;
@@ -134,20 +171,56 @@ struct Place {
       first = uint64_t(u.index) * unit_elems;
     }
   }
-  __device__ __forceinline__ uint64_t element(uint32_t e) const {
+  // Index in memory of element e, and the elements of its row from there on.
+  __device__ __forceinline__ uint64_t index(uint32_t e, uint64_t& run) const {
+    run = ~uint64_t(0);
     if (!pitched) return e;
     const uint64_t k = first + e;
-    uint64_t row;
-    if ((k | columns) <= 0xffffffffull)
-      row = static_cast<uint32_t>(k) / static_cast<uint32_t>(columns);
-    else
-      row = k / columns;
-    return row * stride + (k - row * columns);
+    const uint64_t row = (k | columns) <= 0xffffffffull
+                             ? uint64_t(static_cast<uint32_t>(k) / static_cast<uint32_t>(columns))
+                             : k / columns;
+    const uint64_t col = k - row * columns;
+    run = columns - col;
+    return row * stride + col;
   }
-  __device__ __forceinline__ const void* at(uint32_t e) const {
-    return base + element(e) * kSize<T>;
+  // The next element's index.
+  __device__ __forceinline__ void next(uint64_t& i, uint64_t& run) const {
+    ++i;
+    if (--run == 0u) {
+      i += stride - columns;
+      run = columns;
+    }
+  }
+  // The address of vector-aligned element e.
+  template <uint32_t T>
+  __device__ __forceinline__ uint8_t* vector_at(uint32_t e) const {
+    uint64_t run;
+    return const_cast<uint8_t*>(base) + index(e, run) * kSize<T>;
   }
 };
+
+// Elements e .. e + n - 1 (n <= 8) one by one, the rest zero: of rows, and of
+// contiguous memory.
+template <uint32_t T>
+__device__ __forceinline__ void gather(Raw<T>& raw, const Place& place, uint32_t e, uint32_t n) {
+  raw.zero();
+  uint64_t run;
+  uint64_t i = place.index(e, run);
+#pragma unroll
+  for (uint32_t j = 0; j < kVec; ++j) {
+    if (j < n) {
+      raw.set(j, elem_bits<T>(place.base, i));
+      place.next(i, run);
+    }
+  }
+}
+template <uint32_t T>
+__device__ __forceinline__ void gather_flat(Raw<T>& raw, const uint8_t* p, uint32_t n) {
+  raw.zero();
+#pragma unroll
+  for (uint32_t j = 0; j < kVec; ++j)
+    if (j < n) raw.set(j, elem_bits<T>(p, j));
+}
 
 __device__ __forceinline__ GradUnit load_unit(const GradUnit* units, uint32_t i) {
   GradUnit u;
@@ -158,71 +231,135 @@ __device__ __forceinline__ GradUnit load_unit(const GradUnit* units, uint32_t i)
 }
 
 // ---- norm ----------------------------------------------------------------------
-// The fixed tree of one unit: thread t owns the unit's 8-element vectors t,
-// t + 256, ...; a vector's unscaled squares are added pairwise in f32
-// (add_squares8) and the sums in order to the thread's f64 accumulator; elements
-// past the end count as +0.0.  The block folds as the flat norm's does.
-template <uint32_t T, bool kMul>
-__device__ __forceinline__ double unit_squares(const GradUnit& u, const GradTensor* tensors,
-                                               uint32_t unit_elems, const ScaleInfo& sc,
-                                               uint32_t& top) {
-  constexpr uint32_t kBatch = T == kGradF32 ? 4 : 8;  // 128 bytes of loads in flight per thread
-  const Place<T> place(u, tensors, unit_elems);
-  const uint32_t whole = u.count / kVec;
+// Squares are formed of the stored values times a power of two: 1 for loss
+// scales of 1 to 2^20, else the one next to 1 / scale, so that they are in the
+// range of the unscaled values' (within 2^40) without a division per element;
+// the finalize divides the f64 sum by the exact (scale * factor)^2.
+__device__ __forceinline__ float square_factor(float scale) {
+  if (scale >= 1.0f && scale <= 1048576.0f) return 1.0f;
+  const uint32_t e = (__float_as_uint(scale) >> 23) & 0xffu;
+  const uint32_t inv = e >= 253u ? 1u : 254u - e;  // 2^-126 at the least
+  return __uint_as_float((e == 0u ? 254u : inv) << 23);
+}
+
+// Two f32 operations in one instruction, each rounded alone.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// The term of one 8-element vector: x0^2 + x1^2 + x2^2 + x3^2 and x4^2 + ... + x7^2
+// side by side, each by a product and three fused multiply-adds, their f32 sum,
+// then the lane's f64.  At most 5 roundings of non-negative terms: 5 * 2^-24
+// relative.
+template <bool kFactor>
+__device__ __forceinline__ double add_vector(double acc, const float (&x)[8], float factor) {
+  uint64_t s = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    uint64_t q = pair(x[j], x[j + 4]);
+    if constexpr (kFactor) q = mul2(q, pair(factor, factor));
+    s = j == 0 ? mul2(q, q) : fma2(q, q, s);
+  }
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(s));
+  return __dadd_rn(acc, static_cast<double>(__fadd_rn(lo, hi)));
+}
+
+// The fixed tree of one unit: thread t owns the unit's vectors t, t + 256, ...
+// (elements past the end count as +0.0); the block folds as the flat norm's does.
+template <uint32_t T, bool kFactor>
+struct Squares {
   double acc = 0.0;
-  uint32_t m = 0u;
-  if (u.flags & kGradVector) {
-    for (uint32_t v0 = threadIdx.x; v0 < whole; v0 += kBatch * kListThreads) {
+  uint32_t top = 0u;
+  float factor;
+  __device__ __forceinline__ void take(const Raw<T>& raw) {
+    float x[8];
+    raw.unpack(x);
+    raw.top(top);
+    acc = add_vector<kFactor>(acc, x, factor);
+  }
+};
+
+template <uint32_t T, bool kFactor>
+__device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint8_t* base,
+                                             uint32_t count) {
+  constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;  // 64 bytes of loads per thread in flight
+  constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
+  const uint32_t whole = count / kVec;
+  uint32_t v = threadIdx.x;
+  if (reinterpret_cast<uintptr_t>(base) % kVecBytes<T> == 0u) {
+    const uint8_t* p = base + v * kVecBytes<T>;
+    for (; v + (kBatch - 1) * kListThreads < whole; v += kBatch * kListThreads) {
       Raw<T> raw[kBatch];
 #pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        const uint32_t v = v0 + b * kListThreads;
-        if (v < whole)
-          raw[b].load(place.at(v * kVec));
-        else
-          raw[b].zero();
-      }
+      for (uint32_t b = 0; b < kBatch; ++b) raw[b].load(p + b * kStep);
+      p += kBatch * kStep;
 #pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        float x[8];
-        raw[b].unpack(x);
-        raw[b].top(m);
-        acc = add_squares8<kMul>(acc, x, sc);
-      }
+      for (uint32_t b = 0; b < kBatch; ++b) sq.take(raw[b]);
+    }
+    for (; v < whole; v += kListThreads, p += kStep) {
+      Raw<T> raw;
+      raw.load(p);
+      sq.take(raw);
     }
   } else {
-    for (uint32_t v = threadIdx.x; v < whole; v += kListThreads) {
-      float x[8];
-      uint32_t bits[8];
-#pragma unroll
-      for (uint32_t j = 0; j < kVec; ++j)
-        bits[j] = elem_bits<T>(place.base, place.element(v * kVec + j));
-#pragma unroll
-      for (uint32_t j = 0; j < kVec; ++j) {
-        x[j] = from_bits<T>(bits[j]);
-        m = max(m, bits[j] & (T == kGradF32 ? 0x7fffffffu : 0x7fffu));
-      }
-      acc = add_squares8<kMul>(acc, x, sc);
-    }
-  }
-  // The last, partial vector.
-  const uint32_t rest = u.count - whole * kVec;
-  if (rest && threadIdx.x == whole % kListThreads) {
-    float x[8];
-#pragma unroll
-    for (uint32_t j = 0; j < kVec; ++j) {
-      const uint32_t bits =
-          j < rest ? elem_bits<T>(place.base, place.element(whole * kVec + j)) : 0u;
-      x[j] = from_bits<T>(bits);
-      if constexpr (T == kGradF32)
-        m = max(m, bits & 0x7fffffffu);
+    // Off the boundaries: the first and the last vector, whose blocks can reach
+    // beyond the tensor, element by element.
+    for (; v < whole; v += kListThreads) {
+      Raw<T> raw;
+      if (v > 0u && v + 1u < whole)
+        raw.load_shifted(base + v * kVecBytes<T>);
       else
-        m = __vmaxu2(m, bits & 0x7fffu);
+        gather_flat(raw, base + v * kVecBytes<T>, kVec);
+      sq.take(raw);
     }
-    acc = add_squares8<kMul>(acc, x, sc);
   }
-  top = top_f32<T>(m);
-  return acc;
+  if (threadIdx.x == whole % kListThreads && count % kVec) {
+    Raw<T> raw;
+    gather_flat(raw, base + whole * kVecBytes<T>, count % kVec);
+    sq.take(raw);
+  }
+}
+
+template <uint32_t T, bool kFactor>
+__device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, const Place& place,
+                                            uint32_t count, bool vector) {
+  for (uint32_t e = threadIdx.x * kVec; e < count; e += kListThreads * kVec) {
+    Raw<T> raw;
+    if (vector)
+      raw.load(place.vector_at<T>(e));
+    else
+      gather(raw, place, e, count - e < kVec ? count - e : kVec);
+    sq.take(raw);
+  }
+}
+
+// kRows: the list has pitched tensors.  The kernels without them need fewer
+// registers, so more of their loads are in flight.
+template <uint32_t T, bool kFactor, bool kRows>
+__device__ __forceinline__ double unit_squares(const GradUnit& u, const GradTensor* tensors,
+                                               uint32_t unit_elems, float factor,
+                                               uint32_t& top) {
+  Squares<T, kFactor> sq;
+  sq.factor = factor;
+  if (kRows && (u.flags & kGradPitched))
+    row_squares(sq, Place(u, tensors, unit_elems), u.count, (u.flags & kGradVector) != 0u);
+  else
+    flat_squares(sq, static_cast<const uint8_t*>(u.ptr), u.count);
+  top = top_f32<T>(sq.top);
+  return sq.acc;
 }
 
 // Folds (sum, top) over the block; results valid in thread 0.
@@ -254,69 +391,79 @@ __device__ __forceinline__ void fold_block(double& v, uint32_t& top, double* s_s
   }
 }
 
-template <bool kMul>
+__device__ __forceinline__ void store_partial(const GradPartial* partials, double sum,
+                                              uint32_t top) {
+  *reinterpret_cast<uint4*>(const_cast<GradPartial*>(partials)) =
+      make_uint4(uint32_t(__double2loint(sum)), uint32_t(__double2hiint(sum)), top, 0u);
+}
+
+template <bool kFactor, bool kRows>
 __device__ __forceinline__ double unit_squares_any(const GradUnit& u, const GradTensor* tensors,
-                                                   uint32_t unit_elems, const ScaleInfo& sc,
+                                                   uint32_t unit_elems, float factor,
                                                    uint32_t& top) {
   switch (u.flags & kGradTypeMask) {
-    case kGradF32: return unit_squares<kGradF32, kMul>(u, tensors, unit_elems, sc, top);
-    case kGradBf16: return unit_squares<kGradBf16, kMul>(u, tensors, unit_elems, sc, top);
-    default: return unit_squares<kGradF16, kMul>(u, tensors, unit_elems, sc, top);
+    case kGradF32:
+      return unit_squares<kGradF32, kFactor, kRows>(u, tensors, unit_elems, factor, top);
+    case kGradBf16:
+      return unit_squares<kGradBf16, kFactor, kRows>(u, tensors, unit_elems, factor, top);
+    default: return unit_squares<kGradF16, kFactor, kRows>(u, tensors, unit_elems, factor, top);
   }
 }
 
-__global__ void __launch_bounds__(kListThreads)
+template <bool kRows>
+__global__ void __launch_bounds__(kListThreads, kRows ? 5 : 8)
     list_norm_kernel(GradListView list, float scale, const DeviceScaler* scaler,
-                     GradPartials part) {
+                     GradPartial* partials) {
   __shared__ double s_sum[kListThreads / 32];
   __shared__ uint32_t s_top[kListThreads / 32];
-  pdl_trigger();
   const GradUnit u = load_unit(list.units, blockIdx.x);
-  const ScaleInfo sc = decode_scale(scaler ? scaler->scale : scale);
+  // The kernels behind may start to read gradients once all blocks are here, so
+  // their producers must be done by then: wait first.
+  pdl_wait();
+  pdl_trigger();
+  const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
-  double sum = sc.mul ? unit_squares_any<true>(u, list.tensors, list.unit_elems, sc, top)
-                      : unit_squares_any<false>(u, list.tensors, list.unit_elems, sc, top);
+  double sum = factor == 1.0f
+                   ? unit_squares_any<false, kRows>(u, list.tensors, list.unit_elems, factor, top)
+                   : unit_squares_any<true, kRows>(u, list.tensors, list.unit_elems, factor, top);
   fold_block<kListThreads>(sum, top, s_sum, s_top);
-  if (threadIdx.x == 0) {
-    part.sums[blockIdx.x] = sum;
-    part.tops[blockIdx.x] = top;
-  }
+  if (threadIdx.x == 0) store_partial(partials + blockIdx.x, sum, top);
 }
 
-// Thread t adds partials begin + t, begin + t + 512, ... in order, 8 loads in
-// flight; then the block folds.  Valid in thread 0.
-__device__ __forceinline__ void sum_partials(const GradPartials& part, uint32_t begin,
-                                             uint32_t count, double& v, uint32_t& top,
+// Thread t adds partials t, t + 1024, ... of a run in order, 8 loads in flight;
+// then the block folds.  The sum is that of the unscaled squares.  Valid in
+// thread 0.
+__device__ __forceinline__ void sum_partials(const GradPartial* partials, uint32_t count,
+                                             float scale, double& v, uint32_t& top,
                                              double* s_sum, uint32_t* s_top) {
   v = 0.0;
   top = 0u;
   for (uint32_t i0 = threadIdx.x; i0 < count; i0 += 8 * kFinalThreads) {
-    double q[8];
-    uint32_t w[8];
+    uint4 q[8];
 #pragma unroll
     for (uint32_t b = 0; b < 8; ++b) {
       const uint32_t i = i0 + b * kFinalThreads;
-      q[b] = i < count ? __ldcg(part.sums + begin + i) : 0.0;
-      w[b] = i < count ? __ldcg(part.tops + begin + i) : 0u;
+      q[b] = i < count ? __ldcg(reinterpret_cast<const uint4*>(partials + i))
+                       : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (uint32_t b = 0; b < 8; ++b) {
-      v = __dadd_rn(v, q[b]);
-      top = max(top, w[b]);
+      v = __dadd_rn(v, __hiloint2double(int(q[b].y), int(q[b].x)));
+      top = max(top, q[b].z);
     }
   }
   fold_block<kFinalThreads>(v, top, s_sum, s_top);
+  const double s = __dmul_rn(static_cast<double>(scale), static_cast<double>(square_factor(scale)));
+  v = __ddiv_rn(v, __dmul_rn(s, s));
 }
 
 __device__ __forceinline__ float unscaled_top(uint32_t top, float scale) {
-  const ScaleInfo sc = decode_scale(scale);
-  const float x = __uint_as_float(top);
-  return sc.mul ? unscale<true>(x, sc) : unscale<false>(x, sc);
+  return __fdiv_rn(__uint_as_float(top), scale);
 }
 
 __global__ void __launch_bounds__(kFinalThreads)
-    list_finalize_kernel(GradListView list, GradPartials part, float scale, float max_norm,
-                         int kind, GradListOut out) {
+    list_finalize_kernel(GradListView list, const GradPartial* partials, float scale,
+                         float max_norm, int kind, GradListOut out) {
   __shared__ double s_sum[kFinalThreads / 32];
   __shared__ uint32_t s_top[kFinalThreads / 32];
   pdl_trigger();
@@ -331,7 +478,7 @@ __global__ void __launch_bounds__(kFinalThreads)
   pdl_wait();
   double sum;
   uint32_t top;
-  sum_partials(part, begin, count, sum, top, s_sum, s_top);
+  sum_partials(partials + begin, count, scale, sum, top, s_sum, s_top);
   if (threadIdx.x != 0) return;
   const float largest = unscaled_top(top, scale);
   const float norm = kind != 0 ? largest : __double2float_rn(__dsqrt_rn(sum));
@@ -340,33 +487,33 @@ __global__ void __launch_bounds__(kFinalThreads)
     if (out.tensor_max) out.tensor_max[blockIdx.x - 1u] = largest;
     return;
   }
-  const bool bad = !finite_f32(norm) || !finite_f32(largest);
   // The flat step's formula: the sum rounded once to f32, f32 root and quotient.
   const float root = kind != 0 ? largest : __fsqrt_rn(__double2float_rn(sum));
+  const bool bad = !finite_f32(norm) || !finite_f32(largest) || !finite_f32(root);
   float clip = 1.0f;
-  if (bad || !finite_f32(root))
+  if (bad)
     clip = 0.0f;
   else if (root > 0.0f)
     clip = fminf(__fdiv_rn(max_norm, root), 1.0f);
   out.result[0] = norm;
   out.result[1] = clip;
   out.result[2] = largest;
-  out.result[3] = bad || !finite_f32(root) ? 1.0f : 0.0f;
+  out.result[3] = bad ? 1.0f : 0.0f;
   if (out.sum_squares) *out.sum_squares = sum;
 }
 
 __global__ void __launch_bounds__(kFinalThreads)
-    list_decide_kernel(GradListView list, GradPartials part, DeviceScaler* scaler,
+    list_decide_kernel(GradListView list, const GradPartial* partials, DeviceScaler* scaler,
                        DeviceStepState* st, FinalizeParams fp) {
   __shared__ double s_sum[kFinalThreads / 32];
   __shared__ uint32_t s_top[kFinalThreads / 32];
   pdl_trigger();
   pdl_wait();
+  const float scale = fp.dynamic ? scaler->scale : fp.static_scale;
   double sum;
   uint32_t top;
-  sum_partials(part, 0u, list.n_units, sum, top, s_sum, s_top);
+  sum_partials(partials, list.n_units, scale, sum, top, s_sum, s_top);
   if (threadIdx.x != 0) return;
-  const float scale = fp.dynamic ? scaler->scale : fp.static_scale;
   const uint32_t nonfinite =
       !isfinite(sum) || !finite_f32(unscaled_top(top, scale)) ? 1u : 0u;
   const StepDecision d =
@@ -377,10 +524,22 @@ __global__ void __launch_bounds__(kFinalThreads)
 
 // ---- clip ----------------------------------------------------------------------
 template <uint32_t T>
+__device__ __forceinline__ uint32_t to_bits(float y) {
+  if constexpr (T == kGradF32)
+    return __float_as_uint(y);
+  else if constexpr (T == kGradBf16)
+    return __bfloat16_as_ushort(__float2bfloat16_rn(y));
+  else
+    return __half_as_ushort(__float2half_rn(y));
+}
+// A vector on its own size's boundary; written once, so first to leave the L2.
+template <uint32_t T>
 __device__ __forceinline__ void store8(void* p, const float (&y)[8]) {
   if constexpr (T == kGradF32) {
-    __stcs(static_cast<float4*>(p), make_float4(y[0], y[1], y[2], y[3]));
-    __stcs(static_cast<float4*>(p) + 1, make_float4(y[4], y[5], y[6], y[7]));
+    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p),
+                 "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]),
+                 "f"(y[7])
+                 : "memory");
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -397,222 +556,408 @@ __device__ __forceinline__ void store8(void* p, const float (&y)[8]) {
   }
 }
 template <uint32_t T>
-__device__ __forceinline__ void store1(void* p, float y) {
+__device__ __forceinline__ void store1(void* p, uint64_t i, float y) {
   if constexpr (T == kGradF32)
-    *static_cast<float*>(p) = y;
-  else if constexpr (T == kGradBf16)
-    *static_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(y);
+    static_cast<float*>(p)[i] = y;
   else
-    *static_cast<__half*>(p) = __float2half_rn(y);
+    static_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(to_bits<T>(y));
 }
 
-__device__ __forceinline__ float clipped(float x, const ScaleInfo& sc, float clip) {
-  return __fmul_rn(sc.mul ? unscale<true>(x, sc) : unscale<false>(x, sc), clip);
+// The factor of the clip call, clip / scale rounded to f32: one product per
+// element.  Where the quotient is no normal f32 (extreme scales) it is split
+// into a normal factor and a power of two.
+struct ClipFactor {
+  float factor, power;
+  __device__ __forceinline__ ClipFactor(float clip, float scale) {
+    power = 1.0f;
+    factor = __fdiv_rn(clip, scale);
+    if (factor < 1.17549435e-38f && clip > 0.0f) {
+      power = 5.42101086e-20f;  // 2^-64
+      factor = __fdiv_rn(__fmul_rn(clip, 1.84467441e19f), scale);
+    } else if (!finite_f32(factor)) {
+      power = 1.84467441e19f;  // 2^64
+      factor = __fdiv_rn(__fmul_rn(clip, 5.42101086e-20f), scale);
+    }
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float y = __fmul_rn(x, factor);
+    return power == 1.0f ? y : __fmul_rn(y, power);
+  }
+};
+
+// Elements before the first vector boundary of p.
+template <uint32_t T>
+__device__ __forceinline__ uint32_t peel_of(const void* p, uint32_t count) {
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) % kVecBytes<T>;
+  const uint32_t n = (kVecBytes<T> - off) % kVecBytes<T> / kSize<T>;
+  return n < count ? n : count;
 }
 
-// Reads and writes element by element of the same index; in place each element
-// is written by the thread that read it.
 template <uint32_t T, uint32_t O>
+__device__ __forceinline__ void clip_raw(const Raw<T>& raw, const ClipFactor& f, void* to) {
+  float x[8];
+  raw.unpack(x);
+#pragma unroll
+  for (uint32_t j = 0; j < kVec; ++j) x[j] = f(x[j]);
+  store8<O>(to, x);
+}
+
+// Waits for the norm, once per block; false when a gradient is not finite,
+// which leaves the outputs alone.
+__device__ __forceinline__ bool clip_ready(const float* result, bool& waited) {
+  if (!waited) pdl_wait();
+  waited = true;
+  return __ldcg(result + 3) == 0.0f;
+}
+
+// One unit of the clip, each element read and written by the same thread.
+// Contiguous on both sides: vectors start at the output's boundaries, and the
+// input is shifted where it lies off them.
+template <uint32_t T, uint32_t O>
+__device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint32_t count,
+                                          float scale, const float* result, bool& waited) {
+  constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
+  constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
+  const uint32_t peel = peel_of<O>(dst, count);
+  const uint8_t* from = src + peel * kSize<T>;
+  uint8_t* to = dst + peel * kSize<O>;
+  const uint32_t whole = (count - peel) / kVec;
+  uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
+  uint32_t v = threadIdx.x;
+  if (reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
+    Raw<T> raw[kBatch];
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b)  // on their way while the norm is finished
+      if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep);
+    if (!clip_ready(result, waited)) return;
+    const ClipFactor f(__ldcg(result + 1), scale);
+    while (v < whole) {
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b)
+        if (v + b * kListThreads < whole)
+          clip_raw<T, O>(raw[b], f, to + (v + b * kListThreads) * kVecBytes<O>);
+      v += kBatch * kListThreads;
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b)
+        if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep);
+    }
+  } else {
+    if (!clip_ready(result, waited)) return;
+    const ClipFactor f(__ldcg(result + 1), scale);
+    // The blocks of the first and the last vector can reach beyond the tensor.
+    for (v += 1u; v + 1u < whole; v += kListThreads) {
+      Raw<T> raw;
+      raw.load_shifted(from + v * kVecBytes<T>);
+      clip_raw<T, O>(raw, f, to + v * kVecBytes<O>);
+    }
+    if (whole) {
+      head += kVec;
+      tail = whole > 1u ? tail - kVec : head;
+    }
+  }
+  const ClipFactor f(__ldcg(result + 1), scale);
+  for (uint32_t e = threadIdx.x; e < head + (count - tail); e += kListThreads) {
+    const uint32_t i = e < head ? e : tail + (e - head);
+    store1<O>(dst, i, f(from_bits<T>(elem_bits<T>(src, i))));
+  }
+}
+
+// Rows on either side: whole vectors where both sides have them, else 8 elements
+// a thread.
+template <uint32_t T, uint32_t O>
+__device__ __forceinline__ void clip_rows(const Place& src, const Place& dst, uint32_t count,
+                                          bool vectors, float scale, const float* result,
+                                          bool& waited) {
+  if (!clip_ready(result, waited)) return;
+  const ClipFactor f(__ldcg(result + 1), scale);
+  uint32_t e = threadIdx.x * kVec;
+  if (vectors) {
+    for (; e + kVec <= count; e += kListThreads * kVec) {
+      Raw<T> raw;
+      raw.load(src.vector_at<T>(e));
+      clip_raw<T, O>(raw, f, dst.vector_at<O>(e));
+    }
+  }
+  for (; e < count; e += kListThreads * kVec) {
+    uint64_t run_i, run_o;
+    uint64_t i = src.index(e, run_i), k = dst.index(e, run_o);
+    for (uint32_t j = 0; j < kVec && e + j < count; ++j) {
+      store1<O>(const_cast<uint8_t*>(dst.base), k, f(from_bits<T>(elem_bits<T>(src.base, i))));
+      src.next(i, run_i);
+      dst.next(k, run_o);
+    }
+  }
+}
+
+template <uint32_t T, uint32_t O, bool kRows>
 __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
                                           const GradListView& list, const GradListView& out,
-                                          const ScaleInfo& sc, const float* result,
-                                          bool in_place) {
-  constexpr uint32_t kBatch = T == kGradF32 ? 4 : 8;
-  const Place<T> src(u, list.tensors, list.unit_elems);
-  const Place<O> dst(o, out.tensors, out.unit_elems);
-  const uint32_t whole = (u.flags & o.flags & kGradVector) ? u.count / kVec : 0u;
-  Raw<T> raw[kBatch];
+                                          float scale, const float* result, bool& waited) {
+  if (kRows && ((u.flags | o.flags) & kGradPitched))
+    clip_rows<T, O>(Place(u, list.tensors, list.unit_elems), Place(o, out.tensors, out.unit_elems),
+                    u.count, (u.flags & o.flags & kGradVector) != 0u, scale, result, waited);
+  else
+    clip_flat<T, O>(static_cast<const uint8_t*>(u.ptr),
+                    static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale, result,
+                    waited);
+}
+
+// kOut: the output type (units written in another one are left to the launch for
+// theirs), or in place.  All nine pairs of types in one kernel would spill.
+constexpr uint32_t kOutSame = 3u;
+template <uint32_t kOut, bool kRows>
+__global__ void __launch_bounds__(kListThreads, kRows ? 2 : 4)
+    list_clip_kernel(GradListView list, GradListView out, float scale, const float* result) {
+  constexpr bool kSame = kOut == kOutSame;
   bool waited = false;
-  float clip = 0.0f;
-  for (uint32_t v0 = threadIdx.x; v0 < whole || !waited; v0 += kBatch * kListThreads) {
-#pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) {
-      const uint32_t v = v0 + b * kListThreads;
-      if (v < whole) raw[b].load(src.at(v * kVec));
-    }
-    if (!waited) {
-      // The first loads are on their way; nothing is written before the clip
-      // scale is there.
-      pdl_wait();
-      waited = true;
-      clip = __ldcg(result + 1);
-      const bool bad = __ldcg(result + 3) != 0.0f;
-      // A non-finite gradient leaves the outputs alone; so does a product with
-      // one and one in place, which changes no bit.
-      if (bad || (in_place && clip == 1.0f && sc.s == 1.0f)) return;
-    }
-#pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) {
-      const uint32_t v = v0 + b * kListThreads;
-      if (v < whole) {
-        float x[8];
-        raw[b].unpack(x);
-#pragma unroll
-        for (uint32_t j = 0; j < kVec; ++j) x[j] = clipped(x[j], sc, clip);
-        store8<O>(const_cast<void*>(dst.at(v * kVec)), x);
-      }
-    }
+  // In place with a loss scale of one there may be nothing to do: look before
+  // anything is loaded.
+  if (kSame && scale == 1.0f) {
+    pdl_wait();
+    waited = true;
+    if (__ldcg(result + 1) == 1.0f || __ldcg(result + 3) != 0.0f) return;
   }
-  for (uint32_t e = whole * kVec + threadIdx.x; e < u.count; e += kListThreads) {
-    const float x = from_bits<T>(elem_bits<T>(src.base, src.element(e)));
-    store1<O>(const_cast<void*>(dst.at(e)), clipped(x, sc, clip));
-  }
-}
-
-template <uint32_t T>
-__device__ __forceinline__ void clip_unit_to(const GradUnit& u, const GradUnit& o,
-                                             const GradListView& list, const GradListView& out,
-                                             const ScaleInfo& sc, const float* result,
-                                             bool in_place) {
-  switch (o.flags & kGradTypeMask) {
-    case kGradF32: return clip_unit<T, kGradF32>(u, o, list, out, sc, result, in_place);
-    case kGradBf16: return clip_unit<T, kGradBf16>(u, o, list, out, sc, result, in_place);
-    default: return clip_unit<T, kGradF16>(u, o, list, out, sc, result, in_place);
-  }
-}
-
-__global__ void __launch_bounds__(kListThreads)
-    list_clip_kernel(GradListView list, GradListView out, float scale, const float* result,
-                     bool in_place) {
   // From the end of the list to its start: the norm pass has read the end last,
   // so the part of the gradients that the L2 still holds is read first.
-  const uint32_t i = gridDim.x - 1u - blockIdx.x;
-  const GradUnit u = load_unit(list.units, i);
-  const GradUnit o = load_unit(out.units, i);
-  const ScaleInfo sc = decode_scale(scale);
-  switch (u.flags & kGradTypeMask) {
-    case kGradF32: return clip_unit_to<kGradF32>(u, o, list, out, sc, result, in_place);
-    case kGradBf16: return clip_unit_to<kGradBf16>(u, o, list, out, sc, result, in_place);
-    default: return clip_unit_to<kGradF16>(u, o, list, out, sc, result, in_place);
+  for (uint32_t b = blockIdx.x; b < list.n_units; b += gridDim.x) {
+    const uint32_t i = list.n_units - 1u - b;
+    const GradUnit u = load_unit(list.units, i);
+    const GradUnit o = kSame ? u : load_unit(out.units, i);
+    if (!kSame && (o.flags & kGradTypeMask) != kOut) continue;
+    switch (u.flags & kGradTypeMask) {
+      case kGradF32:
+        clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows>(u, o, list, out, scale, result,
+                                                            waited);
+        break;
+      case kGradBf16:
+        clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows>(u, o, list, out, scale, result,
+                                                              waited);
+        break;
+      default:
+        clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows>(u, o, list, out, scale, result,
+                                                            waited);
+        break;
+    }
   }
 }
 
 // ---- accumulate ------------------------------------------------------------------
-// acc[offset + e] = micro, or += micro (f32), and with kNorm the unit's partial of
-// the sums, in the tree of unit_squares over f32 values.
-template <uint32_t T, bool kNorm, bool kMul>
-__device__ __forceinline__ double accumulate_unit(const GradUnit& u, const GradListView& list,
-                                                  float* acc, bool overwrite,
-                                                  const ScaleInfo& sc, uint32_t& top) {
-  constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
-  const Place<T> src(u, list.tensors, list.unit_elems);
+__device__ __forceinline__ void load_acc(const float* p, float (&y)[8]) {
+  asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]), "=f"(y[4]), "=f"(y[5]),
+                 "=f"(y[6]), "=f"(y[7])
+               : "l"(p)
+               : "memory");
+}
+
+template <uint32_t T>
+__device__ __forceinline__ void add_raw(const Raw<T>& raw, const float (&old)[8], bool overwrite,
+                                        float* to) {
+  float y[8];
+  raw.unpack(y);
+  if (!overwrite) {
+#pragma unroll
+    for (uint32_t j = 0; j < kVec; ++j) y[j] = __fadd_rn(old[j], y[j]);
+  }
+  store8<kGradF32>(to, y);
+}
+template <uint32_t T>
+__device__ __forceinline__ void add_one(const void* src, uint64_t i, bool overwrite, float* to) {
+  const float x = from_bits<T>(elem_bits<T>(src, i));
+  *to = overwrite ? x : __fadd_rn(*to, x);
+}
+
+// acc[offset + e] = micro, or += micro (f32).  Vectors start at the
+// accumulator's boundaries; the input is shifted where it lies off them.
+template <uint32_t T>
+__device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, uint32_t count,
+                                                bool overwrite) {
+  constexpr uint32_t kBatch = 2;
+  const uint32_t peel = peel_of<kGradF32>(dst, count);
+  const uint8_t* from = src + peel * kSize<T>;
+  float* to = dst + peel;
+  const uint32_t whole = (count - peel) / kVec;
+  uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
+  if (reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
+    for (uint32_t v = threadIdx.x; v < whole; v += kBatch * kListThreads) {
+      Raw<T> raw[kBatch];
+      float old[kBatch][8];
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        const uint32_t i = v + b * kListThreads;
+        if (i < whole) {
+          raw[b].load(from + i * kVecBytes<T>);
+          if (!overwrite) load_acc(to + i * kVec, old[b]);
+        }
+      }
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        const uint32_t i = v + b * kListThreads;
+        if (i < whole) add_raw<T>(raw[b], old[b], overwrite, to + i * kVec);
+      }
+    }
+  } else {
+    // The blocks of the first and the last vector can reach beyond the tensor.
+    for (uint32_t v = threadIdx.x + 1u; v + 1u < whole; v += kListThreads) {
+      Raw<T> raw;
+      float old[8];
+      raw.load_shifted(from + v * kVecBytes<T>);
+      if (!overwrite) load_acc(to + v * kVec, old);
+      add_raw<T>(raw, old, overwrite, to + v * kVec);
+    }
+    if (whole) {
+      head += kVec;
+      tail = whole > 1u ? tail - kVec : head;
+    }
+  }
+  for (uint32_t e = threadIdx.x; e < head + (count - tail); e += kListThreads) {
+    const uint32_t i = e < head ? e : tail + (e - head);
+    add_one<T>(src, i, overwrite, dst + i);
+  }
+}
+
+template <uint32_t T>
+__device__ __forceinline__ void accumulate_rows(const Place& src, float* dst, uint32_t count,
+                                                bool vectors, bool overwrite) {
+  for (uint32_t e = threadIdx.x * kVec; e < count; e += kListThreads * kVec) {
+    if (vectors) {
+      Raw<T> raw;
+      float old[8];
+      raw.load(src.vector_at<T>(e));
+      if (!overwrite) load_acc(dst + e, old);
+      add_raw<T>(raw, old, overwrite, dst + e);
+    } else {
+      uint64_t run;
+      uint64_t i = src.index(e, run);
+      for (uint32_t j = 0; j < kVec && e + j < count; ++j) {
+        add_one<T>(src.base, i, overwrite, dst + e + j);
+        src.next(i, run);
+      }
+    }
+  }
+}
+
+template <uint32_t T, bool kRows>
+__device__ __forceinline__ void accumulate_unit(const GradUnit& u, const GradListView& list,
+                                                float* acc, bool overwrite) {
   float* dst = acc + u.offset;
-  const bool vector = (u.flags & kGradVector) && u.offset % 4u == 0u;
+  if (kRows && (u.flags & kGradPitched))
+    accumulate_rows<T>(Place(u, list.tensors, list.unit_elems), dst, u.count,
+                       (u.flags & kGradVector) && reinterpret_cast<uintptr_t>(dst) % 32u == 0u,
+                       overwrite);
+  else
+    accumulate_flat<T>(static_cast<const uint8_t*>(u.ptr), dst, u.count, overwrite);
+}
+
+template <bool kRows>
+__global__ void __launch_bounds__(kListThreads, 4)
+    list_accumulate_kernel(GradListView list, float* acc, int overwrite) {
+  const GradUnit u = load_unit(list.units, blockIdx.x);
+  pdl_wait();
+  pdl_trigger();  // whoever starts early waits for this kernel before it reads
+  switch (u.flags & kGradTypeMask) {
+    case kGradF32: return accumulate_unit<kGradF32, kRows>(u, list, acc, overwrite != 0);
+    case kGradBf16: return accumulate_unit<kGradBf16, kRows>(u, list, acc, overwrite != 0);
+    default: return accumulate_unit<kGradF16, kRows>(u, list, acc, overwrite != 0);
+  }
+}
+
+// The last micro-batch: accumulates the unit's vectors in the tree's order (from
+// its first element, the last one padded with +0.0) and adds the squares of the
+// sums.
+template <uint32_t T, bool kFactor>
+__device__ __forceinline__ double accumulate_squares(const GradUnit& u, const GradListView& list,
+                                                     float* acc, bool overwrite, float factor,
+                                                     uint32_t& top) {
+  constexpr uint32_t kBatch = 2;
+  const Place src(u, list.tensors, list.unit_elems);
+  float* dst = acc + u.offset;
+  const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
   const uint32_t whole = u.count / kVec;
   double sum = 0.0;
   uint32_t m = 0u;
-  auto take = [&](const float (&y)[8]) {
-    if constexpr (kNorm) {
-      float x[8];
+  for (uint32_t v0 = threadIdx.x; v0 * kVec < u.count; v0 += kBatch * kListThreads) {
+    Raw<T> raw[kBatch];
+    float old[kBatch][8];
 #pragma unroll
-      for (uint32_t j = 0; j < kVec; ++j) {
-        x[j] = y[j];
-        m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
-      }
-      sum = add_squares8<kMul>(sum, x, sc);
-    }
-  };
-  uint32_t done = 0u;  // whole vectors done
-  if (vector) {
-    done = whole;
-    for (uint32_t v0 = threadIdx.x; v0 < whole; v0 += kBatch * kListThreads) {
-      Raw<T> raw[kBatch];
-      float4 old[kBatch][2];
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      const uint32_t v = v0 + b * kListThreads;
+      const uint32_t e = v * kVec;
+      const uint32_t n = e >= u.count ? 0u : u.count - e < kVec ? u.count - e : kVec;
+      if (n == kVec && (u.flags & kGradVector))
+        raw[b].load(src.vector_at<T>(e));
+      else if (n == kVec && !src.pitched && v > 0u && v + 1u < whole)
+        raw[b].load_shifted(src.base + e * kSize<T>);
+      else
+        gather(raw[b], src, e, n);
 #pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        const uint32_t v = v0 + b * kListThreads;
-        if (v < whole) {
-          raw[b].load(src.at(v * kVec));
-          if (!overwrite) {
-            old[b][0] = __ldcs(reinterpret_cast<const float4*>(dst + v * kVec));
-            old[b][1] = __ldcs(reinterpret_cast<const float4*>(dst + v * kVec) + 1);
-          }
-        }
-      }
+      for (uint32_t j = 0; j < kVec; ++j) old[b][j] = 0.0f;
+      if (!overwrite) {
+        if (wide && n == kVec) {
+          load_acc(dst + e, old[b]);
+        } else {
 #pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) {
-        const uint32_t v = v0 + b * kListThreads;
-        if (v < whole) {
-          float y[8];
-          raw[b].unpack(y);
-          if (!overwrite) {
-            y[0] = __fadd_rn(old[b][0].x, y[0]); y[1] = __fadd_rn(old[b][0].y, y[1]);
-            y[2] = __fadd_rn(old[b][0].z, y[2]); y[3] = __fadd_rn(old[b][0].w, y[3]);
-            y[4] = __fadd_rn(old[b][1].x, y[4]); y[5] = __fadd_rn(old[b][1].y, y[5]);
-            y[6] = __fadd_rn(old[b][1].z, y[6]); y[7] = __fadd_rn(old[b][1].w, y[7]);
-          }
-          store8<kGradF32>(dst + v * kVec, y);
-          take(y);
+          for (uint32_t j = 0; j < kVec; ++j)
+            if (j < n) old[b][j] = dst[e + j];
         }
       }
     }
-  }
-  if constexpr (kNorm) {
-    // Vector by vector, in the tree's order, the last one padded with +0.0.
-    for (uint32_t v = done + (threadIdx.x + kListThreads - done % kListThreads) % kListThreads;
-         v * kVec < u.count; v += kListThreads) {
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      const uint32_t e = (v0 + b * kListThreads) * kVec;
+      const uint32_t n = e >= u.count ? 0u : u.count - e < kVec ? u.count - e : kVec;
       float y[8];
+      raw[b].unpack(y);
+      if (!overwrite) {
 #pragma unroll
-      for (uint32_t j = 0; j < kVec; ++j) {
-        const uint32_t e = v * kVec + j;
-        y[j] = 0.0f;
-        if (e < u.count) {
-          const float x = from_bits<T>(elem_bits<T>(src.base, src.element(e)));
-          y[j] = overwrite ? x : __fadd_rn(dst[e], x);
-          dst[e] = y[j];
-        }
+        for (uint32_t j = 0; j < kVec; ++j) y[j] = __fadd_rn(old[b][j], y[j]);
       }
-      take(y);
-    }
-    top = m;
-  } else {
-    for (uint32_t e = done * kVec + threadIdx.x; e < u.count; e += kListThreads) {
-      const float x = from_bits<T>(elem_bits<T>(src.base, src.element(e)));
-      dst[e] = overwrite ? x : __fadd_rn(dst[e], x);
+      if (wide && n == kVec) {
+        store8<kGradF32>(dst + e, y);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kVec; ++j)
+          if (j < n) dst[e + j] = y[j];
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kVec; ++j) m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
+      sum = add_vector<kFactor>(sum, y, factor);
     }
   }
+  top = m;
   return sum;
 }
 
-template <bool kNorm, bool kMul>
-__device__ __forceinline__ double accumulate_any(const GradUnit& u, const GradListView& list,
-                                                 float* acc, bool overwrite, const ScaleInfo& sc,
-                                                 uint32_t& top) {
+template <bool kFactor>
+__device__ __forceinline__ double accumulate_squares_any(const GradUnit& u,
+                                                         const GradListView& list, float* acc,
+                                                         bool overwrite, float factor,
+                                                         uint32_t& top) {
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
-      return accumulate_unit<kGradF32, kNorm, kMul>(u, list, acc, overwrite, sc, top);
+      return accumulate_squares<kGradF32, kFactor>(u, list, acc, overwrite, factor, top);
     case kGradBf16:
-      return accumulate_unit<kGradBf16, kNorm, kMul>(u, list, acc, overwrite, sc, top);
-    default:
-      return accumulate_unit<kGradF16, kNorm, kMul>(u, list, acc, overwrite, sc, top);
+      return accumulate_squares<kGradBf16, kFactor>(u, list, acc, overwrite, factor, top);
+    default: return accumulate_squares<kGradF16, kFactor>(u, list, acc, overwrite, factor, top);
   }
-}
-
-__global__ void __launch_bounds__(kListThreads)
-    list_accumulate_kernel(GradListView list, float* acc, int overwrite) {
-  const GradUnit u = load_unit(list.units, blockIdx.x);
-  const ScaleInfo none{1.0f, 1.0f, true};
-  uint32_t top = 0u;
-  accumulate_any<false, true>(u, list, acc, overwrite != 0, none, top);
 }
 
 // Writes what the update reads as its gradients, so it does not trigger: the
 // kernels behind it start when it has completed.
 __global__ void __launch_bounds__(kListThreads)
     list_accumulate_norm_kernel(GradListView list, float* acc, int overwrite, float scale,
-                                const DeviceScaler* scaler, GradPartials part) {
+                                const DeviceScaler* scaler, GradPartial* partials) {
   __shared__ double s_sum[kListThreads / 32];
   __shared__ uint32_t s_top[kListThreads / 32];
   const GradUnit u = load_unit(list.units, blockIdx.x);
-  const ScaleInfo sc = decode_scale(scaler ? scaler->scale : scale);
+  pdl_wait();
+  const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
-  double sum = sc.mul ? accumulate_any<true, true>(u, list, acc, overwrite != 0, sc, top)
-                      : accumulate_any<true, false>(u, list, acc, overwrite != 0, sc, top);
+  double sum = factor == 1.0f
+                   ? accumulate_squares_any<false>(u, list, acc, overwrite != 0, factor, top)
+                   : accumulate_squares_any<true>(u, list, acc, overwrite != 0, factor, top);
   fold_block<kListThreads>(sum, top, s_sum, s_top);
-  if (threadIdx.x == 0) {
-    part.sums[blockIdx.x] = sum;
-    part.tops[blockIdx.x] = top;
-  }
+  if (threadIdx.x == 0) store_partial(partials + blockIdx.x, sum, top);
 }
 
 // ---- the step's update ---------------------------------------------------------
@@ -879,7 +1224,8 @@ __global__ void __launch_bounds__(kBulkThreads)
               search_tensor(e, __ldg(tile_first + e / kTileElems), list.n_tensors, offsets);
           const float wd = __ldg(decay + k) ? p.decay_weight : p.no_decay_weight;
           const float x = grad_at(list.tensors, k, e - __ldg(offsets + k));
-          const float gv = clipped(x, sc, clip);
+          const float gv =
+              __fmul_rn(sc.mul ? unscale<true>(x, sc) : unscale<false>(x, sc), clip);
           float m = mom[e], v = var[e];
           const float t1 = adamw_elem(master[e], gv, m, v, wd, p, bad);
           master[e] = t1;
@@ -923,6 +1269,18 @@ __global__ void list_bind_units_kernel(const GradTensor* tensors, GradUnit* unit
   units[i].flags = t.flags;
 }
 
+// Blocks of one resident wave on the current device.
+template <typename K>
+uint32_t wave_blocks(K kernel) {
+  int device = 0, sms = 0, per_sm = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kListThreads, 0) !=
+          cudaSuccess)
+    return 1u;
+  return uint32_t(std::max(1, sms) * std::max(1, per_sm));
+}
+
 // Launch chained behind the kernel ahead of it on the stream (see pdl_wait).
 template <typename... Args>
 cudaError_t launch_chained(void (*kernel)(Args...), uint32_t grid, uint32_t block, size_t smem,
@@ -943,48 +1301,68 @@ cudaError_t launch_chained(void (*kernel)(Args...), uint32_t grid, uint32_t bloc
 }  // namespace
 
 cudaError_t launch_list_norm(const GradListView& list, float scale, const DeviceScaler* scaler,
-                             const GradPartials& part, cudaStream_t stream) {
+                             GradPartial* partials, cudaStream_t stream) {
   if (list.n_units == 0) return cudaSuccess;
-  list_norm_kernel<<<list.n_units, kListThreads, 0, stream>>>(list, scale, scaler, part);
-  return cudaGetLastError();
+  return launch_chained(list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units, kListThreads, 0, stream, list, scale, scaler,
+                        partials);
 }
 
-cudaError_t launch_list_finalize(const GradListView& list, const GradPartials& part, float scale,
-                                 float max_norm, int kind, const GradListOut& out,
+cudaError_t launch_list_finalize(const GradListView& list, const GradPartial* partials,
+                                 float scale, float max_norm, int kind, const GradListOut& out,
                                  cudaStream_t stream) {
   const uint32_t grid = 1u + (out.tensor_norms || out.tensor_max ? list.n_tensors : 0u);
-  return launch_chained(list_finalize_kernel, grid, kFinalThreads, 0, stream, list, part, scale,
-                        max_norm, kind, out);
+  return launch_chained(list_finalize_kernel, grid, kFinalThreads, 0, stream, list, partials,
+                        scale, max_norm, kind, out);
 }
 
-cudaError_t launch_list_decide(const GradListView& list, const GradPartials& part,
+cudaError_t launch_list_decide(const GradListView& list, const GradPartial* partials,
                                DeviceScaler* scaler, DeviceStepState* st,
                                const FinalizeParams& fp, cudaStream_t stream) {
-  return launch_chained(list_decide_kernel, 1u, kFinalThreads, 0, stream, list, part, scaler, st,
-                        fp);
+  return launch_chained(list_decide_kernel, 1u, kFinalThreads, 0, stream, list, partials, scaler,
+                        st, fp);
 }
+
+namespace {
+template <uint32_t kOut>
+cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, float scale,
+                           const float* result, cudaStream_t stream) {
+  const auto kernel =
+      list.rows || out.rows ? list_clip_kernel<kOut, true> : list_clip_kernel<kOut, false>;
+  // Where there may be nothing to do, one wave of blocks that walk the units, so
+  // that leaving is quick; else a block per unit, which the hardware balances.
+  uint32_t grid = list.n_units;
+  if (kOut == kOutSame && scale == 1.0f) grid = std::min(grid, wave_blocks(kernel));
+  return launch_chained(kernel, grid, kListThreads, 0, stream, list, out, scale, result);
+}
+}  // namespace
 
 cudaError_t launch_list_clip(const GradListView& list, const GradListView& out, float scale,
                              const float* result, bool in_place, cudaStream_t stream) {
   if (list.n_units == 0) return cudaSuccess;
-  return launch_chained(list_clip_kernel, list.n_units, kListThreads, 0, stream, list, out, scale,
-                        result, in_place);
+  if (in_place) return launch_clip_to<kOutSame>(list, list, scale, result, stream);
+  cudaError_t e = cudaSuccess;
+  if (out.types & (1u << kGradF32))
+    e = launch_clip_to<kGradF32>(list, out, scale, result, stream);
+  if (e == cudaSuccess && (out.types & (1u << kGradBf16)))
+    e = launch_clip_to<kGradBf16>(list, out, scale, result, stream);
+  if (e == cudaSuccess && (out.types & (1u << kGradF16)))
+    e = launch_clip_to<kGradF16>(list, out, scale, result, stream);
+  return e;
 }
 
 cudaError_t launch_list_accumulate(const GradListView& list, float* acc, int overwrite,
                                    cudaStream_t stream) {
   if (list.n_units == 0) return cudaSuccess;
-  list_accumulate_kernel<<<list.n_units, kListThreads, 0, stream>>>(list, acc, overwrite);
-  return cudaGetLastError();
+  return launch_chained(list.rows ? list_accumulate_kernel<true> : list_accumulate_kernel<false>, list.n_units, kListThreads, 0, stream, list, acc,
+                        overwrite);
 }
 
 cudaError_t launch_list_accumulate_norm(const GradListView& list, float* acc, int overwrite,
                                         float scale, const DeviceScaler* scaler,
-                                        const GradPartials& part, cudaStream_t stream) {
+                                        GradPartial* partials, cudaStream_t stream) {
   if (list.n_units == 0) return cudaSuccess;
-  list_accumulate_norm_kernel<<<list.n_units, kListThreads, 0, stream>>>(list, acc, overwrite,
-                                                                         scale, scaler, part);
-  return cudaGetLastError();
+  return launch_chained(list_accumulate_norm_kernel, list.n_units, kListThreads, 0, stream, list,
+                        acc, overwrite, scale, scaler, partials);
 }
 
 int list_update_grid(int device) {

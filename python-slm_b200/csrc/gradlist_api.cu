@@ -25,6 +25,8 @@ struct slm_grad_list {
   std::vector<uint64_t> rows;  // 1 for contiguous tensors
   std::vector<Extent> extents;  // non-empty tensors by address
   bool overlapping = false;     // two tensors share an element
+  uint32_t pitched = 0;         // whether any tensor is rows with a pitch
+  uint32_t types = 0;           // bit per type of a tensor with elements
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
@@ -32,8 +34,8 @@ struct slm_grad_list {
   GradUnit* d_units = nullptr;
 
   GradListView view() const {
-    return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems,
-                        elements};
+    return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
+                        types, elements};
   }
 };
 
@@ -47,9 +49,9 @@ uint64_t span_bytes(const GradTensor& t, uint64_t rows) {
 uint32_t layout_flags(uint32_t type, bool pitched, const void* ptr, uint64_t columns,
                       uint64_t row_stride) {
   uint32_t f = type | (pitched ? kGradPitched : 0u);
-  const uint64_t size = type_bytes(type);
-  if (reinterpret_cast<uintptr_t>(ptr) % 16 == 0 &&
-      (!pitched || (columns % kVec == 0 && row_stride * size % 16 == 0)))
+  const uint64_t size = type_bytes(type), vec = kVec * size;
+  if (reinterpret_cast<uintptr_t>(ptr) % vec == 0 &&
+      (!pitched || (columns % kVec == 0 && row_stride * size % vec == 0)))
     f |= kGradVector;
   return f;
 }
@@ -131,6 +133,8 @@ int fill_list(slm_grad_list* l, const slm_grad_view* views, uint32_t n) {
     if (pitched && v.row_stride < v.columns)
       return fail(SLM_ERR_INVALID_ARGUMENT, "a gradient tensor's rows overlap");
     l->rows[k] = pitched ? v.rows : 1;
+    if (pitched) l->pitched = 1;
+    if (t.elements) l->types |= 1u << uint32_t(v.dtype);
     t.flags = layout_flags(uint32_t(v.dtype), pitched, v.data, t.columns, t.row_stride);
     t.offset = l->elements;
     l->elements += t.elements;
@@ -181,16 +185,7 @@ int upload_list(slm_grad_list* l) {
   return cuda_status(cudaStreamSynchronize(nullptr), "upload list");
 }
 
-constexpr uint64_t kAlign = 256;
-uint64_t round_up(uint64_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
-uint64_t workspace_bytes(uint64_t units) {
-  return round_up(units * sizeof(double)) + round_up(units * sizeof(uint32_t)) + kAlign;
-}
-GradPartials split_workspace(void* workspace, uint64_t units) {
-  uint8_t* p = static_cast<uint8_t*>(workspace);
-  return GradPartials{reinterpret_cast<double*>(p),
-                      reinterpret_cast<uint32_t*>(p + round_up(units * sizeof(double)))};
-}
+uint64_t partial_bytes(uint64_t units) { return (units ? units : 1) * sizeof(GradPartial); }
 
 bool positive(float v) { return v > 0.0f && finite_f32(v); }
 
@@ -208,7 +203,7 @@ int check_norm_call(const slm_grad_list* list, float loss_scale, float max_norm,
     return fail(SLM_ERR_INVALID_ARGUMENT, "results must be aligned to their element size");
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return fail(SLM_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
-  if (bytes < workspace_bytes(list->n_units))
+  if (bytes < partial_bytes(list->n_units))
     return fail(SLM_ERR_INVALID_ARGUMENT,
                 "the workspace is smaller than slm_grad_list_workspace_bytes(list)");
   return SLM_OK;
@@ -217,7 +212,7 @@ int check_norm_call(const slm_grad_list* list, float loss_scale, float max_norm,
 int norm_kernels(const slm_grad_list* list, float loss_scale, float max_norm, int kind,
                  const GradListOut& out, void* workspace, cudaStream_t s) {
   const GradListView v = list->view();
-  const GradPartials part = split_workspace(workspace, list->n_units);
+  GradPartial* part = static_cast<GradPartial*>(workspace);
   int st = cuda_status(launch_list_norm(v, loss_scale, nullptr, part, s), "list norm kernel");
   if (st) return st;
   return cuda_status(launch_list_finalize(v, part, loss_scale, max_norm, kind, out, s),
@@ -266,13 +261,13 @@ uint64_t slmopt::list_partial_bytes(const std::vector<uint64_t>& offsets) {
   uint64_t units = 0;
   for (size_t k = 0; k + 1 < offsets.size(); ++k)
     units += (offsets[k + 1] - offsets[k] + unit - 1) / unit;
-  return workspace_bytes(units);
+  return partial_bytes(units);
 }
 
 int slmopt::enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list,
                               const slm_step_config* cfg, cudaStream_t s) {
   const FinalizeParams fp = finalize_params(h, cfg);
-  const GradPartials part = split_workspace(h->d_list_partials, list->n_units);
+  GradPartial* part = static_cast<GradPartial*>(h->d_list_partials);
   const GradListView v = list->view();
   int st = h->cuda(launch_list_norm(v, fp.static_scale, fp.dynamic ? h->d_scaler : nullptr, part, s),
                    "list norm kernel");
@@ -345,7 +340,7 @@ int slm_grad_list_destroy(slm_grad_list* list) {
 uint64_t slm_grad_list_elements(const slm_grad_list* list) { return list ? list->elements : 0; }
 
 uint64_t slm_grad_list_workspace_bytes(const slm_grad_list* list) {
-  return list ? workspace_bytes(list->n_units) : 0;
+  return list ? partial_bytes(list->n_units) : 0;
 }
 
 int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n, void* stream) {
@@ -505,7 +500,7 @@ int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
   h->pass_grads = nullptr;
   h->pass_is_list = false;
   const FinalizeParams fp = finalize_params(h, cfg);
-  const GradPartials part = split_workspace(h->d_list_partials, list->n_units);
+  GradPartial* part = static_cast<GradPartial*>(h->d_list_partials);
   const GradListView v = list->view();
   if ((st = h->cuda(launch_list_accumulate_norm(v, acc_device, overwrite, fp.static_scale,
                                                 fp.dynamic ? h->d_scaler : nullptr, part, s),

@@ -253,7 +253,7 @@ int adamw_update_grid(int device, int dtype);
 // fixed tree, which therefore restarts at every tensor.
 constexpr uint32_t kGradF32 = 0, kGradBf16 = 1, kGradF16 = 2;  // slm_dtype
 constexpr uint32_t kGradTypeMask = 3u;
-constexpr uint32_t kGradVector = 4u;   // every 8-element vector is one run on a 16-byte boundary
+constexpr uint32_t kGradVector = 4u;   // every 8-element vector is one run on its size's boundary
 constexpr uint32_t kGradPitched = 8u;  // rows are further apart than their columns
 struct __align__(16) GradTensor {
   const void* ptr;
@@ -287,6 +287,8 @@ struct GradListView {
   const GradTensor* tensors;
   uint32_t n_units, n_tensors;
   uint32_t unit_elems;
+  uint32_t rows;   // whether any tensor is pitched
+  uint32_t types;  // bit per type of a tensor with elements
   uint64_t elements;
 };
 struct GradListOut {
@@ -295,16 +297,17 @@ struct GradListOut {
   float* tensor_max;     // n_tensors, or NULL
   double* sum_squares;   // or NULL
 };
-// Per unit: f64 sum of squares and f32 bits of the largest magnitude (of the
-// stored values; the finalize unscales it).
-struct GradPartials {
-  double* sums;
-  uint32_t* tops;
+// A unit's share of the norm: the f64 sum of its squares (see square_factor) and
+// the f32 bits of its largest magnitude, not unscaled.
+struct __align__(16) GradPartial {
+  double sum;
+  uint32_t top;
+  uint32_t reserved;
 };
 cudaError_t launch_list_norm(const GradListView& list, float scale, const DeviceScaler* scaler,
-                             const GradPartials& part, cudaStream_t stream);
-cudaError_t launch_list_finalize(const GradListView& list, const GradPartials& part, float scale,
-                                 float max_norm, int kind, const GradListOut& out,
+                             GradPartial* partials, cudaStream_t stream);
+cudaError_t launch_list_finalize(const GradListView& list, const GradPartial* partials,
+                                 float scale, float max_norm, int kind, const GradListOut& out,
                                  cudaStream_t stream);
 cudaError_t launch_list_clip(const GradListView& list, const GradListView& out, float scale,
                              const float* result, bool in_place, cudaStream_t stream);
@@ -313,9 +316,9 @@ cudaError_t launch_list_accumulate(const GradListView& list, float* acc, int ove
 // The last micro-batch: accumulates and forms the partials of the sums.
 cudaError_t launch_list_accumulate_norm(const GradListView& list, float* acc, int overwrite,
                                         float scale, const DeviceScaler* scaler,
-                                        const GradPartials& part, cudaStream_t stream);
+                                        GradPartial* partials, cudaStream_t stream);
 // The handle's decision (clip, skip, scaler) from a list's partials.
-cudaError_t launch_list_decide(const GradListView& list, const GradPartials& part,
+cudaError_t launch_list_decide(const GradListView& list, const GradPartial* partials,
                                DeviceScaler* scaler, DeviceStepState* st,
                                const FinalizeParams& fp, cudaStream_t stream);
 // AdamW over the flat state with the gradients read from the list's tensors,
