@@ -433,7 +433,7 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * infinite and counts as a non-finite gradient, one below 1e-38 loses bits. */
 typedef struct slm_grad_view {
   const void* data;     /* device memory, aligned to the element */
-  uint64_t rows, columns;
+  uint64_t rows, columns; /* at most 2^30 columns where rows have a pitch */
   uint64_t row_stride;  /* elements from one row to the next, >= columns */
   int32_t dtype;        /* slm_dtype */
 } slm_grad_view;

@@ -153,67 +153,84 @@ __device__ __forceinline__ uint32_t top_f32(uint32_t m) {
 }
 
 // ---- where a unit's elements lie -------------------------------------------------
-// Element e of the unit in row-major order; a pitched tensor's rows are walked
-// with one division per run.
-struct Place {
-  const uint8_t* base;
-  uint64_t first;  // pitched: the unit's first element within its tensor
-  uint64_t columns, stride;
-  bool pitched;
-  __device__ __forceinline__ Place(const GradUnit& u, const GradTensor* tensors,
-                                   uint32_t unit_elems)
-      : base(static_cast<const uint8_t*>(u.ptr)), first(0), columns(0), stride(0),
-        pitched((u.flags & kGradPitched) != 0u) {
-    if (pitched) {
-      const GradTensor* t = tensors + u.tensor;
-      columns = __ldg(&t->columns);
-      stride = __ldg(&t->row_stride);
-      first = uint64_t(u.index) * unit_elems;
+// A thread's place in a unit, moved from vector to vector (256 vectors apart)
+// without a division: the row-major position is kept as an address and a column.
+// A contiguous unit is one row.
+template <uint32_t T>
+struct Rows {
+  uint8_t* p;         // the next element
+  uint32_t col;       // its column
+  uint32_t columns;
+  uint32_t col_step;  // of 2,048 elements
+  uint64_t step;      // bytes, before a wrap
+  uint64_t wrap;      // bytes from a row's end to the next row
+  __device__ __forceinline__ Rows(const GradUnit& u, const GradListView& list) {
+    const uint32_t e = threadIdx.x * kVec;
+    p = static_cast<uint8_t*>(const_cast<void*>(u.ptr));
+    if (u.flags & kGradPitched) {
+      const GradTensor* t = list.tensors + u.tensor;
+      const uint64_t stride = __ldg(&t->row_stride);
+      columns = static_cast<uint32_t>(__ldg(&t->columns));
+      const uint64_t k = uint64_t(u.index) * list.unit_elems + e;
+      const uint64_t row = k <= 0xffffffffull ? uint64_t(uint32_t(k) / columns) : k / columns;
+      col = static_cast<uint32_t>(k - row * columns);
+      p += (row * stride + col) * kSize<T>;
+      const uint32_t rows = kListThreads * kVec / columns;
+      col_step = kListThreads * kVec - rows * columns;
+      step = (rows * stride + col_step) * kSize<T>;
+      wrap = (stride - columns) * kSize<T>;
+    } else {
+      columns = u.count;
+      col = e;
+      p += uint64_t(e) * kSize<T>;
+      col_step = kListThreads * kVec;
+      step = uint64_t(col_step) * kSize<T>;
+      wrap = 0u;
     }
   }
-  // Index in memory of element e, and the elements of its row from there on.
-  __device__ __forceinline__ uint64_t index(uint32_t e, uint64_t& run) const {
-    run = ~uint64_t(0);
-    if (!pitched) return e;
-    const uint64_t k = first + e;
-    const uint64_t row = (k | columns) <= 0xffffffffull
-                             ? uint64_t(static_cast<uint32_t>(k) / static_cast<uint32_t>(columns))
-                             : k / columns;
-    const uint64_t col = k - row * columns;
-    run = columns - col;
-    return row * stride + col;
-  }
-  // The next element's index.
-  __device__ __forceinline__ void next(uint64_t& i, uint64_t& run) const {
-    ++i;
-    if (--run == 0u) {
-      i += stride - columns;
-      run = columns;
+  __device__ __forceinline__ void next_vector() {
+    p += step;
+    col += col_step;
+    if (col >= columns) {
+      col -= columns;
+      p += wrap;
     }
   }
-  // The address of vector-aligned element e.
-  template <uint32_t T>
-  __device__ __forceinline__ uint8_t* vector_at(uint32_t e) const {
-    uint64_t run;
-    return const_cast<uint8_t*>(base) + index(e, run) * kSize<T>;
+  __device__ __forceinline__ void next_element() {
+    p += kSize<T>;
+    if (++col == columns) {
+      col = 0u;
+      p += wrap;
+    }
+  }
+  // Whether the next vector is one run on its boundary.
+  __device__ __forceinline__ bool aligned() const {
+    return col + kVec <= columns && reinterpret_cast<uintptr_t>(p) % kVecBytes<T> == 0u;
+  }
+  // The next n <= 8 elements, the rest zero.
+  __device__ __forceinline__ void load(Raw<T>& raw, uint32_t n) const {
+    if (n == kVec && aligned()) {
+      raw.load(p);
+    } else if (n == kVec && col >= kVec && col + 2u * kVec <= columns) {
+      raw.load_shifted(p);  // its blocks lie within the row
+    } else {
+      raw.zero();
+      Rows r = *this;
+#pragma unroll
+      for (uint32_t j = 0; j < kVec; ++j) {
+        if (j < n) {
+          raw.set(j, elem_bits<T>(r.p, 0));
+          r.next_element();
+        }
+      }
+    }
   }
 };
-
-// Elements e .. e + n - 1 (n <= 8) one by one, the rest zero: of rows, and of
-// contiguous memory.
-template <uint32_t T>
-__device__ __forceinline__ void gather(Raw<T>& raw, const Place& place, uint32_t e, uint32_t n) {
-  raw.zero();
-  uint64_t run;
-  uint64_t i = place.index(e, run);
-#pragma unroll
-  for (uint32_t j = 0; j < kVec; ++j) {
-    if (j < n) {
-      raw.set(j, elem_bits<T>(place.base, i));
-      place.next(i, run);
-    }
-  }
+__device__ __forceinline__ uint32_t vector_elems(uint32_t e, uint32_t count) {
+  return e >= count ? 0u : count - e < kVec ? count - e : kVec;
 }
+
+// n <= 8 elements of contiguous memory one by one, the rest zero.
 template <uint32_t T>
 __device__ __forceinline__ void gather_flat(Raw<T>& raw, const uint8_t* p, uint32_t n) {
   raw.zero();
@@ -334,28 +351,30 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
 }
 
 template <uint32_t T, bool kFactor>
-__device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, const Place& place,
-                                            uint32_t count, bool vector) {
-  for (uint32_t e = threadIdx.x * kVec; e < count; e += kListThreads * kVec) {
-    Raw<T> raw;
-    if (vector)
-      raw.load(place.vector_at<T>(e));
-    else
-      gather(raw, place, e, count - e < kVec ? count - e : kVec);
-    sq.take(raw);
+__device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, Rows<T> rows,
+                                            uint32_t count) {
+  constexpr uint32_t kBatch = 2;
+  for (uint32_t e = threadIdx.x * kVec; e < count; e += kBatch * kListThreads * kVec) {
+    Raw<T> raw[kBatch];
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      rows.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count));
+      rows.next_vector();
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) sq.take(raw[b]);
   }
 }
 
 // kRows: the list has pitched tensors.  The kernels without them need fewer
 // registers, so more of their loads are in flight.
 template <uint32_t T, bool kFactor, bool kRows>
-__device__ __forceinline__ double unit_squares(const GradUnit& u, const GradTensor* tensors,
-                                               uint32_t unit_elems, float factor,
-                                               uint32_t& top) {
+__device__ __forceinline__ double unit_squares(const GradUnit& u, const GradListView& list,
+                                               float factor, uint32_t& top) {
   Squares<T, kFactor> sq;
   sq.factor = factor;
   if (kRows && (u.flags & kGradPitched))
-    row_squares(sq, Place(u, tensors, unit_elems), u.count, (u.flags & kGradVector) != 0u);
+    row_squares(sq, Rows<T>(u, list), u.count);
   else
     flat_squares(sq, static_cast<const uint8_t*>(u.ptr), u.count);
   top = top_f32<T>(sq.top);
@@ -398,15 +417,14 @@ __device__ __forceinline__ void store_partial(const GradPartial* partials, doubl
 }
 
 template <bool kFactor, bool kRows>
-__device__ __forceinline__ double unit_squares_any(const GradUnit& u, const GradTensor* tensors,
-                                                   uint32_t unit_elems, float factor,
-                                                   uint32_t& top) {
+__device__ __forceinline__ double unit_squares_any(const GradUnit& u, const GradListView& list,
+                                                   float factor, uint32_t& top) {
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
-      return unit_squares<kGradF32, kFactor, kRows>(u, tensors, unit_elems, factor, top);
+      return unit_squares<kGradF32, kFactor, kRows>(u, list, factor, top);
     case kGradBf16:
-      return unit_squares<kGradBf16, kFactor, kRows>(u, tensors, unit_elems, factor, top);
-    default: return unit_squares<kGradF16, kFactor, kRows>(u, tensors, unit_elems, factor, top);
+      return unit_squares<kGradBf16, kFactor, kRows>(u, list, factor, top);
+    default: return unit_squares<kGradF16, kFactor, kRows>(u, list, factor, top);
   }
 }
 
@@ -424,8 +442,8 @@ __global__ void __launch_bounds__(kListThreads, kRows ? 5 : 8)
   const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
   double sum = factor == 1.0f
-                   ? unit_squares_any<false, kRows>(u, list.tensors, list.unit_elems, factor, top)
-                   : unit_squares_any<true, kRows>(u, list.tensors, list.unit_elems, factor, top);
+                   ? unit_squares_any<false, kRows>(u, list, factor, top)
+                   : unit_squares_any<true, kRows>(u, list, factor, top);
   fold_block<kListThreads>(sum, top, s_sum, s_top);
   if (threadIdx.x == 0) store_partial(partials + blockIdx.x, sum, top);
 }
@@ -662,29 +680,38 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
   }
 }
 
-// Rows on either side: whole vectors where both sides have them, else 8 elements
-// a thread.
+// Rows on either side.
 template <uint32_t T, uint32_t O>
-__device__ __forceinline__ void clip_rows(const Place& src, const Place& dst, uint32_t count,
-                                          bool vectors, float scale, const float* result,
-                                          bool& waited) {
+__device__ __forceinline__ void clip_rows(Rows<T> src, Rows<O> dst, uint32_t count, float scale,
+                                          const float* result, bool& waited) {
+  constexpr uint32_t kBatch = 2;
   if (!clip_ready(result, waited)) return;
   const ClipFactor f(__ldcg(result + 1), scale);
-  uint32_t e = threadIdx.x * kVec;
-  if (vectors) {
-    for (; e + kVec <= count; e += kListThreads * kVec) {
-      Raw<T> raw;
-      raw.load(src.vector_at<T>(e));
-      clip_raw<T, O>(raw, f, dst.vector_at<O>(e));
+  for (uint32_t e = threadIdx.x * kVec; e < count; e += kBatch * kListThreads * kVec) {
+    Raw<T> raw[kBatch];
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      src.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count));
+      src.next_vector();
     }
-  }
-  for (; e < count; e += kListThreads * kVec) {
-    uint64_t run_i, run_o;
-    uint64_t i = src.index(e, run_i), k = dst.index(e, run_o);
-    for (uint32_t j = 0; j < kVec && e + j < count; ++j) {
-      store1<O>(const_cast<uint8_t*>(dst.base), k, f(from_bits<T>(elem_bits<T>(src.base, i))));
-      src.next(i, run_i);
-      dst.next(k, run_o);
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      const uint32_t n = vector_elems(e + b * (kListThreads * kVec), count);
+      if (n == kVec && dst.aligned()) {
+        clip_raw<T, O>(raw[b], f, dst.p);
+      } else {
+        float x[8];
+        raw[b].unpack(x);
+        Rows<O> r = dst;
+#pragma unroll
+        for (uint32_t j = 0; j < kVec; ++j) {
+          if (j < n) {
+            store1<O>(r.p, 0, f(x[j]));
+            r.next_element();
+          }
+        }
+      }
+      dst.next_vector();
     }
   }
 }
@@ -694,8 +721,7 @@ __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
                                           const GradListView& list, const GradListView& out,
                                           float scale, const float* result, bool& waited) {
   if (kRows && ((u.flags | o.flags) & kGradPitched))
-    clip_rows<T, O>(Place(u, list.tensors, list.unit_elems), Place(o, out.tensors, out.unit_elems),
-                    u.count, (u.flags & o.flags & kGradVector) != 0u, scale, result, waited);
+    clip_rows<T, O>(Rows<T>(u, list), Rows<O>(o, out), u.count, scale, result, waited);
   else
     clip_flat<T, O>(static_cast<const uint8_t*>(u.ptr),
                     static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale, result,
@@ -706,7 +732,7 @@ __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
 // theirs), or in place.  All nine pairs of types in one kernel would spill.
 constexpr uint32_t kOutSame = 3u;
 template <uint32_t kOut, bool kRows>
-__global__ void __launch_bounds__(kListThreads, kRows ? 2 : 4)
+__global__ void __launch_bounds__(kListThreads, 4)
     list_clip_kernel(GradListView list, GradListView out, float scale, const float* result) {
   constexpr bool kSame = kOut == kOutSame;
   bool waited = false;
@@ -817,23 +843,26 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
 }
 
 template <uint32_t T>
-__device__ __forceinline__ void accumulate_rows(const Place& src, float* dst, uint32_t count,
-                                                bool vectors, bool overwrite) {
+__device__ __forceinline__ void accumulate_rows(Rows<T> src, float* dst, uint32_t count,
+                                                bool overwrite) {
+  const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
   for (uint32_t e = threadIdx.x * kVec; e < count; e += kListThreads * kVec) {
-    if (vectors) {
-      Raw<T> raw;
-      float old[8];
-      raw.load(src.vector_at<T>(e));
+    const uint32_t n = vector_elems(e, count);
+    Raw<T> raw;
+    float old[8];
+    if (wide && n == kVec) {
       if (!overwrite) load_acc(dst + e, old);
+      src.load(raw, n);
       add_raw<T>(raw, old, overwrite, dst + e);
     } else {
-      uint64_t run;
-      uint64_t i = src.index(e, run);
-      for (uint32_t j = 0; j < kVec && e + j < count; ++j) {
-        add_one<T>(src.base, i, overwrite, dst + e + j);
-        src.next(i, run);
-      }
+      src.load(raw, n);
+      float x[8];
+      raw.unpack(x);
+#pragma unroll
+      for (uint32_t j = 0; j < kVec; ++j)
+        if (j < n) dst[e + j] = overwrite ? x[j] : __fadd_rn(dst[e + j], x[j]);
     }
+    src.next_vector();
   }
 }
 
@@ -842,9 +871,7 @@ __device__ __forceinline__ void accumulate_unit(const GradUnit& u, const GradLis
                                                 float* acc, bool overwrite) {
   float* dst = acc + u.offset;
   if (kRows && (u.flags & kGradPitched))
-    accumulate_rows<T>(Place(u, list.tensors, list.unit_elems), dst, u.count,
-                       (u.flags & kGradVector) && reinterpret_cast<uintptr_t>(dst) % 32u == 0u,
-                       overwrite);
+    accumulate_rows<T>(Rows<T>(u, list), dst, u.count, overwrite);
   else
     accumulate_flat<T>(static_cast<const uint8_t*>(u.ptr), dst, u.count, overwrite);
 }
@@ -870,10 +897,9 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
                                                      float* acc, bool overwrite, float factor,
                                                      uint32_t& top) {
   constexpr uint32_t kBatch = 2;
-  const Place src(u, list.tensors, list.unit_elems);
+  Rows<T> src(u, list);
   float* dst = acc + u.offset;
   const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
-  const uint32_t whole = u.count / kVec;
   double sum = 0.0;
   uint32_t m = 0u;
   for (uint32_t v0 = threadIdx.x; v0 * kVec < u.count; v0 += kBatch * kListThreads) {
@@ -881,15 +907,10 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
     float old[kBatch][8];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
-      const uint32_t v = v0 + b * kListThreads;
-      const uint32_t e = v * kVec;
-      const uint32_t n = e >= u.count ? 0u : u.count - e < kVec ? u.count - e : kVec;
-      if (n == kVec && (u.flags & kGradVector))
-        raw[b].load(src.vector_at<T>(e));
-      else if (n == kVec && !src.pitched && v > 0u && v + 1u < whole)
-        raw[b].load_shifted(src.base + e * kSize<T>);
-      else
-        gather(raw[b], src, e, n);
+      const uint32_t e = (v0 + b * kListThreads) * kVec;
+      const uint32_t n = vector_elems(e, u.count);
+      src.load(raw[b], n);
+      src.next_vector();
 #pragma unroll
       for (uint32_t j = 0; j < kVec; ++j) old[b][j] = 0.0f;
       if (!overwrite) {
@@ -905,7 +926,7 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
       const uint32_t e = (v0 + b * kListThreads) * kVec;
-      const uint32_t n = e >= u.count ? 0u : u.count - e < kVec ? u.count - e : kVec;
+      const uint32_t n = vector_elems(e, u.count);
       float y[8];
       raw[b].unpack(y);
       if (!overwrite) {

@@ -132,6 +132,8 @@ int fill_list(slm_grad_list* l, const slm_grad_view* views, uint32_t n) {
     const bool pitched = t.elements && v.rows > 1 && v.row_stride != v.columns;
     if (pitched && v.row_stride < v.columns)
       return fail(SLM_ERR_INVALID_ARGUMENT, "a gradient tensor's rows overlap");
+    if (pitched && v.columns > (1u << 30))
+      return fail(SLM_ERR_SIZE_LIMIT, "rows with a pitch have at most 2^30 columns");
     l->rows[k] = pitched ? v.rows : 1;
     if (pitched) l->pitched = 1;
     if (t.elements) l->types |= 1u << uint32_t(v.dtype);

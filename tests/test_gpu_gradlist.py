@@ -708,6 +708,77 @@ def test_the_trainer_takes_lists(torch):
         assert shas[0] == shas[1]
 
 
+# ---- rows with a pitch -----------------------------------------------------------
+# (rows, columns, row stride, first column): odd and even pitches, rows shorter and
+# longer than a vector, a block's 2,048 elements and a unit
+ROWS = [(37, 25, 31, 3), (100, 24, 25, 0), (5, 4096, 5000, 8), (3, 1, 7, 2), (1000, 7, 9, 1),
+        (2, 3001, 3008, 5), (513, 8, 16, 0), (64, 1000, 1024, 8), (9, 2048, 2056, 8),
+        (700, 40, 41, 1), (2, 20_000, 20_001, 1), (4097, 1, 2, 1), (300, 16, 24, 8)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows, columns, stride, first", ROWS)
+def test_rows(torch, rows, columns, stride, first, name):
+    k = kind_of(torch, name)
+    gen = torch.Generator("cuda").manual_seed(rows)
+
+    def slab(kind):
+        room = (1e-2 * torch.randn(rows * stride + first, generator=gen, device="cuda")).to(kind)
+        return room, room[first:first + rows * stride].view(rows, stride)[:, :columns]
+
+    room, x = slab(k)
+    keep = room.clone()
+    other = (1e-2 * torch.randn(333, generator=gen, device="cuda")).to(k)
+    tensors = [x, other]
+    before = [t.clone() for t in tensors]
+    n = rows * columns + 333
+    limit = norms64(torch, tensors, 2.0, "l2")[0] / 2
+    with GradientList(tensors) as lst:
+        check_norm(torch, lst.norm(per_tensor=True, loss_scale=3.0), tensors, 3.0, 1.0)
+        want = tree_sum([t.float().reshape(-1).cpu().numpy() for t in before], 4096)
+        assert float(lst.norm().sum_squares) == want
+        flat = torch.cat([t.reshape(-1).float() for t in tensors])
+        for start in (0, 1):  # an accumulator on and off the 32-byte boundaries
+            acc = torch.randn(n + 8, generator=gen, device="cuda")[4 * start:4 * start + n]
+            old = acc.clone()
+            lst.accumulate(acc)
+            assert torch.equal(acc, old + flat)
+            lst.accumulate(acc, overwrite=True)
+            assert torch.equal(acc, flat)
+        for out in TYPES:  # rows into rows of another pitch, and into contiguous memory
+            for pitched in (True, False):
+                to, y = slab(kind_of(torch, out))
+                to_keep = to.clone()
+                if not pitched:
+                    y = torch.empty(rows, columns, dtype=kind_of(torch, out), device="cuda")
+                targets = [y, torch.empty_like(other, dtype=kind_of(torch, out))]
+                with GradientList(targets) as o:
+                    r = lst.clip(limit, loss_scale=2.0, out=o)
+                    check_norm(torch, r, before, 2.0, limit)
+                    check_clipped(torch, targets, before, 2.0, 0.5)
+                if pitched:  # nothing beside the columns
+                    y.copy_(to_keep[first:first + rows * stride].view(rows, stride)[:, :columns])
+                    assert torch.equal(to, to_keep)
+        lst.clip(limit, loss_scale=2.0)
+        check_clipped(torch, tensors, before, 2.0, 0.5)
+        x.copy_(before[0])
+        assert torch.equal(room, keep)
+    with B200Adamw(TensorTable.from_sizes([rows * columns, 333])) as opt:
+        tensors[1].copy_(before[1])
+        opts = StepOptions(one_based_update=10, max_grad_norm=limit, static_loss_scale=2.0)
+        with GradientList(tensors) as lst:
+            st = load(torch, opt, 9)
+            opt.step(lst, opts)
+            check_state(torch, opt.state_tensors(), st, before, [True, True], opts, 2.0, 0.5)
+            # the last micro-batch, added to what is there
+            acc = torch.randn(n, generator=gen, device="cuda")
+            old = acc.clone()
+            opt.norm_pass_accumulate(acc, lst, opts)
+            assert torch.equal(acc, old + flat)
+            res = opt.read_result()
+            near(res.grad_norm, float((acc.double() / 2.0).square().sum().sqrt()), 4 * U, "norm")
+
+
 # ---- streams, graphs, addresses ----------------------------------------------------
 def test_bind_follows_new_addresses(torch):
     sizes = [1 + (37 * i) % 5000 for i in range(700)]  # more than two bind batches
