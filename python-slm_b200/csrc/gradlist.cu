@@ -27,6 +27,20 @@ namespace {
 constexpr uint32_t kListThreads = 256;
 constexpr uint32_t kFinalThreads = 1024;
 
+// ---- L2 priorities ---------------------------------------------------------------
+// What a kernel reads or writes for the last time leaves the L2 first; what the
+// clip reads again soon (the list's end, see GradListView::keep) stays longest.
+__device__ __forceinline__ uint64_t l2_first_out() {
+  uint64_t r;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(r));
+  return r;
+}
+__device__ __forceinline__ uint64_t l2_normal() {
+  uint64_t r;
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(r));
+  return r;
+}
+
 // ---- element types ------------------------------------------------------------
 template <uint32_t T>
 constexpr uint32_t kSize = T == kGradF32 ? 4u : 2u;
@@ -63,17 +77,18 @@ struct Raw {
     for (uint32_t i = 0; i < kWords; ++i) w[i] = 0u;
   }
   // One load of a vector on its own size's boundary.
-  __device__ __forceinline__ void load(const void* p) {
+  __device__ __forceinline__ void load(const void* p, uint64_t policy) {
     if constexpr (T == kGradF32) {
-      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
-                     "=r"(w[6]), "=r"(w[7])
-                   : "l"(p)
-                   : "memory");
+      asm volatile(
+          "ld.global.L1::no_allocate.L2::cache_hint.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8], %9;"
+          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+            "=r"(w[7])
+          : "l"(p), "l"(policy)
+          : "memory");
     } else {
-      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+      asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.b32 {%0,%1,%2,%3}, [%4], %5;"
                    : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                   : "l"(p)
+                   : "l"(p), "l"(policy)
                    : "memory");
     }
   }
@@ -208,9 +223,9 @@ struct Rows {
     return col + kVec <= columns && reinterpret_cast<uintptr_t>(p) % kVecBytes<T> == 0u;
   }
   // The next n <= 8 elements, the rest zero.
-  __device__ __forceinline__ void load(Raw<T>& raw, uint32_t n) const {
+  __device__ __forceinline__ void load(Raw<T>& raw, uint32_t n, uint64_t policy) const {
     if (n == kVec && aligned()) {
-      raw.load(p);
+      raw.load(p, policy);
     } else if (n == kVec && col >= kVec && col + 2u * kVec <= columns) {
       raw.load_shifted(p);  // its blocks lie within the row
     } else {
@@ -311,7 +326,7 @@ struct Squares {
 
 template <uint32_t T, bool kFactor>
 __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint8_t* base,
-                                             uint32_t count) {
+                                             uint32_t count, uint64_t policy) {
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;  // 64 bytes of loads per thread in flight
   constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
   const uint32_t whole = count / kVec;
@@ -321,14 +336,14 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
     for (; v + (kBatch - 1) * kListThreads < whole; v += kBatch * kListThreads) {
       Raw<T> raw[kBatch];
 #pragma unroll
-      for (uint32_t b = 0; b < kBatch; ++b) raw[b].load(p + b * kStep);
+      for (uint32_t b = 0; b < kBatch; ++b) raw[b].load(p + b * kStep, policy);
       p += kBatch * kStep;
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b) sq.take(raw[b]);
     }
     for (; v < whole; v += kListThreads, p += kStep) {
       Raw<T> raw;
-      raw.load(p);
+      raw.load(p, policy);
       sq.take(raw);
     }
   } else {
@@ -352,13 +367,13 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
 
 template <uint32_t T, bool kFactor>
 __device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, Rows<T> rows,
-                                            uint32_t count) {
+                                            uint32_t count, uint64_t policy) {
   constexpr uint32_t kBatch = 2;
   for (uint32_t e = threadIdx.x * kVec; e < count; e += kBatch * kListThreads * kVec) {
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
-      rows.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count));
+      rows.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count), policy);
       rows.next_vector();
     }
 #pragma unroll
@@ -373,10 +388,11 @@ __device__ __forceinline__ double unit_squares(const GradUnit& u, const GradList
                                                float factor, uint32_t& top) {
   Squares<T, kFactor> sq;
   sq.factor = factor;
+  const uint64_t policy = blockIdx.x < list.keep ? l2_first_out() : l2_normal();
   if (kRows && (u.flags & kGradPitched))
-    row_squares(sq, Rows<T>(u, list), u.count);
+    row_squares(sq, Rows<T>(u, list), u.count, policy);
   else
-    flat_squares(sq, static_cast<const uint8_t*>(u.ptr), u.count);
+    flat_squares(sq, static_cast<const uint8_t*>(u.ptr), u.count, policy);
   top = top_f32<T>(sq.top);
   return sq.acc;
 }
@@ -570,7 +586,9 @@ __device__ __forceinline__ void store8(void* p, const float (&y)[8]) {
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    __stcs(static_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+    asm volatile("st.global.L2::cache_hint.v4.b32 [%0], {%1,%2,%3,%4}, %5;" ::"l"(p), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "l"(l2_first_out())
+                 : "memory");
   }
 }
 template <uint32_t T>
@@ -643,10 +661,11 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
   uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
   uint32_t v = threadIdx.x;
   if (reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
+    const uint64_t policy = l2_first_out();
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b)  // on their way while the norm is finished
-      if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep);
+      if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep, policy);
     if (!clip_ready(result, waited)) return;
     const ClipFactor f(__ldcg(result + 1), scale);
     while (v < whole) {
@@ -657,7 +676,7 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
       v += kBatch * kListThreads;
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b)
-        if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep);
+        if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep, policy);
     }
   } else {
     if (!clip_ready(result, waited)) return;
@@ -691,7 +710,7 @@ __device__ __forceinline__ void clip_rows(Rows<T> src, Rows<O> dst, uint32_t cou
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
-      src.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count));
+      src.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count), l2_first_out());
       src.next_vector();
     }
 #pragma unroll
@@ -812,7 +831,7 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
       for (uint32_t b = 0; b < kBatch; ++b) {
         const uint32_t i = v + b * kListThreads;
         if (i < whole) {
-          raw[b].load(from + i * kVecBytes<T>);
+          raw[b].load(from + i * kVecBytes<T>, l2_first_out());
           if (!overwrite) load_acc(to + i * kVec, old[b]);
         }
       }
@@ -852,10 +871,10 @@ __device__ __forceinline__ void accumulate_rows(Rows<T> src, float* dst, uint32_
     float old[8];
     if (wide && n == kVec) {
       if (!overwrite) load_acc(dst + e, old);
-      src.load(raw, n);
+      src.load(raw, n, l2_first_out());
       add_raw<T>(raw, old, overwrite, dst + e);
     } else {
-      src.load(raw, n);
+      src.load(raw, n, l2_first_out());
       float x[8];
       raw.unpack(x);
 #pragma unroll
@@ -909,7 +928,7 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
     for (uint32_t b = 0; b < kBatch; ++b) {
       const uint32_t e = (v0 + b * kListThreads) * kVec;
       const uint32_t n = vector_elems(e, u.count);
-      src.load(raw[b], n);
+      src.load(raw[b], n, l2_first_out());
       src.next_vector();
 #pragma unroll
       for (uint32_t j = 0; j < kVec; ++j) old[b][j] = 0.0f;

@@ -30,12 +30,13 @@ struct slm_grad_list {
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
+  uint32_t keep = 0;  // see GradListView
   GradTensor* d_tensors = nullptr;
   GradUnit* d_units = nullptr;
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        types, elements};
+                        types, keep, elements};
   }
 };
 
@@ -167,6 +168,12 @@ int upload_list(slm_grad_list* l) {
       u.flags = t.flags;
       u.offset = t.offset + e;
     }
+  }
+  l->keep = l->n_units;
+  for (uint64_t bytes = 0; l->keep > 0; --l->keep) {
+    const GradUnit& u = table[l->keep - 1];
+    bytes += uint64_t(u.count) * type_bytes(u.flags & kGradTypeMask);
+    if (bytes > kGradKeepBytes) break;
   }
   int st;
   const size_t tensor_bytes = l->tensors.size() * sizeof(GradTensor);
