@@ -24,8 +24,10 @@
 namespace slmopt {
 namespace {
 
-constexpr uint32_t kListThreads = 256;
-constexpr uint32_t kFinalThreads = 1024;
+constexpr uint32_t kListThreads = 256;  // of one unit
+
+// The thread's index among a unit's 256 (a block may work on several units).
+__device__ __forceinline__ uint32_t unit_thread() { return threadIdx.x % kListThreads; }
 
 // ---- L2 priorities ---------------------------------------------------------------
 // What a kernel reads or writes for the last time leaves the L2 first; what the
@@ -180,7 +182,7 @@ struct Rows {
   uint64_t step;      // bytes, before a wrap
   uint64_t wrap;      // bytes from a row's end to the next row
   __device__ __forceinline__ Rows(const GradUnit& u, const GradListView& list) {
-    const uint32_t e = threadIdx.x * kVec;
+    const uint32_t e = unit_thread() * kVec;
     p = static_cast<uint8_t*>(const_cast<void*>(u.ptr));
     if (u.flags & kGradPitched) {
       const GradTensor* t = list.tensors + u.tensor;
@@ -330,7 +332,7 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;  // 64 bytes of loads per thread in flight
   constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
   const uint32_t whole = count / kVec;
-  uint32_t v = threadIdx.x;
+  uint32_t v = unit_thread();
   if (reinterpret_cast<uintptr_t>(base) % kVecBytes<T> == 0u) {
     const uint8_t* p = base + v * kVecBytes<T>;
     for (; v + (kBatch - 1) * kListThreads < whole; v += kBatch * kListThreads) {
@@ -358,7 +360,7 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
       sq.take(raw);
     }
   }
-  if (threadIdx.x == whole % kListThreads && count % kVec) {
+  if (unit_thread() == whole % kListThreads && count % kVec) {
     Raw<T> raw;
     gather_flat(raw, base + whole * kVecBytes<T>, count % kVec);
     sq.take(raw);
@@ -369,7 +371,7 @@ template <uint32_t T, bool kFactor>
 __device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, Rows<T> rows,
                                             uint32_t count, uint64_t policy) {
   constexpr uint32_t kBatch = 2;
-  for (uint32_t e = threadIdx.x * kVec; e < count; e += kBatch * kListThreads * kVec) {
+  for (uint32_t e = unit_thread() * kVec; e < count; e += kBatch * kListThreads * kVec) {
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
@@ -397,39 +399,51 @@ __device__ __forceinline__ double unit_squares(const GradUnit& u, const GradList
   return sq.acc;
 }
 
-// Folds (sum, top) over the block; results valid in thread 0.
-template <uint32_t kThreads>
-__device__ __forceinline__ void fold_block(double& v, uint32_t& top, double* s_sum,
-                                           uint32_t* s_top) {
+__device__ __forceinline__ double fold_warp(double v) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) v = __dadd_rn(v, __shfl_down_sync(kFull, v, off));
-  top = __reduce_max_sync(kFull, top);
-  if ((threadIdx.x & 31u) == 0u) {
-    s_sum[threadIdx.x >> 5] = v;
-    s_top[threadIdx.x >> 5] = top;
+  return v;
+}
+// The halving tree over n (a power of two) warps' sums.
+template <int n>
+__device__ __forceinline__ double fold_sums(const double* sums) {
+  double w[n];
+#pragma unroll
+  for (int i = 0; i < n; ++i) w[i] = sums[i];
+#pragma unroll
+  for (int off = n / 2; off >= 1; off >>= 1) {
+#pragma unroll
+    for (int i = 0; i < off; ++i) w[i] = __dadd_rn(w[i], w[i + off]);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    constexpr int kWarps = int(kThreads / 32);
-    double w[kWarps];
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      w[i] = s_sum[i];
-      top = max(top, s_top[i]);
-    }
-#pragma unroll
-    for (int off = kWarps / 2; off >= 1; off >>= 1) {
-#pragma unroll
-      for (int i = 0; i < off; ++i) w[i] = __dadd_rn(w[i], w[i + off]);
-    }
-    v = w[0];
-  }
+  return w[0];
 }
 
-__device__ __forceinline__ void store_partial(const GradPartial* partials, double sum,
-                                              uint32_t top) {
-  *reinterpret_cast<uint4*>(const_cast<GradPartial*>(partials)) =
-      make_uint4(uint32_t(__double2loint(sum)), uint32_t(__double2hiint(sum)), top, 0u);
+// Folds a unit's 256 lanes and stores the partial.  `slot` is shared memory of
+// these 256 threads alone, `barrier` theirs too.
+struct UnitSlot {
+  double sum[kListThreads / 32];
+  uint32_t top[kListThreads / 32];
+};
+__device__ __forceinline__ void unit_barrier(uint32_t barrier) {
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kListThreads) : "memory");
+}
+__device__ __forceinline__ void fold_unit(double v, uint32_t top, UnitSlot& slot,
+                                          uint32_t barrier, GradPartial* to) {
+  v = fold_warp(v);
+  top = __reduce_max_sync(kFull, top);
+  const uint32_t warp = unit_thread() / 32u;
+  if ((threadIdx.x & 31u) == 0u) {
+    slot.sum[warp] = v;
+    slot.top[warp] = top;
+  }
+  unit_barrier(barrier);
+  if (unit_thread() == 0u) {
+#pragma unroll
+    for (uint32_t i = 0; i < kListThreads / 32; ++i) top = max(top, slot.top[i]);
+    const double sum = fold_sums<kListThreads / 32>(slot.sum);
+    *reinterpret_cast<uint4*>(to) =
+        make_uint4(uint32_t(__double2loint(sum)), uint32_t(__double2hiint(sum)), top, 0u);
+  }
 }
 
 template <bool kFactor, bool kRows>
@@ -445,61 +459,151 @@ __device__ __forceinline__ double unit_squares_any(const GradUnit& u, const Grad
 }
 
 template <bool kRows>
+__device__ __forceinline__ void unit_partial(const GradListView& list, const GradUnit& u,
+                                             float factor, UnitSlot& slot, uint32_t barrier,
+                                             GradPartial* to) {
+  uint32_t top = 0u;
+  const double sum = factor == 1.0f ? unit_squares_any<false, kRows>(u, list, factor, top)
+                                    : unit_squares_any<true, kRows>(u, list, factor, top);
+  fold_unit(sum, top, slot, barrier, to);
+}
+
+// ---- the norm from the partials ----------------------------------------------------
+// The fixed tree over a run of partials: 1,024 lanes, lane t adds partials t,
+// t + 1024, ... in order; lanes fold by warps of 32, the 32 warps' sums by halves.
+// kThreads threads hold 1,024 / kThreads lanes each, with 8 loads in flight.
+constexpr uint32_t kLanes = 1024;
+struct LaneSlot {
+  double sum[kLanes / 32];
+  uint32_t top[kLanes / 32];
+};
+template <uint32_t kThreads>
+__device__ __forceinline__ void sum_partials(const GradPartial* partials, uint32_t count,
+                                             LaneSlot& slot, double& sum, uint32_t& top) {
+  constexpr uint32_t kHold = kLanes / kThreads;
+  constexpr uint32_t kAhead = kHold < 8 ? 8 / kHold : 1;  // steps of kLanes loaded together
+  double v[kHold];
+  top = 0u;
+#pragma unroll
+  for (uint32_t h = 0; h < kHold; ++h) v[h] = 0.0;
+  for (uint32_t i0 = threadIdx.x; i0 < count; i0 += kAhead * kLanes) {
+    uint4 q[kAhead][kHold];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+#pragma unroll
+      for (uint32_t h = 0; h < kHold; ++h) {
+        const uint32_t i = i0 + a * kLanes + h * kThreads;
+        q[a][h] = i < count ? __ldcg(reinterpret_cast<const uint4*>(partials + i))
+                            : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+#pragma unroll
+      for (uint32_t h = 0; h < kHold; ++h) {
+        v[h] = __dadd_rn(v[h], __hiloint2double(int(q[a][h].y), int(q[a][h].x)));
+        top = max(top, q[a][h].z);
+      }
+    }
+  }
+  top = __reduce_max_sync(kFull, top);
+#pragma unroll
+  for (uint32_t h = 0; h < kHold; ++h) {
+    v[h] = fold_warp(v[h]);
+    const uint32_t warp = (threadIdx.x + h * kThreads) / 32u;
+    if ((threadIdx.x & 31u) == 0u) {
+      slot.sum[warp] = v[h];
+      slot.top[warp] = top;
+    }
+  }
+  __syncthreads();
+  sum = 0.0;
+  if (threadIdx.x < 32u) {
+    // The halving tree over 32 sums is a shuffle tree over a warp.
+    sum = fold_warp(slot.sum[threadIdx.x]);
+    top = __reduce_max_sync(kFull, slot.top[threadIdx.x]);
+  }
+}
+
+// The f64 sum of the unscaled squares.
+__device__ __forceinline__ double unscaled_sum(double sum, float scale) {
+  const double s = __dmul_rn(static_cast<double>(scale), static_cast<double>(square_factor(scale)));
+  return s == 1.0 ? sum : __ddiv_rn(sum, __dmul_rn(s, s));
+}
+__device__ __forceinline__ float unscaled_top(uint32_t top, float scale) {
+  return __fdiv_rn(__uint_as_float(top), scale);
+}
+
+__device__ __forceinline__ void write_tensor(const GradListOut& out, uint32_t t, double sum,
+                                             uint32_t top, float scale, int kind) {
+  const float largest = unscaled_top(top, scale);
+  if (out.tensor_norms)
+    out.tensor_norms[t] =
+        kind != 0 ? largest : __double2float_rn(__dsqrt_rn(unscaled_sum(sum, scale)));
+  if (out.tensor_max) out.tensor_max[t] = largest;
+}
+
+// The four values of a call: norm, clip scale, largest magnitude, non-finite flag.
+__device__ __forceinline__ float4 norm_values(double raw, uint32_t top, float scale,
+                                              float max_norm, int kind) {
+  const double sum = unscaled_sum(raw, scale);
+  const float largest = unscaled_top(top, scale);
+  const float norm = kind != 0 ? largest : __double2float_rn(__dsqrt_rn(sum));
+  // The flat step's formula: the sum rounded once to f32, f32 root and quotient.
+  const float root = kind != 0 ? largest : __fsqrt_rn(__double2float_rn(sum));
+  const bool bad = !finite_f32(norm) || !finite_f32(largest) || !finite_f32(root);
+  float clip = 1.0f;
+  if (bad)
+    clip = 0.0f;
+  else if (root > 0.0f)
+    clip = fminf(__fdiv_rn(max_norm, root), 1.0f);
+  return make_float4(norm, clip, largest, bad ? 1.0f : 0.0f);
+}
+__device__ __forceinline__ void write_norm(const GradListOut& out, const float4& v, double sum) {
+  out.result[0] = v.x;
+  out.result[1] = v.y;
+  out.result[2] = v.z;
+  out.result[3] = v.w;
+  if (out.sum_squares) *out.sum_squares = sum;
+}
+
+// The step's decision (clip, skip, scaler).
+__device__ __forceinline__ void write_step(double raw, uint32_t top, DeviceScaler* scaler,
+                                           DeviceStepState* st, const FinalizeParams& fp) {
+  const float scale = fp.dynamic ? scaler->scale : fp.static_scale;
+  const double sum = unscaled_sum(raw, scale);
+  const uint32_t nonfinite =
+      !isfinite(sum) || !finite_f32(unscaled_top(top, scale)) ? 1u : 0u;
+  const StepDecision d =
+      decide_step(sum, nonfinite, scale, fp.dynamic ? scaler->good_steps : 0u, fp);
+  write_decision(d, sum, nonfinite, scale, st, scaler, fp);
+  st->result_nonfinite = 0u;
+}
+
+// scaler: where the loss scale is, if it is on the device.  The norm is finished
+// by a kernel of its own: a completion counter would have to be shared by
+// concurrent calls of a list, and cost more than the chained launch (4.5M
+// elements: 11.9 us with the last of 1,107 blocks finishing, 8.2 us with two
+// kernels).
+template <bool kRows>
 __global__ void __launch_bounds__(kListThreads, kRows ? 5 : 8)
     list_norm_kernel(GradListView list, float scale, const DeviceScaler* scaler,
                      GradPartial* partials) {
-  __shared__ double s_sum[kListThreads / 32];
-  __shared__ uint32_t s_top[kListThreads / 32];
+  __shared__ UnitSlot slot;
   const GradUnit u = load_unit(list.units, blockIdx.x);
   // The kernels behind may start to read gradients once all blocks are here, so
   // their producers must be done by then: wait first.
   pdl_wait();
   pdl_trigger();
-  const float factor = square_factor(scaler ? scaler->scale : scale);
-  uint32_t top = 0u;
-  double sum = factor == 1.0f
-                   ? unit_squares_any<false, kRows>(u, list, factor, top)
-                   : unit_squares_any<true, kRows>(u, list, factor, top);
-  fold_block<kListThreads>(sum, top, s_sum, s_top);
-  if (threadIdx.x == 0) store_partial(partials + blockIdx.x, sum, top);
+  unit_partial<kRows>(list, u, square_factor(scaler ? scaler->scale : scale), slot, 1u,
+                      partials + blockIdx.x);
 }
 
-// Thread t adds partials t, t + 1024, ... of a run in order, 8 loads in flight;
-// then the block folds.  The sum is that of the unscaled squares.  Valid in
-// thread 0.
-__device__ __forceinline__ void sum_partials(const GradPartial* partials, uint32_t count,
-                                             float scale, double& v, uint32_t& top,
-                                             double* s_sum, uint32_t* s_top) {
-  v = 0.0;
-  top = 0u;
-  for (uint32_t i0 = threadIdx.x; i0 < count; i0 += 8 * kFinalThreads) {
-    uint4 q[8];
-#pragma unroll
-    for (uint32_t b = 0; b < 8; ++b) {
-      const uint32_t i = i0 + b * kFinalThreads;
-      q[b] = i < count ? __ldcg(reinterpret_cast<const uint4*>(partials + i))
-                       : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-    for (uint32_t b = 0; b < 8; ++b) {
-      v = __dadd_rn(v, __hiloint2double(int(q[b].y), int(q[b].x)));
-      top = max(top, q[b].z);
-    }
-  }
-  fold_block<kFinalThreads>(v, top, s_sum, s_top);
-  const double s = __dmul_rn(static_cast<double>(scale), static_cast<double>(square_factor(scale)));
-  v = __ddiv_rn(v, __dmul_rn(s, s));
-}
-
-__device__ __forceinline__ float unscaled_top(uint32_t top, float scale) {
-  return __fdiv_rn(__uint_as_float(top), scale);
-}
-
-__global__ void __launch_bounds__(kFinalThreads)
+// Block 0: the list's values; one more block per tensor for the tensors' own.
+__global__ void __launch_bounds__(kLanes)
     list_finalize_kernel(GradListView list, const GradPartial* partials, float scale,
                          float max_norm, int kind, GradListOut out) {
-  __shared__ double s_sum[kFinalThreads / 32];
-  __shared__ uint32_t s_top[kFinalThreads / 32];
+  __shared__ LaneSlot lanes;
   pdl_trigger();
   uint32_t begin = 0u, count = list.n_units;
   if (blockIdx.x > 0) {
@@ -512,48 +616,25 @@ __global__ void __launch_bounds__(kFinalThreads)
   pdl_wait();
   double sum;
   uint32_t top;
-  sum_partials(partials + begin, count, scale, sum, top, s_sum, s_top);
+  sum_partials<kLanes>(partials + begin, count, lanes, sum, top);
   if (threadIdx.x != 0) return;
-  const float largest = unscaled_top(top, scale);
-  const float norm = kind != 0 ? largest : __double2float_rn(__dsqrt_rn(sum));
-  if (blockIdx.x > 0) {
-    if (out.tensor_norms) out.tensor_norms[blockIdx.x - 1u] = norm;
-    if (out.tensor_max) out.tensor_max[blockIdx.x - 1u] = largest;
-    return;
-  }
-  // The flat step's formula: the sum rounded once to f32, f32 root and quotient.
-  const float root = kind != 0 ? largest : __fsqrt_rn(__double2float_rn(sum));
-  const bool bad = !finite_f32(norm) || !finite_f32(largest) || !finite_f32(root);
-  float clip = 1.0f;
-  if (bad)
-    clip = 0.0f;
-  else if (root > 0.0f)
-    clip = fminf(__fdiv_rn(max_norm, root), 1.0f);
-  out.result[0] = norm;
-  out.result[1] = clip;
-  out.result[2] = largest;
-  out.result[3] = bad ? 1.0f : 0.0f;
-  if (out.sum_squares) *out.sum_squares = sum;
+  if (blockIdx.x > 0)
+    write_tensor(out, blockIdx.x - 1u, sum, top, scale, kind);
+  else
+    write_norm(out, norm_values(sum, top, scale, max_norm, kind), unscaled_sum(sum, scale));
 }
 
-__global__ void __launch_bounds__(kFinalThreads)
+// The step's decision from the partials.
+__global__ void __launch_bounds__(kLanes)
     list_decide_kernel(GradListView list, const GradPartial* partials, DeviceScaler* scaler,
                        DeviceStepState* st, FinalizeParams fp) {
-  __shared__ double s_sum[kFinalThreads / 32];
-  __shared__ uint32_t s_top[kFinalThreads / 32];
+  __shared__ LaneSlot lanes;
   pdl_trigger();
   pdl_wait();
-  const float scale = fp.dynamic ? scaler->scale : fp.static_scale;
   double sum;
   uint32_t top;
-  sum_partials(partials, list.n_units, scale, sum, top, s_sum, s_top);
-  if (threadIdx.x != 0) return;
-  const uint32_t nonfinite =
-      !isfinite(sum) || !finite_f32(unscaled_top(top, scale)) ? 1u : 0u;
-  const StepDecision d =
-      decide_step(sum, nonfinite, scale, fp.dynamic ? scaler->good_steps : 0u, fp);
-  write_decision(d, sum, nonfinite, scale, st, scaler, fp);
-  st->result_nonfinite = 0u;
+  sum_partials<kLanes>(partials, list.n_units, lanes, sum, top);
+  if (threadIdx.x == 0) write_step(sum, top, scaler, st, fp);
 }
 
 // ---- clip ----------------------------------------------------------------------
@@ -638,20 +719,30 @@ __device__ __forceinline__ void clip_raw(const Raw<T>& raw, const ClipFactor& f,
   store8<O>(to, x);
 }
 
-// Waits for the norm, once per block; false when a gradient is not finite,
-// which leaves the outputs alone.
-__device__ __forceinline__ bool clip_ready(const float* result, bool& waited) {
-  if (!waited) pdl_wait();
-  waited = true;
-  return __ldcg(result + 3) == 0.0f;
-}
+// What the clip needs of the norm, which may still be on its way: it is waited
+// for once per block, after the first loads have been issued.
+struct ClipState {
+  const float* result;  // in global memory, while not `known`
+  float clip, bad;
+  bool known;
+  // False when a gradient is not finite, which leaves the outputs alone.
+  __device__ __forceinline__ bool ready() {
+    if (!known) {
+      pdl_wait();
+      clip = __ldcg(result + 1);
+      bad = __ldcg(result + 3);
+      known = true;
+    }
+    return bad == 0.0f;
+  }
+};
 
 // One unit of the clip, each element read and written by the same thread.
 // Contiguous on both sides: vectors start at the output's boundaries, and the
 // input is shifted where it lies off them.
 template <uint32_t T, uint32_t O>
 __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint32_t count,
-                                          float scale, const float* result, bool& waited) {
+                                          float scale, ClipState& state) {
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
   constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
   const uint32_t peel = peel_of<O>(dst, count);
@@ -659,15 +750,15 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
   uint8_t* to = dst + peel * kSize<O>;
   const uint32_t whole = (count - peel) / kVec;
   uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
-  uint32_t v = threadIdx.x;
+  uint32_t v = unit_thread();
   if (reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
     const uint64_t policy = l2_first_out();
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b)  // on their way while the norm is finished
       if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep, policy);
-    if (!clip_ready(result, waited)) return;
-    const ClipFactor f(__ldcg(result + 1), scale);
+    if (!state.ready()) return;
+    const ClipFactor f(state.clip, scale);
     while (v < whole) {
 #pragma unroll
       for (uint32_t b = 0; b < kBatch; ++b)
@@ -679,8 +770,8 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
         if (v + b * kListThreads < whole) raw[b].load(from + v * kVecBytes<T> + b * kStep, policy);
     }
   } else {
-    if (!clip_ready(result, waited)) return;
-    const ClipFactor f(__ldcg(result + 1), scale);
+    if (!state.ready()) return;
+    const ClipFactor f(state.clip, scale);
     // The blocks of the first and the last vector can reach beyond the tensor.
     for (v += 1u; v + 1u < whole; v += kListThreads) {
       Raw<T> raw;
@@ -692,8 +783,8 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
       tail = whole > 1u ? tail - kVec : head;
     }
   }
-  const ClipFactor f(__ldcg(result + 1), scale);
-  for (uint32_t e = threadIdx.x; e < head + (count - tail); e += kListThreads) {
+  const ClipFactor f(state.clip, scale);
+  for (uint32_t e = unit_thread(); e < head + (count - tail); e += kListThreads) {
     const uint32_t i = e < head ? e : tail + (e - head);
     store1<O>(dst, i, f(from_bits<T>(elem_bits<T>(src, i))));
   }
@@ -702,11 +793,11 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
 // Rows on either side.
 template <uint32_t T, uint32_t O>
 __device__ __forceinline__ void clip_rows(Rows<T> src, Rows<O> dst, uint32_t count, float scale,
-                                          const float* result, bool& waited) {
+                                          ClipState& state) {
   constexpr uint32_t kBatch = 2;
-  if (!clip_ready(result, waited)) return;
-  const ClipFactor f(__ldcg(result + 1), scale);
-  for (uint32_t e = threadIdx.x * kVec; e < count; e += kBatch * kListThreads * kVec) {
+  if (!state.ready()) return;
+  const ClipFactor f(state.clip, scale);
+  for (uint32_t e = unit_thread() * kVec; e < count; e += kBatch * kListThreads * kVec) {
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
@@ -738,51 +829,134 @@ __device__ __forceinline__ void clip_rows(Rows<T> src, Rows<O> dst, uint32_t cou
 template <uint32_t T, uint32_t O, bool kRows>
 __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
                                           const GradListView& list, const GradListView& out,
-                                          float scale, const float* result, bool& waited) {
+                                          float scale, ClipState& state) {
   if (kRows && ((u.flags | o.flags) & kGradPitched))
-    clip_rows<T, O>(Rows<T>(u, list), Rows<O>(o, out), u.count, scale, result, waited);
+    clip_rows<T, O>(Rows<T>(u, list), Rows<O>(o, out), u.count, scale, state);
   else
     clip_flat<T, O>(static_cast<const uint8_t*>(u.ptr),
-                    static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale, result,
-                    waited);
+                    static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale,
+                    state);
 }
 
 // kOut: the output type (units written in another one are left to the launch for
 // theirs), or in place.  All nine pairs of types in one kernel would spill.
 constexpr uint32_t kOutSame = 3u;
 template <uint32_t kOut, bool kRows>
+__device__ __forceinline__ void clip_any(const GradListView& list, const GradListView& out,
+                                         uint32_t i, float scale, ClipState& state) {
+  constexpr bool kSame = kOut == kOutSame;
+  const GradUnit u = load_unit(list.units, i);
+  const GradUnit o = kSame ? u : load_unit(out.units, i);
+  if (!kSame && (o.flags & kGradTypeMask) != kOut) return;
+  switch (u.flags & kGradTypeMask) {
+    case kGradF32:
+      return clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows>(u, o, list, out, scale, state);
+    case kGradBf16:
+      return clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows>(u, o, list, out, scale, state);
+    default:
+      return clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows>(u, o, list, out, scale, state);
+  }
+}
+
+template <uint32_t kOut, bool kRows>
 __global__ void __launch_bounds__(kListThreads, 4)
     list_clip_kernel(GradListView list, GradListView out, float scale, const float* result) {
-  constexpr bool kSame = kOut == kOutSame;
-  bool waited = false;
+  ClipState state{result, 0.0f, 0.0f, false};
   // In place with a loss scale of one there may be nothing to do: look before
   // anything is loaded.
-  if (kSame && scale == 1.0f) {
-    pdl_wait();
-    waited = true;
-    if (__ldcg(result + 1) == 1.0f || __ldcg(result + 3) != 0.0f) return;
-  }
+  if (kOut == kOutSame && scale == 1.0f && (!state.ready() || state.clip == 1.0f)) return;
   // From the end of the list to its start: the norm pass has read the end last,
   // so the part of the gradients that the L2 still holds is read first.
-  for (uint32_t b = blockIdx.x; b < list.n_units; b += gridDim.x) {
-    const uint32_t i = list.n_units - 1u - b;
-    const GradUnit u = load_unit(list.units, i);
-    const GradUnit o = kSame ? u : load_unit(out.units, i);
-    if (!kSame && (o.flags & kGradTypeMask) != kOut) continue;
-    switch (u.flags & kGradTypeMask) {
-      case kGradF32:
-        clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows>(u, o, list, out, scale, result,
-                                                            waited);
-        break;
-      case kGradBf16:
-        clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows>(u, o, list, out, scale, result,
-                                                              waited);
-        break;
-      default:
-        clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows>(u, o, list, out, scale, result,
-                                                            waited);
-        break;
+  for (uint32_t b = blockIdx.x; b < list.n_units; b += gridDim.x)
+    clip_any<kOut, kRows>(list, out, list.n_units - 1u - b, scale, state);
+}
+
+// ---- small lists -------------------------------------------------------------------
+// One launch of one thread-block cluster for lists whose time is latency: the
+// partials, a cluster barrier, and the norm (every block for itself where it
+// goes on to clip) from the same tree.  A block works on 4 units at a time; unit
+// i goes to block i % cluster first.
+constexpr uint32_t kSmallThreads = 1024;
+constexpr uint32_t kSmallGroups = kSmallThreads / kListThreads;
+constexpr uint32_t kSmallNorm = 4u, kSmallStep = 5u;  // kMode; 0..3: clip to kOut
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The tree over at most 1,024 partials by one warp; valid in lane 0.
+__device__ __forceinline__ void sum_partials_warp(const GradPartial* partials, uint32_t count,
+                                                  double& sum, uint32_t& top) {
+  const uint32_t lane = threadIdx.x & 31u;
+  double mine = 0.0;
+  top = 0u;
+  for (uint32_t w = 0; w * 32u < count; ++w) {
+    const uint32_t i = w * 32u + lane;
+    const uint4 q = i < count ? __ldcg(reinterpret_cast<const uint4*>(partials + i))
+                              : make_uint4(0u, 0u, 0u, 0u);
+    const double s =
+        __shfl_sync(kFull, fold_warp(__hiloint2double(int(q.y), int(q.x))), 0);
+    if (lane == w) mine = s;
+    top = max(top, q.z);
+  }
+  sum = fold_warp(mine);
+  top = __reduce_max_sync(kFull, top);
+}
+
+template <uint32_t kMode>
+__global__ void __launch_bounds__(kSmallThreads, 1)
+    list_small_kernel(GradListView list, GradListView to, float scale, float max_norm, int kind,
+                      GradListOut out, GradPartial* partials, DeviceScaler* scaler,
+                      DeviceStepState* st, FinalizeParams fp) {
+  __shared__ UnitSlot slots[kSmallGroups];
+  __shared__ LaneSlot lanes;
+  __shared__ float2 s_clip;
+  constexpr bool kClip = kMode <= kOutSame;
+  const uint32_t group = threadIdx.x / kListThreads;
+  const uint32_t begin = blockIdx.x + gridDim.x * group, step = gridDim.x * kSmallGroups;
+  pdl_wait();
+  if (!kClip) pdl_trigger();  // a clip's outputs may be what the next kernel loads early
+  if (kMode == kSmallStep && fp.dynamic) scale = scaler->scale;
+  const float factor = square_factor(scale);
+  for (uint32_t i = begin; i < list.n_units; i += step) {
+    unit_partial<true>(list, load_unit(list.units, i), factor, slots[group], 1u + group,
+                       partials + i);
+    unit_barrier(1u + group);  // the slot is free again
+  }
+  cluster_barrier();
+  if (kClip || blockIdx.x == 0u) {
+    double sum;
+    uint32_t top;
+    sum_partials<kSmallThreads>(partials, list.n_units, lanes, sum, top);
+    if (threadIdx.x == 0u) {
+      if constexpr (kMode == kSmallStep) {
+        write_step(sum, top, scaler, st, fp);
+      } else {
+        const float4 v = norm_values(sum, top, scale, max_norm, kind);
+        s_clip = make_float2(v.y, v.w);
+        if (blockIdx.x == 0u) write_norm(out, v, unscaled_sum(sum, scale));
+      }
     }
+  }
+  if (kMode != kSmallStep && (out.tensor_norms || out.tensor_max)) {
+    const uint32_t warp = blockIdx.x + gridDim.x * (threadIdx.x / 32u);
+    for (uint32_t t = warp; t < list.n_tensors; t += gridDim.x * (kSmallThreads / 32u)) {
+      const uint32_t first = __ldg(&list.tensors[t].first_unit);
+      const uint32_t end =
+          t + 1u < list.n_tensors ? __ldg(&list.tensors[t + 1u].first_unit) : list.n_units;
+      double sum;
+      uint32_t top;
+      sum_partials_warp(partials + first, end - first, sum, top);
+      if ((threadIdx.x & 31u) == 0u) write_tensor(out, t, sum, top, scale, kind);
+    }
+  }
+  if constexpr (kClip) {
+    __syncthreads();
+    ClipState state{nullptr, s_clip.x, s_clip.y, true};
+    if (!state.ready() || (kMode == kOutSame && scale == 1.0f && state.clip == 1.0f)) return;
+    for (uint32_t i = begin; i < list.n_units; i += step)
+      clip_any<kMode, true>(list, to, i, scale, state);
   }
 }
 
@@ -824,7 +998,7 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
   const uint32_t whole = (count - peel) / kVec;
   uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
   if (reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
-    for (uint32_t v = threadIdx.x; v < whole; v += kBatch * kListThreads) {
+    for (uint32_t v = unit_thread(); v < whole; v += kBatch * kListThreads) {
       Raw<T> raw[kBatch];
       float old[kBatch][8];
 #pragma unroll
@@ -843,7 +1017,7 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
     }
   } else {
     // The blocks of the first and the last vector can reach beyond the tensor.
-    for (uint32_t v = threadIdx.x + 1u; v + 1u < whole; v += kListThreads) {
+    for (uint32_t v = unit_thread() + 1u; v + 1u < whole; v += kListThreads) {
       Raw<T> raw;
       float old[8];
       raw.load_shifted(from + v * kVecBytes<T>);
@@ -855,7 +1029,7 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
       tail = whole > 1u ? tail - kVec : head;
     }
   }
-  for (uint32_t e = threadIdx.x; e < head + (count - tail); e += kListThreads) {
+  for (uint32_t e = unit_thread(); e < head + (count - tail); e += kListThreads) {
     const uint32_t i = e < head ? e : tail + (e - head);
     add_one<T>(src, i, overwrite, dst + i);
   }
@@ -865,7 +1039,7 @@ template <uint32_t T>
 __device__ __forceinline__ void accumulate_rows(Rows<T> src, float* dst, uint32_t count,
                                                 bool overwrite) {
   const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
-  for (uint32_t e = threadIdx.x * kVec; e < count; e += kListThreads * kVec) {
+  for (uint32_t e = unit_thread() * kVec; e < count; e += kListThreads * kVec) {
     const uint32_t n = vector_elems(e, count);
     Raw<T> raw;
     float old[8];
@@ -921,7 +1095,7 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
   const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
   double sum = 0.0;
   uint32_t m = 0u;
-  for (uint32_t v0 = threadIdx.x; v0 * kVec < u.count; v0 += kBatch * kListThreads) {
+  for (uint32_t v0 = unit_thread(); v0 * kVec < u.count; v0 += kBatch * kListThreads) {
     Raw<T> raw[kBatch];
     float old[kBatch][8];
 #pragma unroll
@@ -987,17 +1161,15 @@ __device__ __forceinline__ double accumulate_squares_any(const GradUnit& u,
 __global__ void __launch_bounds__(kListThreads)
     list_accumulate_norm_kernel(GradListView list, float* acc, int overwrite, float scale,
                                 const DeviceScaler* scaler, GradPartial* partials) {
-  __shared__ double s_sum[kListThreads / 32];
-  __shared__ uint32_t s_top[kListThreads / 32];
+  __shared__ UnitSlot slot;
   const GradUnit u = load_unit(list.units, blockIdx.x);
   pdl_wait();
   const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
-  double sum = factor == 1.0f
+  const double sum = factor == 1.0f
                    ? accumulate_squares_any<false>(u, list, acc, overwrite != 0, factor, top)
                    : accumulate_squares_any<true>(u, list, acc, overwrite != 0, factor, top);
-  fold_block<kListThreads>(sum, top, s_sum, s_top);
-  if (threadIdx.x == 0) store_partial(partials + blockIdx.x, sum, top);
+  fold_unit(sum, top, slot, 1u, partials + blockIdx.x);
 }
 
 // ---- the step's update ---------------------------------------------------------
@@ -1340,25 +1512,101 @@ cudaError_t launch_chained(void (*kernel)(Args...), uint32_t grid, uint32_t bloc
 
 }  // namespace
 
-cudaError_t launch_list_norm(const GradListView& list, float scale, const DeviceScaler* scaler,
-                             GradPartial* partials, cudaStream_t stream) {
-  if (list.n_units == 0) return cudaSuccess;
-  return launch_chained(list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units, kListThreads, 0, stream, list, scale, scaler,
-                        partials);
+namespace {
+template <uint32_t kMode>
+cudaError_t launch_small(const GradListView& list, const GradListView& to, float scale,
+                         float max_norm, int kind, const GradListOut& out, GradPartial* partials,
+                         DeviceScaler* scaler, DeviceStepState* st, const FinalizeParams& fp,
+                         cudaStream_t stream) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = list.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(list.cluster);
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, list_small_kernel<kMode>, list, to, scale, max_norm, kind, out,
+                            partials, scaler, st, fp);
 }
 
-cudaError_t launch_list_finalize(const GradListView& list, const GradPartial* partials,
-                                 float scale, float max_norm, int kind, const GradListOut& out,
-                                 cudaStream_t stream) {
+template <uint32_t kMode>
+bool small_fits(uint32_t cluster) {
+  if (cluster > 8 &&
+      cudaFuncSetAttribute(list_small_kernel<kMode>,
+                           cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, list_small_kernel<kMode>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return n > 0;
+}
+bool all_small_fit(uint32_t c) {
+  return small_fits<kGradF32>(c) && small_fits<kGradBf16>(c) && small_fits<kGradF16>(c) &&
+         small_fits<kOutSame>(c) && small_fits<kSmallNorm>(c) && small_fits<kSmallStep>(c);
+}
+
+// A list small enough for one cluster, on a device that can hold one.
+bool is_small(const GradListView& list) {
+  return list.cluster != 0u && list.n_units <= kGradSmallUnits;
+}
+}  // namespace
+
+uint32_t list_small_cluster() { return all_small_fit(16u) ? 16u : all_small_fit(8u) ? 8u : 0u; }
+
+cudaError_t launch_list_norm(const GradListView& list, float scale, float max_norm, int kind,
+                             const GradListOut& out, GradPartial* partials, cudaStream_t stream) {
+  if (is_small(list))
+    return launch_small<kSmallNorm>(list, list, scale, max_norm, kind, out, partials, nullptr,
+                                    nullptr, FinalizeParams{}, stream);
+  if (list.n_units > 0) {
+    const cudaError_t e = launch_chained(
+        list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units, kListThreads,
+        0, stream, list, scale, static_cast<const DeviceScaler*>(nullptr), partials);
+    if (e != cudaSuccess) return e;
+  }
   const uint32_t grid = 1u + (out.tensor_norms || out.tensor_max ? list.n_tensors : 0u);
-  return launch_chained(list_finalize_kernel, grid, kFinalThreads, 0, stream, list, partials,
-                        scale, max_norm, kind, out);
+  return launch_chained(list_finalize_kernel, grid, kLanes, 0, stream, list,
+                        static_cast<const GradPartial*>(partials), scale, max_norm, kind, out);
+}
+
+cudaError_t launch_list_norm_decide(const GradListView& list, GradPartial* partials,
+                                    DeviceScaler* scaler, DeviceStepState* st,
+                                    const FinalizeParams& fp, cudaStream_t stream) {
+  if (is_small(list))
+    return launch_small<kSmallStep>(list, list, fp.static_scale, 1.0f, 0, GradListOut{}, partials,
+                                    scaler, st, fp, stream);
+  const cudaError_t e = launch_chained(
+      list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units, kListThreads, 0,
+      stream, list, fp.static_scale, static_cast<const DeviceScaler*>(fp.dynamic ? scaler : nullptr),
+      partials);
+  if (e != cudaSuccess) return e;
+  return launch_list_decide(list, partials, scaler, st, fp, stream);
 }
 
 cudaError_t launch_list_decide(const GradListView& list, const GradPartial* partials,
                                DeviceScaler* scaler, DeviceStepState* st,
                                const FinalizeParams& fp, cudaStream_t stream) {
-  return launch_chained(list_decide_kernel, 1u, kFinalThreads, 0, stream, list, partials, scaler,
+  return launch_chained(list_decide_kernel, 1u, kLanes, 0, stream, list, partials, scaler,
                         st, fp);
 }
 
@@ -1376,17 +1624,27 @@ cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, fl
 }
 }  // namespace
 
-cudaError_t launch_list_clip(const GradListView& list, const GradListView& out, float scale,
-                             const float* result, bool in_place, cudaStream_t stream) {
-  if (list.n_units == 0) return cudaSuccess;
-  if (in_place) return launch_clip_to<kOutSame>(list, list, scale, result, stream);
-  cudaError_t e = cudaSuccess;
-  if (out.types & (1u << kGradF32))
-    e = launch_clip_to<kGradF32>(list, out, scale, result, stream);
-  if (e == cudaSuccess && (out.types & (1u << kGradBf16)))
-    e = launch_clip_to<kGradBf16>(list, out, scale, result, stream);
-  if (e == cudaSuccess && (out.types & (1u << kGradF16)))
-    e = launch_clip_to<kGradF16>(list, out, scale, result, stream);
+cudaError_t launch_list_clip(const GradListView& list, const GradListView& to, bool in_place,
+                             float scale, float max_norm, int kind, const GradListOut& out,
+                             GradPartial* partials, cudaStream_t stream) {
+  const bool one_type = in_place || (to.types & (to.types - 1u)) == 0u;
+  if (is_small(list) && one_type) {
+    const auto launch = in_place ? launch_small<kOutSame>
+                        : to.types == 1u << kGradF32  ? launch_small<kGradF32>
+                        : to.types == 1u << kGradBf16 ? launch_small<kGradBf16>
+                                                      : launch_small<kGradF16>;
+    return launch(list, to, scale, max_norm, kind, out, partials, nullptr, nullptr,
+                  FinalizeParams{}, stream);
+  }
+  cudaError_t e = launch_list_norm(list, scale, max_norm, kind, out, partials, stream);
+  if (e != cudaSuccess || list.n_units == 0) return e;
+  if (in_place) return launch_clip_to<kOutSame>(list, list, scale, out.result, stream);
+  if (to.types & (1u << kGradF32))
+    e = launch_clip_to<kGradF32>(list, to, scale, out.result, stream);
+  if (e == cudaSuccess && (to.types & (1u << kGradBf16)))
+    e = launch_clip_to<kGradBf16>(list, to, scale, out.result, stream);
+  if (e == cudaSuccess && (to.types & (1u << kGradF16)))
+    e = launch_clip_to<kGradF16>(list, to, scale, out.result, stream);
   return e;
 }
 

@@ -30,13 +30,13 @@ struct slm_grad_list {
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
-  uint32_t keep = 0;  // see GradListView
+  uint32_t keep = 0, cluster = 0;  // see GradListView
   GradTensor* d_tensors = nullptr;
   GradUnit* d_units = nullptr;
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        types, keep, elements};
+                        types, cluster, keep, elements};
   }
 };
 
@@ -148,6 +148,7 @@ int fill_list(slm_grad_list* l, const slm_grad_view* views, uint32_t n) {
 
 int upload_list(slm_grad_list* l) {
   l->unit_elems = grad_unit_elems(l->elements);
+  l->cluster = list_small_cluster();
   uint64_t units = 0;
   for (GradTensor& t : l->tensors) {
     t.first_unit = uint32_t(units);
@@ -218,16 +219,6 @@ int check_norm_call(const slm_grad_list* list, float loss_scale, float max_norm,
   return SLM_OK;
 }
 
-int norm_kernels(const slm_grad_list* list, float loss_scale, float max_norm, int kind,
-                 const GradListOut& out, void* workspace, cudaStream_t s) {
-  const GradListView v = list->view();
-  GradPartial* part = static_cast<GradPartial*>(workspace);
-  int st = cuda_status(launch_list_norm(v, loss_scale, nullptr, part, s), "list norm kernel");
-  if (st) return st;
-  return cuda_status(launch_list_finalize(v, part, loss_scale, max_norm, kind, out, s),
-                     "list finalize kernel");
-}
-
 // Whether an element of `out` lies on an element of `list` other than, for the
 // same tensor in the same layout and type, itself.
 bool collides(const slm_grad_list& list, const slm_grad_list& out) {
@@ -275,14 +266,10 @@ uint64_t slmopt::list_partial_bytes(const std::vector<uint64_t>& offsets) {
 
 int slmopt::enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list,
                               const slm_step_config* cfg, cudaStream_t s) {
-  const FinalizeParams fp = finalize_params(h, cfg);
-  GradPartial* part = static_cast<GradPartial*>(h->d_list_partials);
-  const GradListView v = list->view();
-  int st = h->cuda(launch_list_norm(v, fp.static_scale, fp.dynamic ? h->d_scaler : nullptr, part, s),
-                   "list norm kernel");
-  if (st) return st;
-  return h->cuda(launch_list_decide(v, part, h->d_scaler, h->d_state, fp, s),
-                 "list decide kernel");
+  return h->cuda(launch_list_norm_decide(list->view(),
+                                         static_cast<GradPartial*>(h->d_list_partials),
+                                         h->d_scaler, h->d_state, finalize_params(h, cfg), s),
+                 "list norm kernel");
 }
 
 int slmopt::enqueue_list_update(slm_opt_handle* h, const GradListView& list,
@@ -399,8 +386,10 @@ int slm_grad_list_norm(const slm_grad_list* list, float loss_scale, float max_no
   DeviceGuard guard(list->device);
   const GradListOut out{&result_device->norm, tensor_norms_device, tensor_max_device,
                         sum_squares_device};
-  return norm_kernels(list, loss_scale, max_norm, kind, out, workspace_device,
-                      static_cast<cudaStream_t>(stream));
+  return cuda_status(launch_list_norm(list->view(), loss_scale, max_norm, kind, out,
+                                      static_cast<GradPartial*>(workspace_device),
+                                      static_cast<cudaStream_t>(stream)),
+                     "list norm kernels");
 }
 
 int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, float loss_scale,
@@ -430,13 +419,12 @@ int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, floa
                   "an output tensor overlaps a gradient tensor without being that tensor");
   }
   DeviceGuard guard(list->device);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const GradListOut o{&result_device->norm, tensor_norms_device, tensor_max_device,
                       sum_squares_device};
-  if ((st = norm_kernels(list, loss_scale, max_norm, kind, o, workspace_device, s))) return st;
-  return cuda_status(launch_list_clip(list->view(), to->view(), loss_scale, &result_device->norm,
-                                      in_place, s),
-                     "list clip kernel");
+  return cuda_status(launch_list_clip(list->view(), to->view(), in_place, loss_scale, max_norm,
+                                      kind, o, static_cast<GradPartial*>(workspace_device),
+                                      static_cast<cudaStream_t>(stream)),
+                     "list clip kernels");
 }
 
 int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint64_t n,

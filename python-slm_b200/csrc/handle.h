@@ -36,7 +36,12 @@ struct DeviceGuard {
   bool ok = false;
   explicit DeviceGuard(int device) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    ok = cudaSetDevice(device) == cudaSuccess;
+    if (prev == device) {  // nothing to switch, nothing to restore
+      prev = -1;
+      ok = true;
+    } else {
+      ok = cudaSetDevice(device) == cudaSuccess;
+    }
   }
   ~DeviceGuard() {
     if (prev >= 0) cudaSetDevice(prev);

@@ -283,6 +283,8 @@ constexpr uint64_t kGradUnitsAimed = 8192;
 // 62.4, 60.9 / 62.1 / 65.4, 69.6.  More than that is not kept: the last pass's writes
 // are still in the L2.
 constexpr uint64_t kGradKeepBytes = uint64_t(24) << 20;
+// Lists of at most so many units are taken by one cluster in one launch.
+constexpr uint32_t kGradSmallUnits = 256;
 inline uint32_t grad_unit_elems(uint64_t total) {
   uint32_t u = kGradUnitMin;
   while (u < kGradUnitMax && total / u > kGradUnitsAimed) u *= 2;
@@ -295,6 +297,7 @@ struct GradListView {
   uint32_t unit_elems;
   uint32_t rows;   // whether any tensor is pitched
   uint32_t types;  // bit per type of a tensor with elements
+  uint32_t cluster;  // blocks of the cluster for small lists, see list_small_cluster
   uint32_t keep;   // units from here on stay in the L2 for a second pass
   uint64_t elements;
 };
@@ -311,20 +314,27 @@ struct __align__(16) GradPartial {
   uint32_t top;
   uint32_t reserved;
 };
-cudaError_t launch_list_norm(const GradListView& list, float scale, const DeviceScaler* scaler,
+// The norm of a list: the values of `out`.
+cudaError_t launch_list_norm(const GradListView& list, float scale, float max_norm, int kind,
+                             const GradListOut& out, GradPartial* partials, cudaStream_t stream);
+// The norm, then every element of `list` to `to` (in place: itself).
+cudaError_t launch_list_clip(const GradListView& list, const GradListView& to, bool in_place,
+                             float scale, float max_norm, int kind, const GradListOut& out,
                              GradPartial* partials, cudaStream_t stream);
-cudaError_t launch_list_finalize(const GradListView& list, const GradPartial* partials,
-                                 float scale, float max_norm, int kind, const GradListOut& out,
-                                 cudaStream_t stream);
-cudaError_t launch_list_clip(const GradListView& list, const GradListView& out, float scale,
-                             const float* result, bool in_place, cudaStream_t stream);
+// Blocks of the cluster that takes a small list in one launch; 0 if the current
+// device holds none.
+uint32_t list_small_cluster();
+// The norm pass of an optimizer handle: the decision (clip, skip, scaler) too.
+cudaError_t launch_list_norm_decide(const GradListView& list, GradPartial* partials,
+                                    DeviceScaler* scaler, DeviceStepState* st,
+                                    const FinalizeParams& fp, cudaStream_t stream);
 cudaError_t launch_list_accumulate(const GradListView& list, float* acc, int overwrite,
                                    cudaStream_t stream);
 // The last micro-batch: accumulates and forms the partials of the sums.
 cudaError_t launch_list_accumulate_norm(const GradListView& list, float* acc, int overwrite,
                                         float scale, const DeviceScaler* scaler,
                                         GradPartial* partials, cudaStream_t stream);
-// The handle's decision (clip, skip, scaler) from a list's partials.
+// The handle's decision from the partials of launch_list_accumulate_norm.
 cudaError_t launch_list_decide(const GradListView& list, const GradPartial* partials,
                                DeviceScaler* scaler, DeviceStepState* st,
                                const FinalizeParams& fp, cudaStream_t stream);

@@ -12,6 +12,8 @@ import ctypes
 
 from . import _lib
 
+# Workspaces up to this size are kept with the results of a call.
+_SHARED_BYTES = 4096
 _KINDS = {"l2": _lib.NORM_L2, "max": _lib.NORM_MAX}
 
 
@@ -54,50 +56,57 @@ class GradientNorm:
     is not finite (the clip scale is then 0.0) else 0.0; and with per_tensor each
     tensor's norm, then each tensor's largest magnitude."""
 
-    __slots__ = ("values", "_work", "_tensors")
+    __slots__ = ("_buffer", "_count", "_tensors")
 
-    def __init__(self, values, work, tensors: int):
-        self.values = values
-        self._work = work
+    def __init__(self, buffer, count: int, tensors: int):
+        # f32: the values, the f64 sum of squares, and scratch of the call.
+        self._buffer = buffer
+        self._count = count
         self._tensors = tensors
 
     @property
+    def values(self):
+        return self._buffer.as_strided((self._count,), (1,))
+
+    @property
     def norm(self):
-        return self.values[0]
+        return self._buffer[0]
 
     @property
     def clip_scale(self):
-        return self.values[1]
+        return self._buffer[1]
 
     @property
     def max_abs(self):
-        return self.values[2]
+        return self._buffer[2]
 
     @property
     def nonfinite(self):
-        return self.values[3]
+        return self._buffer[3]
 
     @property
     def sum_squares(self):
         """The f64 sum of squares (0-d tensor): what ranks that hold different
         tensors add up."""
-        return self._work[0]
+        import torch
+
+        return self._buffer[self._count:self._count + 2].view(torch.float64)[0]
 
     @property
     def tensor_norms(self):
-        if self.values.numel() == 4:
+        if self._count == 4:
             raise ValueError("the call was made without per_tensor")
-        return self.values[4:4 + self._tensors]
+        return self._buffer[4:4 + self._tensors]
 
     @property
     def tensor_max(self):
-        if self.values.numel() == 4:
+        if self._count == 4:
             raise ValueError("the call was made without per_tensor")
-        return self.values[4 + self._tensors:]
+        return self._buffer[4 + self._tensors:self._count]
 
     def read(self) -> _lib.ListNorm:
         """The four values on the host; waits for them."""
-        return _lib.ListNorm(*self.values[:4].tolist())
+        return _lib.ListNorm(*self._buffer[:4].tolist())
 
 
 class GradientList:
@@ -136,7 +145,9 @@ class GradientList:
         self._h = h
         self.elements = int(self.lib.slm_grad_list_elements(h))
         self._work_bytes = int(self.lib.slm_grad_list_workspace_bytes(h))
-        self._work_doubles = 2 + (self._work_bytes + 7) // 8
+        # What every call needs, looked up once.
+        self._empty, self._f32, self._index = torch.empty, torch.float32, self.device.index
+        self._norm_call, self._clip_call = self.lib.slm_grad_list_norm, self.lib.slm_grad_list_clip
 
     def _layout(self, t):
         import torch
@@ -201,37 +212,44 @@ class GradientList:
         return self._run(True, out, loss_scale, max_norm, kind, per_tensor, stream)
 
     def _run(self, write, out, loss_scale, max_norm, kind, per_tensor, stream) -> GradientNorm:
-        import torch
-
         code = _KINDS.get(kind)
         if code is None:
             raise ValueError('kind must be "l2" or "max"')
+        h = self._h or self.handle
         n = len(self.tensors)
-        values = torch.empty(4 + (2 * n if per_tensor else 0), dtype=torch.float32,
+        count = 4 + 2 * n if per_tensor else 4
+        # A small workspace shares the results' allocation; a large one is freed
+        # with the call instead of living as long as the results.
+        head = (count + 5) & ~3
+        small = self._work_bytes <= _SHARED_BYTES
+        buffer = self._empty(head + self._work_bytes // 4 if small else head, dtype=self._f32,
                              device=self.device)
-        # One allocation: the f64 sum of squares, then the workspace.
-        work = torch.empty(self._work_doubles, dtype=torch.float64, device=self.device)
-        s = _stream_handle(stream)
-        _use_on(values, work, s)
-        v, w = values.data_ptr(), work.data_ptr()
+        work = buffer if small else self._empty(self._work_bytes // 4, dtype=self._f32,
+                                                device=self.device)
+        s = stream if stream is None or type(stream) is int else _stream_handle(stream)
+        if _current_stream(self._index) != (s or 0):
+            _use_on(buffer, s)
+            if not small:
+                _use_on(work, s)
+        v = buffer.data_ptr()
+        w = v + 4 * head if small else work.data_ptr()
         norms, tops = (v + 16, v + 16 + 4 * n) if per_tensor else (None, None)
         if write:
-            st = self.lib.slm_grad_list_clip(self.handle, out.handle if out is not None else None,
-                                             loss_scale, max_norm, code, v, norms, tops, w, w + 16,
-                                             self._work_bytes, s)
+            to = None if out is None else out._h or out.handle
+            st = self._clip_call(h, to, loss_scale, max_norm, code, v, norms, tops, v + 4 * count,
+                                 w, self._work_bytes, s)
         else:
-            st = self.lib.slm_grad_list_norm(self.handle, loss_scale, max_norm, code, v, norms,
-                                             tops, w, w + 16, self._work_bytes, s)
-        _lib.check(st)
-        return GradientNorm(values, work, n)
+            st = self._norm_call(h, loss_scale, max_norm, code, v, norms, tops, v + 4 * count, w,
+                                 self._work_bytes, s)
+        if st:
+            _lib.check(st)
+        return GradientNorm(buffer, count, n)
 
     def accumulate(self, acc, overwrite: bool = False, stream=None) -> None:
         """acc (f32, one value per element, tensor after tensor) += the
         gradients, or acc = the gradients."""
-        import torch
-
-        if not acc.is_cuda or acc.device != self.device or acc.dtype != torch.float32 or \
-                not acc.is_contiguous() or acc.numel() != self.elements:
+        if acc.device != self.device or acc.dtype != self._f32 or not acc.is_contiguous() or \
+                acc.numel() != self.elements:
             raise ValueError("acc must be a contiguous f32 tensor on the list's device with one "
                              "value per element")
         _lib.check(self.lib.slm_grad_list_accumulate(self.handle, acc.data_ptr(), self.elements,
@@ -245,14 +263,17 @@ def _stream_handle(stream) -> int | None:
     return int(stream.cuda_stream)  # torch.cuda.Stream
 
 
-def _use_on(values, work, stream: int | None) -> None:
-    """Tells torch's allocator when memory it gave for the current stream is used
+def _current_stream(index: int) -> int:
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _use_on(tensor, stream: int | None) -> None:
+    """Tells torch's allocator that memory it gave for the current stream is used
     on another one."""
     import torch
 
     handle = stream or 0
-    if torch.cuda.current_stream(values.device).cuda_stream != handle:
-        other = torch.cuda.ExternalStream(handle, device=values.device) if handle else \
-            torch.cuda.default_stream(values.device)
-        values.record_stream(other)
-        work.record_stream(other)
+    tensor.record_stream(torch.cuda.ExternalStream(handle, device=tensor.device) if handle else
+                         torch.cuda.default_stream(tensor.device))
