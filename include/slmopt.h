@@ -421,7 +421,7 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * row-major order, tensor after tensor.
  *
  * Norm: each tensor is cut into units of consecutive elements (a power of two
- * between 4,096 and 2^30, so that a list has about 8,192 of them at most).
+ * between 8,192 and 2^30, so that a list has about 16,384 of them at most).
  * Within a unit 8 consecutive values are squared and added in f32 (fused
  * multiply-adds), and these sums in f64 by the flat norm's tree; the units'
  * partials are added in f64 in a fixed order and divided by the loss scale

@@ -175,11 +175,9 @@ int allocate_state(slm_opt_handle* h, uint64_t w16_elems) {
           "upload tile table");
   const DeviceScaler sc{65536.0f, 0u};
   SLM_TRY(cudaMemcpy(h->d_scaler, &sc, sizeof(sc), cudaMemcpyHostToDevice), "upload scaler");
-  if (!h->sharded()) {
+  if (!h->sharded())
     SLM_TRY(cudaMalloc(&h->d_list_partials, list_partial_bytes(h->offsets)),
             "cudaMalloc list partials");
-    h->grid_list_update = list_update_grid(h->device);
-  }
 #undef SLM_TRY
   h->grid_norm = norm_partials_grid(h->device);
   h->grid_norm_bulk = norm_bulk_grid(h->device);

@@ -26,7 +26,7 @@ struct slm_grad_list {
   std::vector<Extent> extents;  // non-empty tensors by address
   bool overlapping = false;     // two tensors share an element
   uint32_t pitched = 0;         // whether any tensor is rows with a pitch
-  uint32_t types = 0;           // bit per type of a tensor with elements
+  uint32_t off_vectors = 0, types = 0;  // see GradListView; bit per type of a tensor with elements
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
@@ -36,7 +36,7 @@ struct slm_grad_list {
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        types, cluster, keep, elements};
+                        off_vectors, types, cluster, keep, elements};
   }
 };
 
@@ -140,6 +140,7 @@ int fill_list(slm_grad_list* l, const slm_grad_view* views, uint32_t n) {
     if (t.elements) l->types |= 1u << uint32_t(v.dtype);
     t.flags = layout_flags(uint32_t(v.dtype), pitched, v.data, t.columns, t.row_stride);
     t.offset = l->elements;
+    if (t.elements && t.offset % kVec) l->off_vectors = 1;
     l->elements += t.elements;
     if (l->elements > kMost) return fail(SLM_ERR_SIZE_LIMIT, "the list is larger than any memory");
   }
@@ -274,10 +275,8 @@ int slmopt::enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list,
 
 int slmopt::enqueue_list_update(slm_opt_handle* h, const GradListView& list,
                                 const slm_step_config* cfg, cudaStream_t s) {
-  const AdamwParams p = adamw_params(cfg);
-  return h->cuda(launch_list_update(list, h->master, h->m1, h->m2, h->w16, h->d_offsets,
-                                    h->d_decay, h->d_tile_first, p, h->d_state,
-                                    h->grid_list_update, s),
+  return h->cuda(launch_list_update(list, h->master, h->m1, h->m2, h->w16, h->d_decay,
+                                    adamw_params(cfg), h->d_state, s),
                  "list update kernel");
 }
 

@@ -105,7 +105,6 @@ struct slm_opt_handle {
   int grid_norm = 0;       // resident blocks of the per-chunk tree kernels
   int grid_norm_bulk = 0;  // persistent grid of the bulk-copy norm pass
   int grid_update[2] = {0, 0};
-  int grid_list_update = 0;
   void* d_list_partials = nullptr;  // norm partials of a gradient list over the table
   // Gradients seen by the last norm pass (consumed by the update pass).
   const void* pass_grads = nullptr;

@@ -272,11 +272,14 @@ struct __align__(16) GradUnit {
   uint64_t offset;  // flat position of the unit's first element
 };
 static_assert(sizeof(GradTensor) == 48 && sizeof(GradUnit) == 32, "list tables");
-// The smallest and largest unit; between them the number of units stays near
-// kGradUnitsAimed, which bounds the partials a finalize has to add.
-constexpr uint32_t kGradUnitMin = 4096;
+// The smallest and largest unit; between them a list has at most about
+// kGradUnitsAimed, which bounds the partials that its norm has to add.  4,096 and
+// 16,384 elements were slower than 8,192: the norm of 30M values in 257 tensors 26.9
+// against 23.2 us, clip of 24M f32 62.8 / 53.4, accumulate of 135M 208.7 (16,384)
+// / 204.1.
+constexpr uint32_t kGradUnitMin = 8192;
 constexpr uint32_t kGradUnitMax = 1u << 30;
-constexpr uint64_t kGradUnitsAimed = 8192;
+constexpr uint64_t kGradUnitsAimed = 16384;
 // How much of the list's end the norm pass leaves in the L2 for the clip, which
 // walks it from there.  Clip of 270 MB of bf16: 132.3 us with none, 129.6 / 128.6 /
 // 127.3 with 16 / 24 / 48 MB, 133.2 without priorities; of 96 MB in f32 column slices:
@@ -296,6 +299,7 @@ struct GradListView {
   uint32_t n_units, n_tensors;
   uint32_t unit_elems;
   uint32_t rows;   // whether any tensor is pitched
+  uint32_t off_vectors;  // whether any tensor starts inside a vector of the flat order
   uint32_t types;  // bit per type of a tensor with elements
   uint32_t cluster;  // blocks of the cluster for small lists, see list_small_cluster
   uint32_t keep;   // units from here on stay in the L2 for a second pass
@@ -341,11 +345,8 @@ cudaError_t launch_list_decide(const GradListView& list, const GradPartial* part
 // AdamW over the flat state with the gradients read from the list's tensors,
 // which are the state's tensors in order.
 cudaError_t launch_list_update(const GradListView& list, float* master, float* moment,
-                               float* variance, uint16_t* w16, const uint64_t* offsets,
-                               const uint8_t* decay, const uint32_t* tile_first,
-                               const AdamwParams& p, DeviceStepState* st, int grid,
-                               cudaStream_t stream);
-int list_update_grid(int device);
+                               float* variance, uint16_t* w16, const uint8_t* decay,
+                               const AdamwParams& p, DeviceStepState* st, cudaStream_t stream);
 // Points the list's tables at new first elements (tensors [begin, begin + n)).
 constexpr uint32_t kGradBindBatch = 256;
 struct GradBind {

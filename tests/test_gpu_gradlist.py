@@ -48,8 +48,10 @@ SIZES = {
     "a vector": [8],
     "vector and one": [9],
     "nothing, little, nothing": [0, 5, 0],
-    "a unit": [4096],
-    "a unit and one": [4097],
+    "half a unit": [4096],
+    "half a unit and one": [4097],
+    "a unit": [8192],
+    "a unit and one": [8193],
     "units": [2048 * 256, 8191, 12288, 3],
     "odd": [70001, 33, 1, 1, 65537, 777],
     "many tiny": [1 + (7 * i) % 40 for i in range(500)],
@@ -194,7 +196,7 @@ def fold(lanes):
                          ids=["odd", "units", "many tiny"])
 def test_norm_is_the_documented_tree_whatever_the_layout(torch, sizes, place):
     tensors = make(torch, sizes, ["bf16", "f32"], place)
-    want = tree_sum([t.float().reshape(-1).cpu().numpy() for t in tensors], 4096)
+    want = tree_sum([t.float().reshape(-1).cpu().numpy() for t in tensors], 8192)
     with GradientList(tensors) as lst:
         first = lst.norm()
         assert float(first.sum_squares) == want
@@ -735,7 +737,7 @@ def test_rows(torch, rows, columns, stride, first, name):
     limit = norms64(torch, tensors, 2.0, "l2")[0] / 2
     with GradientList(tensors) as lst:
         check_norm(torch, lst.norm(per_tensor=True, loss_scale=3.0), tensors, 3.0, 1.0)
-        want = tree_sum([t.float().reshape(-1).cpu().numpy() for t in before], 4096)
+        want = tree_sum([t.float().reshape(-1).cpu().numpy() for t in before], 8192)
         assert float(lst.norm().sum_squares) == want
         flat = torch.cat([t.reshape(-1).float() for t in tensors])
         for start in (0, 1):  # an accumulator on and off the 32-byte boundaries
