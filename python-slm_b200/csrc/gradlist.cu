@@ -1408,8 +1408,8 @@ bool all_small_fit(uint32_t c) {
 }
 
 // A list small enough for one cluster, on a device that can hold one.
-bool is_small(const GradListView& list) {
-  return list.cluster != 0u && list.n_units <= kGradSmallUnits;
+bool is_small(const GradListView& list, uint32_t units) {
+  return list.cluster != 0u && list.n_units <= units;
 }
 }  // namespace
 
@@ -1417,7 +1417,7 @@ uint32_t list_small_cluster() { return all_small_fit(16u) ? 16u : all_small_fit(
 
 cudaError_t launch_list_norm(const GradListView& list, float scale, float max_norm, int kind,
                              const GradListOut& out, GradPartial* partials, cudaStream_t stream) {
-  if (is_small(list))
+  if (is_small(list, kGradSmallNorm))
     return launch_small<kSmallNorm>(list, list, scale, max_norm, kind, out, partials, nullptr,
                                     nullptr, FinalizeParams{}, stream);
   if (list.n_units > 0) {
@@ -1434,7 +1434,7 @@ cudaError_t launch_list_norm(const GradListView& list, float scale, float max_no
 cudaError_t launch_list_norm_decide(const GradListView& list, GradPartial* partials,
                                     DeviceScaler* scaler, DeviceStepState* st,
                                     const FinalizeParams& fp, cudaStream_t stream) {
-  if (is_small(list))
+  if (is_small(list, kGradSmallStep))
     return launch_small<kSmallStep>(list, list, fp.static_scale, 1.0f, 0, GradListOut{}, partials,
                                     scaler, st, fp, stream);
   const cudaError_t e = launch_chained(
@@ -1470,7 +1470,7 @@ cudaError_t launch_list_clip(const GradListView& list, const GradListView& to, b
                              float scale, float max_norm, int kind, const GradListOut& out,
                              GradPartial* partials, cudaStream_t stream) {
   const bool one_type = in_place || (to.types & (to.types - 1u)) == 0u;
-  if (is_small(list) && one_type) {
+  if (is_small(list, kGradSmallClip) && one_type) {
     const auto launch = in_place ? launch_small<kOutSame>
                         : to.types == 1u << kGradF32  ? launch_small<kGradF32>
                         : to.types == 1u << kGradBf16 ? launch_small<kGradBf16>

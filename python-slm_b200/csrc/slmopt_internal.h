@@ -286,8 +286,12 @@ constexpr uint64_t kGradUnitsAimed = 16384;
 // 62.4, 60.9 / 62.1 / 65.4, 69.6.  More than that is not kept: the last pass's writes
 // are still in the L2.
 constexpr uint64_t kGradKeepBytes = uint64_t(24) << 20;
-// Lists of at most so many units are taken by one cluster in one launch.
-constexpr uint32_t kGradSmallUnits = 256;
+// Lists of at most so many units (of 8,192 elements) are taken by one cluster in
+// one launch.  One cluster against kernels over the whole GPU, bf16, us a call in a
+// row of calls: norm of 0.25 / 1 / 2 / 4M elements 7.7 / 8.5 / 10.1 / 15.7 against
+// 10.2 / 10.4 / 10.2 / 11.9; clip of 0.25 / 0.5 / 1M 7.8 / 10.5 / 14.8 against 12.4 /
+// 12.6 / 12.4; step on 0.03 / 0.25 / 0.5M 7.2 / 8.0 / 10.3 against 8.2 / 8.4 / 8.7.
+constexpr uint32_t kGradSmallNorm = 192, kGradSmallClip = 80, kGradSmallStep = 40;
 inline uint32_t grad_unit_elems(uint64_t total) {
   uint32_t u = kGradUnitMin;
   while (u < kGradUnitMax && total / u > kGradUnitsAimed) u *= 2;
