@@ -20,6 +20,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace slmopt {
 namespace {
@@ -124,6 +125,43 @@ struct Raw {
     for (uint32_t i = 0; i < kWords; ++i)
       w[i] = T == kGradF32 ? b[i] : __funnelshift_r(b[i], b[i + 1], bits);
   }
+  // The same from a 16-byte boundary on, with the shift's whole words known to the
+  // compiler (one for a contiguous unit) and its half word in bits: only what is
+  // needed of the last block is loaded.
+  template <uint32_t kShift>
+  __device__ __forceinline__ void load_shifted_by(const uint8_t* block, uint32_t bits) {
+    uint32_t b[kWords + 4];
+#pragma unroll
+    for (uint32_t i = 0; i < kWords / 4; ++i) {
+      const uint4 r = reinterpret_cast<const uint4*>(block)[i];
+      b[4 * i] = r.x;
+      b[4 * i + 1] = r.y;
+      b[4 * i + 2] = r.z;
+      b[4 * i + 3] = r.w;
+    }
+    constexpr uint32_t kMore = kShift + (T == kGradF32 ? 0u : 1u);  // words of the last block
+    const uint8_t* last = block + kWords * 4;
+    if constexpr (kMore == 1u) {
+      b[kWords] = *reinterpret_cast<const uint32_t*>(last);
+    } else if constexpr (kMore == 2u) {
+      const uint2 r = *reinterpret_cast<const uint2*>(last);
+      b[kWords] = r.x;
+      b[kWords + 1] = r.y;
+    } else if constexpr (kMore > 2u) {
+      const uint4 r = *reinterpret_cast<const uint4*>(last);
+      b[kWords] = r.x;
+      b[kWords + 1] = r.y;
+      b[kWords + 2] = r.z;
+      b[kWords + 3] = r.w;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) {
+      if constexpr (T == kGradF32)
+        w[i] = b[i + kShift];
+      else
+        w[i] = __funnelshift_r(b[i + kShift], b[i + kShift + 1], bits);
+    }
+  }
   __device__ __forceinline__ void set(uint32_t j, uint32_t bits) {
     if constexpr (T == kGradF32)
       w[j] = bits;
@@ -160,6 +198,17 @@ struct Raw {
   }
 };
 
+// Calls f with the whole words of the shift of a contiguous run at p, as a constant.
+template <typename F>
+__device__ __forceinline__ void by_shift(const uint8_t* p, F f) {
+  switch ((reinterpret_cast<uintptr_t>(p) & 15u) / 4u) {
+    case 0: return f(std::integral_constant<uint32_t, 0>());
+    case 1: return f(std::integral_constant<uint32_t, 1>());
+    case 2: return f(std::integral_constant<uint32_t, 2>());
+    default: return f(std::integral_constant<uint32_t, 3>());
+  }
+}
+
 // A thread's largest magnitude as f32 bits.
 template <uint32_t T>
 __device__ __forceinline__ uint32_t top_f32(uint32_t m) {
@@ -181,21 +230,19 @@ struct Rows {
   uint32_t col_step;  // of 2,048 elements
   uint64_t step;      // bytes, before a wrap
   uint64_t wrap;      // bytes from a row's end to the next row
-  __device__ __forceinline__ Rows(const GradUnit& u, const GradListView& list,
-                                  uint32_t e = unit_thread() * kVec) {
+  // At element e of the unit.
+  __device__ __forceinline__ Rows(const GradUnit& u, uint32_t e) {
     p = static_cast<uint8_t*>(const_cast<void*>(u.ptr));
     if (u.flags & kGradPitched) {
-      const GradTensor* t = list.tensors + u.tensor;
-      const uint64_t stride = __ldg(&t->row_stride);
-      columns = static_cast<uint32_t>(__ldg(&t->columns));
-      const uint64_t k = uint64_t(u.index) * list.unit_elems + e;
-      const uint64_t row = k <= 0xffffffffull ? uint64_t(uint32_t(k) / columns) : k / columns;
-      col = static_cast<uint32_t>(k - row * columns);
-      p += (row * stride + col) * kSize<T>;
+      columns = u.columns;
+      const uint32_t k = u.column + e;
+      const uint32_t row = k / columns;
+      col = k - row * columns;
+      p += (int64_t(row * u.row_stride) + col - u.column) * int64_t(kSize<T>);
       const uint32_t rows = kListThreads * kVec / columns;
       col_step = kListThreads * kVec - rows * columns;
-      step = (rows * stride + col_step) * kSize<T>;
-      wrap = (stride - columns) * kSize<T>;
+      step = (rows * u.row_stride + col_step) * kSize<T>;
+      wrap = (u.row_stride - columns) * kSize<T>;
     } else {
       columns = u.count;
       col = e;
@@ -256,11 +303,13 @@ __device__ __forceinline__ void gather_flat(Raw<T>& raw, const uint8_t* p, uint3
     if (j < n) raw.set(j, elem_bits<T>(p, j));
 }
 
+template <bool kRows>
 __device__ __forceinline__ GradUnit load_unit(const GradUnit* units, uint32_t i) {
   GradUnit u;
   const uint4* p = reinterpret_cast<const uint4*>(units + i);
   *reinterpret_cast<uint4*>(&u) = __ldg(p);
   *(reinterpret_cast<uint4*>(&u) + 1) = __ldg(p + 1);
+  if constexpr (kRows) *(reinterpret_cast<uint4*>(&u) + 2) = __ldg(p + 2);
   return u;
 }
 
@@ -351,14 +400,18 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
   } else {
     // Off the boundaries: the first and the last vector, whose blocks can reach
     // beyond the tensor, element by element.
-    for (; v < whole; v += kListThreads) {
-      Raw<T> raw;
-      if (v > 0u && v + 1u < whole)
-        raw.load_shifted(base + v * kVecBytes<T>);
-      else
-        gather_flat(raw, base + v * kVecBytes<T>, kVec);
-      sq.take(raw);
-    }
+    const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base)) & 15u;
+    by_shift(base, [&](auto shift) {
+      for (; v < whole; v += kListThreads) {
+        Raw<T> raw;
+        if (v > 0u && v + 1u < whole)
+          raw.template load_shifted_by<decltype(shift)::value>(base - d + v * kVecBytes<T>,
+                                                               (d & 2u) * 8u);
+        else
+          gather_flat(raw, base + v * kVecBytes<T>, kVec);
+        sq.take(raw);
+      }
+    });
   }
   if (unit_thread() == whole % kListThreads && count % kVec) {
     Raw<T> raw;
@@ -369,17 +422,31 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
 
 template <uint32_t T, bool kFactor>
 __device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, Rows<T> rows,
-                                            uint32_t count, uint64_t policy) {
-  constexpr uint32_t kBatch = 2;
-  for (uint32_t e = unit_thread() * kVec; e < count; e += kBatch * kListThreads * kVec) {
-    Raw<T> raw[kBatch];
+                                            uint32_t count, bool vectors, uint64_t policy) {
+  uint32_t e = unit_thread() * kVec;
+  if (vectors) {
+    // Every vector is one aligned run.
+    constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
+    for (; e < count; e += kBatch * kListThreads * kVec) {
+      Raw<T> raw[kBatch];
 #pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) {
-      rows.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count), policy);
-      rows.next_vector();
+      for (uint32_t b = 0; b < kBatch; ++b) {
+        if (e + b * (kListThreads * kVec) < count)
+          raw[b].load(rows.p, policy);
+        else
+          raw[b].zero();
+        rows.next_vector();
+      }
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; ++b) sq.take(raw[b]);
     }
-#pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) sq.take(raw[b]);
+    return;
+  }
+  for (; e < count; e += kListThreads * kVec) {
+    Raw<T> raw;
+    rows.load(raw, vector_elems(e, count), policy);
+    rows.next_vector();
+    sq.take(raw);
   }
 }
 
@@ -392,7 +459,8 @@ __device__ __forceinline__ double unit_squares(const GradUnit& u, const GradList
   sq.factor = factor;
   const uint64_t policy = blockIdx.x < list.keep ? l2_first_out() : l2_normal();
   if (kRows && (u.flags & kGradPitched))
-    row_squares(sq, Rows<T>(u, list), u.count, policy);
+    row_squares(sq, Rows<T>(u, unit_thread() * kVec), u.count, (u.flags & kGradVector) != 0u,
+                policy);
   else
     flat_squares(sq, static_cast<const uint8_t*>(u.ptr), u.count, policy);
   top = top_f32<T>(sq.top);
@@ -590,7 +658,7 @@ __global__ void __launch_bounds__(kListThreads, kRows ? 5 : 8)
     list_norm_kernel(GradListView list, float scale, const DeviceScaler* scaler,
                      GradPartial* partials) {
   __shared__ UnitSlot slot;
-  const GradUnit u = load_unit(list.units, blockIdx.x);
+  const GradUnit u = load_unit<kRows>(list.units, blockIdx.x);
   // The kernels behind may start to read gradients once all blocks are here, so
   // their producers must be done by then: wait first.
   pdl_wait();
@@ -638,6 +706,7 @@ __global__ void __launch_bounds__(kLanes)
 }
 
 // ---- clip ----------------------------------------------------------------------
+constexpr uint32_t kNoRows = 0u, kRowVectors = 1u, kAnyRows = 2u;
 template <uint32_t T>
 __device__ __forceinline__ uint32_t to_bits(float y) {
   if constexpr (T == kGradF32)
@@ -743,18 +812,19 @@ struct ClipState {
 // One unit of the clip, each element read and written by the same thread.
 // Contiguous on both sides: vectors start at the output's boundaries, and the
 // input is shifted where it lies off them.
-template <uint32_t T, uint32_t O>
+// kAligned: no tensor of either list lies off the boundaries.
+template <uint32_t T, uint32_t O, bool kAligned>
 __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint32_t count,
                                           float scale, ClipState& state) {
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
   constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
-  const uint32_t peel = peel_of<O>(dst, count);
+  const uint32_t peel = kAligned ? 0u : peel_of<O>(dst, count);
   const uint8_t* from = src + peel * kSize<T>;
   uint8_t* to = dst + peel * kSize<O>;
   const uint32_t whole = (count - peel) / kVec;
   uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
   uint32_t v = unit_thread();
-  if (reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
+  if (kAligned || reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
     const uint64_t policy = l2_first_out();
     Raw<T> raw[kBatch];
 #pragma unroll
@@ -776,11 +846,15 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
     if (!state.ready()) return;
     const ClipFactor f(state.clip, scale);
     // The blocks of the first and the last vector can reach beyond the tensor.
-    for (v += 1u; v + 1u < whole; v += kListThreads) {
-      Raw<T> raw;
-      raw.load_shifted(from + v * kVecBytes<T>);
-      clip_raw<T, O>(raw, f, to + v * kVecBytes<O>);
-    }
+    const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
+    by_shift(from, [&](auto shift) {
+      for (v += 1u; v + 1u < whole; v += kListThreads) {
+        Raw<T> raw;
+        raw.template load_shifted_by<decltype(shift)::value>(from - d + v * kVecBytes<T>,
+                                                             (d & 2u) * 8u);
+        clip_raw<T, O>(raw, f, to + v * kVecBytes<O>);
+      }
+    });
     if (whole) {
       head += kVec;
       tail = whole > 1u ? tail - kVec : head;
@@ -793,50 +867,79 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
   }
 }
 
-// Rows on either side.
+// Rows on either side where every vector is one aligned run on both.
 template <uint32_t T, uint32_t O>
-__device__ __forceinline__ void clip_rows(Rows<T> src, Rows<O> dst, uint32_t count, float scale,
-                                          ClipState& state) {
+__device__ __forceinline__ void clip_row_vectors(const GradUnit& u, const GradUnit& o, float scale,
+                                                 ClipState& state) {
   constexpr uint32_t kBatch = 2;
   if (!state.ready()) return;
   const ClipFactor f(state.clip, scale);
-  for (uint32_t e = unit_thread() * kVec; e < count; e += kBatch * kListThreads * kVec) {
+  uint32_t e = unit_thread() * kVec;
+  Rows<T> src(u, e);
+  Rows<O> dst(o, e);
+  for (; e < u.count; e += kBatch * kListThreads * kVec) {
     Raw<T> raw[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
-      src.load(raw[b], vector_elems(e + b * (kListThreads * kVec), count), l2_first_out());
+      if (e + b * (kListThreads * kVec) < u.count) raw[b].load(src.p, l2_first_out());
       src.next_vector();
     }
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
-      const uint32_t n = vector_elems(e + b * (kListThreads * kVec), count);
-      if (n == kVec && dst.aligned()) {
-        clip_raw<T, O>(raw[b], f, dst.p);
-      } else {
-        float x[8];
-        raw[b].unpack(x);
-        Rows<O> r = dst;
-#pragma unroll
-        for (uint32_t j = 0; j < kVec; ++j) {
-          if (j < n) {
-            store1<O>(r.p, 0, f(x[j]));
-            r.next_element();
-          }
-        }
-      }
+      if (e + b * (kListThreads * kVec) < u.count) clip_raw<T, O>(raw[b], f, dst.p);
       dst.next_vector();
     }
   }
 }
 
-template <uint32_t T, uint32_t O, bool kRows>
+// Any rows.  With rows in and contiguous memory out, vectors start at the
+// output's boundaries.
+template <uint32_t T, uint32_t O>
+__device__ __forceinline__ void clip_rows(const GradUnit& u, const GradUnit& o, float scale,
+                                          ClipState& state) {
+  if (!state.ready()) return;
+  const ClipFactor f(state.clip, scale);
+  const uint32_t head = o.flags & kGradPitched ? 0u : peel_of<O>(o.ptr, u.count);
+  uint32_t e = head + unit_thread() * kVec;
+  Rows<T> src(u, e);
+  Rows<O> dst(o, e);
+  for (; e < u.count; e += kListThreads * kVec) {
+    const uint32_t n = vector_elems(e, u.count);
+    Raw<T> raw;
+    src.load(raw, n, l2_first_out());
+    if (n == kVec && dst.aligned()) {
+      clip_raw<T, O>(raw, f, dst.p);
+    } else {
+      float x[8];
+      raw.unpack(x);
+      Rows<O> to = dst;
+#pragma unroll
+      for (uint32_t j = 0; j < kVec; ++j) {
+        if (j < n) {
+          store1<O>(to.p, 0, f(x[j]));
+          to.next_element();
+        }
+      }
+    }
+    src.next_vector();
+    dst.next_vector();
+  }
+  if (unit_thread() < head)
+    store1<O>(Rows<O>(o, unit_thread()).p, 0,
+              f(from_bits<T>(elem_bits<T>(Rows<T>(u, unit_thread()).p, 0))));
+}
+
+// kRows: kNoRows, kRowVectors, kAnyRows, each with the registers it needs.
+template <uint32_t T, uint32_t O, uint32_t kRows>
 __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
                                           const GradListView& list, const GradListView& out,
                                           float scale, ClipState& state) {
-  if (kRows && ((u.flags | o.flags) & kGradPitched))
-    clip_rows<T, O>(Rows<T>(u, list), Rows<O>(o, out), u.count, scale, state);
+  if (kRows == kRowVectors && ((u.flags | o.flags) & kGradPitched))
+    clip_row_vectors<T, O>(u, o, scale, state);
+  else if (kRows == kAnyRows && ((u.flags | o.flags) & kGradPitched))
+    clip_rows<T, O>(u, o, scale, state);
   else
-    clip_flat<T, O>(static_cast<const uint8_t*>(u.ptr),
+    clip_flat<T, O, kRows == kRowVectors>(static_cast<const uint8_t*>(u.ptr),
                     static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale,
                     state);
 }
@@ -844,12 +947,12 @@ __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
 // kOut: the output type (units written in another one are left to the launch for
 // theirs), or in place.  All nine pairs of types in one kernel would spill.
 constexpr uint32_t kOutSame = 3u;
-template <uint32_t kOut, bool kRows>
+template <uint32_t kOut, uint32_t kRows>
 __device__ __forceinline__ void clip_any(const GradListView& list, const GradListView& out,
                                          uint32_t i, float scale, ClipState& state) {
   constexpr bool kSame = kOut == kOutSame;
-  const GradUnit u = load_unit(list.units, i);
-  const GradUnit o = kSame ? u : load_unit(out.units, i);
+  const GradUnit u = load_unit<kRows != kNoRows>(list.units, i);
+  const GradUnit o = kSame ? u : load_unit<kRows != kNoRows>(out.units, i);
   if (!kSame && (o.flags & kGradTypeMask) != kOut) return;
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
@@ -861,8 +964,8 @@ __device__ __forceinline__ void clip_any(const GradListView& list, const GradLis
   }
 }
 
-template <uint32_t kOut, bool kRows>
-__global__ void __launch_bounds__(kListThreads, 4)
+template <uint32_t kOut, uint32_t kRows>
+__global__ void __launch_bounds__(kListThreads, kRows == kAnyRows ? 3 : 4)
     list_clip_kernel(GradListView list, GradListView out, float scale, const float* result) {
   ClipState state{result, 0.0f, 0.0f, false};
   // In place with a loss scale of one there may be nothing to do: look before
@@ -870,8 +973,12 @@ __global__ void __launch_bounds__(kListThreads, 4)
   if (kOut == kOutSame && scale == 1.0f && (!state.ready() || state.clip == 1.0f)) return;
   // From the end of the list to its start: the norm pass has read the end last,
   // so the part of the gradients that the L2 still holds is read first.
-  for (uint32_t b = blockIdx.x; b < list.n_units; b += gridDim.x)
-    clip_any<kOut, kRows>(list, out, list.n_units - 1u - b, scale, state);
+  if constexpr (kOut == kOutSame) {
+    for (uint32_t b = blockIdx.x; b < list.n_units; b += gridDim.x)
+      clip_any<kOut, kRows>(list, out, list.n_units - 1u - b, scale, state);
+  } else {
+    clip_any<kOut, kRows>(list, out, list.n_units - 1u - blockIdx.x, scale, state);
+  }
 }
 
 // ---- small lists -------------------------------------------------------------------
@@ -923,7 +1030,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   if (kMode == kSmallStep && fp.dynamic) scale = scaler->scale;
   const float factor = square_factor(scale);
   for (uint32_t i = begin; i < list.n_units; i += step) {
-    unit_partial<true>(list, load_unit(list.units, i), factor, slots[group], 1u + group,
+    unit_partial<true>(list, load_unit<true>(list.units, i), factor, slots[group], 1u + group,
                        partials + i);
     unit_barrier(1u + group);  // the slot is free again
   }
@@ -959,7 +1066,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     ClipState state{nullptr, s_clip.x, s_clip.y, true};
     if (!state.ready() || (kMode == kOutSame && scale == 1.0f && state.clip == 1.0f)) return;
     for (uint32_t i = begin; i < list.n_units; i += step)
-      clip_any<kMode, true>(list, to, i, scale, state);
+      clip_any<kMode, kAnyRows>(list, to, i, scale, state);
   }
 }
 
@@ -1020,13 +1127,17 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
     }
   } else {
     // The blocks of the first and the last vector can reach beyond the tensor.
-    for (uint32_t v = unit_thread() + 1u; v + 1u < whole; v += kListThreads) {
-      Raw<T> raw;
-      float old[8];
-      raw.load_shifted(from + v * kVecBytes<T>);
-      if (!overwrite) load_acc(to + v * kVec, old);
-      add_raw<T>(raw, old, overwrite, to + v * kVec);
-    }
+    const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
+    by_shift(from, [&](auto shift) {
+      for (uint32_t v = unit_thread() + 1u; v + 1u < whole; v += kListThreads) {
+        Raw<T> raw;
+        float old[8];
+        raw.template load_shifted_by<decltype(shift)::value>(from - d + v * kVecBytes<T>,
+                                                             (d & 2u) * 8u);
+        if (!overwrite) load_acc(to + v * kVec, old);
+        add_raw<T>(raw, old, overwrite, to + v * kVec);
+      }
+    });
     if (whole) {
       head += kVec;
       tail = whole > 1u ? tail - kVec : head;
@@ -1039,27 +1150,30 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
 }
 
 template <uint32_t T>
-__device__ __forceinline__ void accumulate_rows(Rows<T> src, float* dst, uint32_t count,
-                                                bool overwrite) {
-  const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
-  for (uint32_t e = unit_thread() * kVec; e < count; e += kListThreads * kVec) {
+__device__ __forceinline__ void accumulate_rows(const GradUnit& u, float* dst, bool overwrite) {
+  const uint32_t count = u.count;
+  const uint32_t head = peel_of<kGradF32>(dst, count);
+  uint32_t e = head + unit_thread() * kVec;
+  Rows<T> src(u, e);
+  for (; e < count; e += kListThreads * kVec) {
     const uint32_t n = vector_elems(e, count);
     Raw<T> raw;
     float old[8];
-    if (wide && n == kVec) {
-      if (!overwrite) load_acc(dst + e, old);
-      src.load(raw, n, l2_first_out());
+    if (!overwrite && n == kVec) load_acc(dst + e, old);
+    src.load(raw, n, l2_first_out());
+    src.next_vector();
+    if (n == kVec) {
       add_raw<T>(raw, old, overwrite, dst + e);
     } else {
-      src.load(raw, n, l2_first_out());
       float x[8];
       raw.unpack(x);
 #pragma unroll
       for (uint32_t j = 0; j < kVec; ++j)
         if (j < n) dst[e + j] = overwrite ? x[j] : __fadd_rn(dst[e + j], x[j]);
     }
-    src.next_vector();
   }
+  if (unit_thread() < head)
+    add_one<T>(Rows<T>(u, unit_thread()).p, 0, overwrite, dst + unit_thread());
 }
 
 template <uint32_t T, bool kRows>
@@ -1067,7 +1181,7 @@ __device__ __forceinline__ void accumulate_unit(const GradUnit& u, const GradLis
                                                 float* acc, bool overwrite) {
   float* dst = acc + u.offset;
   if (kRows && (u.flags & kGradPitched))
-    accumulate_rows<T>(Rows<T>(u, list), dst, u.count, overwrite);
+    accumulate_rows<T>(u, dst, overwrite);
   else
     accumulate_flat<T>(static_cast<const uint8_t*>(u.ptr), dst, u.count, overwrite);
 }
@@ -1075,7 +1189,7 @@ __device__ __forceinline__ void accumulate_unit(const GradUnit& u, const GradLis
 template <bool kRows>
 __global__ void __launch_bounds__(kListThreads, 4)
     list_accumulate_kernel(GradListView list, float* acc, int overwrite) {
-  const GradUnit u = load_unit(list.units, blockIdx.x);
+  const GradUnit u = load_unit<kRows>(list.units, blockIdx.x);
   pdl_wait();
   pdl_trigger();  // whoever starts early waits for this kernel before it reads
   switch (u.flags & kGradTypeMask) {
@@ -1093,7 +1207,7 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
                                                      float* acc, bool overwrite, float factor,
                                                      uint32_t& top) {
   constexpr uint32_t kBatch = 2;
-  Rows<T> src(u, list);
+  Rows<T> src(u, unit_thread() * kVec);
   float* dst = acc + u.offset;
   const bool wide = reinterpret_cast<uintptr_t>(dst) % 32u == 0u;
   double sum = 0.0;
@@ -1165,7 +1279,7 @@ __global__ void __launch_bounds__(kListThreads)
     list_accumulate_norm_kernel(GradListView list, float* acc, int overwrite, float scale,
                                 const DeviceScaler* scaler, GradPartial* partials) {
   __shared__ UnitSlot slot;
-  const GradUnit u = load_unit(list.units, blockIdx.x);
+  const GradUnit u = load_unit<true>(list.units, blockIdx.x);
   pdl_wait();
   const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
@@ -1199,7 +1313,7 @@ __device__ __forceinline__ void update_grads(const GradUnit& u, const GradListVi
                                              uint32_t e, float (&x)[8]) {
   Raw<T> raw;
   if (kRows && (u.flags & kGradPitched)) {
-    Rows<T>(u, list, e).load(raw, kVec, l2_first_out());
+    Rows<T>(u, e).load(raw, kVec, l2_first_out());
   } else {
     const uint8_t* p = static_cast<const uint8_t*>(u.ptr) + e * kSize<T>;
     if (reinterpret_cast<uintptr_t>(p) % kVecBytes<T> == 0u)
@@ -1215,7 +1329,7 @@ template <uint32_t T, bool kRows>
 __device__ __forceinline__ float update_grad(const GradUnit& u, const GradListView& list,
                                              uint32_t e) {
   if (kRows && (u.flags & kGradPitched))
-    return from_bits<T>(elem_bits<T>(Rows<T>(u, list, e).p, 0));
+    return from_bits<T>(elem_bits<T>(Rows<T>(u, e).p, 0));
   return from_bits<T>(elem_bits<T>(u.ptr, e));
 }
 
@@ -1240,7 +1354,7 @@ __global__ void __launch_bounds__(kUpdateBlock, 8)
   // From the end of a list whose end is what the L2 holds after the norm.
   const uint32_t b = backwards ? gridDim.x - 1u - blockIdx.x : blockIdx.x;
   const uint32_t unit = b / blocks_per_unit;
-  const GradUnit u = load_unit(list.units, unit);
+  const GradUnit u = load_unit<kRows>(list.units, unit);
   // The vector's first element within the unit; below zero in front of a unit
   // that starts inside a vector of the state.
   const int32_t e = int32_t((b - unit * blocks_per_unit) * kUpdateElems + threadIdx.x * kVec) -
@@ -1315,11 +1429,9 @@ __global__ void list_bind_units_kernel(const GradTensor* tensors, GradUnit* unit
   const uint32_t k = units[i].tensor;
   if (k < begin || k - begin >= n) return;
   const GradTensor& t = tensors[k];
-  const uint64_t skip = (t.flags & kGradPitched)
-                            ? 0u
-                            : uint64_t(units[i].index) * unit_elems *
-                                  elem_bytes(t.flags & kGradTypeMask);
-  units[i].ptr = static_cast<const uint8_t*>(t.ptr) + skip;
+  uint64_t at = uint64_t(units[i].index) * unit_elems;
+  if (t.flags & kGradPitched) at = at / t.columns * t.row_stride + at % t.columns;
+  units[i].ptr = static_cast<const uint8_t*>(t.ptr) + at * elem_bytes(t.flags & kGradTypeMask);
   units[i].flags = t.flags;
 }
 
@@ -1456,8 +1568,9 @@ namespace {
 template <uint32_t kOut>
 cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, float scale,
                            const float* result, cudaStream_t stream) {
-  const auto kernel =
-      list.rows || out.rows ? list_clip_kernel<kOut, true> : list_clip_kernel<kOut, false>;
+  const auto kernel = !list.rows && !out.rows ? list_clip_kernel<kOut, kNoRows>
+                      : list.off_runs || out.off_runs ? list_clip_kernel<kOut, kAnyRows>
+                                                      : list_clip_kernel<kOut, kRowVectors>;
   // Where there may be nothing to do, one wave of blocks that walk the units, so
   // that leaving is quick; else a block per unit, which the hardware balances.
   uint32_t grid = list.n_units;

@@ -26,7 +26,7 @@ struct slm_grad_list {
   std::vector<Extent> extents;  // non-empty tensors by address
   bool overlapping = false;     // two tensors share an element
   uint32_t pitched = 0;         // whether any tensor is rows with a pitch
-  uint32_t off_vectors = 0, types = 0;  // see GradListView; bit per type of a tensor with elements
+  uint32_t off_runs = 0, off_vectors = 0, types = 0;  // see GradListView; bit per type of a tensor with elements
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
@@ -36,7 +36,7 @@ struct slm_grad_list {
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        off_vectors, types, cluster, keep, elements};
+                        off_runs, off_vectors, types, cluster, keep, elements};
   }
 };
 
@@ -72,8 +72,12 @@ bool share_elements(const GradTensor& a, const GradTensor& b) {
   return col < x.columns * sx || col + y.columns * sy > pitch;
 }
 
-void find_overlaps(slm_grad_list* l) {
+// What depends on the tensors' addresses.
+void look_at_addresses(slm_grad_list* l) {
   l->extents.clear();
+  l->off_runs = 0;
+  for (const GradTensor& t : l->tensors)
+    if (t.elements && !(t.flags & kGradVector)) l->off_runs = 1;
   for (uint32_t k = 0; k < l->tensors.size(); ++k) {
     const GradTensor& t = l->tensors[k];
     if (t.elements)
@@ -163,7 +167,14 @@ int upload_list(slm_grad_list* l) {
     const uint64_t size = type_bytes(t.flags & kGradTypeMask);
     for (uint64_t e = 0, i = 0; e < t.elements; e += l->unit_elems, ++i) {
       GradUnit& u = table[t.first_unit + i];
-      u.ptr = static_cast<const uint8_t*>(t.ptr) + ((t.flags & kGradPitched) ? 0 : e * size);
+      uint64_t at = e;
+      if (t.flags & kGradPitched) {
+        u.row_stride = t.row_stride;
+        u.columns = uint32_t(t.columns);
+        u.column = uint32_t(e % t.columns);
+        at = e / t.columns * t.row_stride + u.column;
+      }
+      u.ptr = static_cast<const uint8_t*>(t.ptr) + at * size;
       u.count = uint32_t(std::min<uint64_t>(l->unit_elems, t.elements - e));
       u.tensor = k;
       u.index = uint32_t(i);
@@ -304,7 +315,7 @@ int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
         st = check_pointer(l->tensors[k].ptr, l->tensors[k].flags & kGradTypeMask, device);
     if (!st) {
       l->device = device;
-      find_overlaps(l);
+      look_at_addresses(l);
       DeviceGuard guard(device);
       st = guard.ok ? upload_list(l) : fail(SLM_ERR_CUDA, "cudaSetDevice failed");
     }
@@ -353,7 +364,7 @@ int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n,
       t.flags = layout_flags(t.flags & kGradTypeMask, (t.flags & kGradPitched) != 0u, t.ptr,
                              t.columns, t.row_stride);
     }
-    find_overlaps(list);
+    look_at_addresses(list);
   } catch (const std::exception&) {
     return fail(SLM_ERR_OUT_OF_MEMORY, "host allocation failed");
   }

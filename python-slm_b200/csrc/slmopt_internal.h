@@ -264,14 +264,18 @@ struct __align__(16) GradTensor {
   uint32_t flags;
 };
 struct __align__(16) GradUnit {
-  const void* ptr;  // first element of the unit; of the tensor when kGradPitched
+  const void* ptr;  // the unit's first element
+  uint64_t offset;  // its flat position
   uint32_t count;   // elements, 1..unit_elems
   uint32_t tensor;
-  uint32_t index;   // unit number within its tensor
   uint32_t flags;
-  uint64_t offset;  // flat position of the unit's first element
+  uint32_t index;   // unit number within its tensor
+  // Of a pitched tensor:
+  uint64_t row_stride;
+  uint32_t columns;
+  uint32_t column;  // of the first element
 };
-static_assert(sizeof(GradTensor) == 48 && sizeof(GradUnit) == 32, "list tables");
+static_assert(sizeof(GradTensor) == 48 && sizeof(GradUnit) == 48, "list tables");
 // The smallest and largest unit; between them a list has at most about
 // kGradUnitsAimed, which bounds the partials that its norm has to add.  4,096 and
 // 16,384 elements were slower than 8,192: the norm of 30M values in 257 tensors 26.9
@@ -303,6 +307,7 @@ struct GradListView {
   uint32_t n_units, n_tensors;
   uint32_t unit_elems;
   uint32_t rows;   // whether any tensor is pitched
+  uint32_t off_runs;     // whether any tensor is not kGradVector
   uint32_t off_vectors;  // whether any tensor starts inside a vector of the flat order
   uint32_t types;  // bit per type of a tensor with elements
   uint32_t cluster;  // blocks of the cluster for small lists, see list_small_cluster
