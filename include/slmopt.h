@@ -413,6 +413,9 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * is aligned to their element -- and takes them as they lie: norm, clipping,
  * accumulation into the flat f32 buffer, and the optimizer step.
  *
+ * Memory between the rows of a tensor with a pitch may be read (and is not used),
+ * never written.
+ *
  * A list borrows its tensors: they must stay allocated while the list or work
  * enqueued with it uses them.  It is immutable but for slm_grad_list_bind, so
  * calls with it may run at the same time on several streams or in several

@@ -162,6 +162,19 @@ struct Raw {
         w[i] = __funnelshift_r(b[i + kShift], b[i + kShift + 1], bits);
     }
   }
+  // Elements from `split` on (1..7) from another vector.
+  __device__ __forceinline__ void merge(const Raw& b, uint32_t split) {
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) {
+      if constexpr (T == kGradF32) {
+        if (i >= split) w[i] = b.w[i];
+      } else {
+        const uint32_t low = 2u * i < split ? 0xffffu : 0u;
+        const uint32_t keep = 2u * i + 1u < split ? low | 0xffff0000u : low;
+        w[i] = (w[i] & keep) | (b.w[i] & ~keep);
+      }
+    }
+  }
   __device__ __forceinline__ void set(uint32_t j, uint32_t bits) {
     if constexpr (T == kGradF32)
       w[j] = bits;
@@ -271,12 +284,20 @@ struct Rows {
   __device__ __forceinline__ bool aligned() const {
     return col + kVec <= columns && reinterpret_cast<uintptr_t>(p) % kVecBytes<T> == 0u;
   }
-  // The next n <= 8 elements, the rest zero.
-  __device__ __forceinline__ void load(Raw<T>& raw, uint32_t n, uint64_t policy) const {
+  // The next n <= 8 elements, the rest zero.  inside: see inside_unit; off the
+  // boundaries a vector is shifted from its blocks, and one that goes on in the
+  // next row put together from two.
+  __device__ __forceinline__ void load(Raw<T>& raw, uint32_t n, bool inside,
+                                       uint64_t policy) const {
     if (n == kVec && aligned()) {
       raw.load(p, policy);
-    } else if (n == kVec && col >= kVec && col + 2u * kVec <= columns) {
-      raw.load_shifted(p);  // its blocks lie within the row
+    } else if (n == kVec && inside && columns >= kVec) {
+      raw.load_shifted(p);
+      if (col + kVec > columns) {
+        Raw<T> next;
+        next.load_shifted(p + wrap);
+        raw.merge(next, columns - col);
+      }
     } else {
       raw.zero();
       Rows r = *this;
@@ -290,6 +311,11 @@ struct Rows {
     }
   }
 };
+// Whether the 16-byte blocks around the 8 elements from e on lie between the
+// tensor's first and last element (in memory, gaps between its rows included).
+__device__ __forceinline__ bool inside_unit(const GradUnit& u, uint32_t e) {
+  return (u.index > 0u || e >= kVec) && e + 2u * kVec <= u.count;
+}
 __device__ __forceinline__ uint32_t vector_elems(uint32_t e, uint32_t count) {
   return e >= count ? 0u : count - e < kVec ? count - e : kVec;
 }
@@ -421,10 +447,12 @@ __device__ __forceinline__ void flat_squares(Squares<T, kFactor>& sq, const uint
 }
 
 template <uint32_t T, bool kFactor>
-__device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, Rows<T> rows,
-                                            uint32_t count, bool vectors, uint64_t policy) {
+__device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, const GradUnit& u,
+                                            uint64_t policy) {
+  const uint32_t count = u.count;
   uint32_t e = unit_thread() * kVec;
-  if (vectors) {
+  Rows<T> rows(u, e);
+  if (u.flags & kGradVector) {
     // Every vector is one aligned run.
     constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
     for (; e < count; e += kBatch * kListThreads * kVec) {
@@ -444,7 +472,7 @@ __device__ __forceinline__ void row_squares(Squares<T, kFactor>& sq, Rows<T> row
   }
   for (; e < count; e += kListThreads * kVec) {
     Raw<T> raw;
-    rows.load(raw, vector_elems(e, count), policy);
+    rows.load(raw, vector_elems(e, count), inside_unit(u, e), policy);
     rows.next_vector();
     sq.take(raw);
   }
@@ -459,8 +487,7 @@ __device__ __forceinline__ double unit_squares(const GradUnit& u, const GradList
   sq.factor = factor;
   const uint64_t policy = blockIdx.x < list.keep ? l2_first_out() : l2_normal();
   if (kRows && (u.flags & kGradPitched))
-    row_squares(sq, Rows<T>(u, unit_thread() * kVec), u.count, (u.flags & kGradVector) != 0u,
-                policy);
+    row_squares(sq, u, policy);
   else
     flat_squares(sq, static_cast<const uint8_t*>(u.ptr), u.count, policy);
   top = top_f32<T>(sq.top);
@@ -906,7 +933,7 @@ __device__ __forceinline__ void clip_rows(const GradUnit& u, const GradUnit& o, 
   for (; e < u.count; e += kListThreads * kVec) {
     const uint32_t n = vector_elems(e, u.count);
     Raw<T> raw;
-    src.load(raw, n, l2_first_out());
+    src.load(raw, n, inside_unit(u, e), l2_first_out());
     if (n == kVec && dst.aligned()) {
       clip_raw<T, O>(raw, f, dst.p);
     } else {
@@ -1127,17 +1154,13 @@ __device__ __forceinline__ void accumulate_flat(const uint8_t* src, float* dst, 
     }
   } else {
     // The blocks of the first and the last vector can reach beyond the tensor.
-    const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
-    by_shift(from, [&](auto shift) {
-      for (uint32_t v = unit_thread() + 1u; v + 1u < whole; v += kListThreads) {
-        Raw<T> raw;
-        float old[8];
-        raw.template load_shifted_by<decltype(shift)::value>(from - d + v * kVecBytes<T>,
-                                                             (d & 2u) * 8u);
-        if (!overwrite) load_acc(to + v * kVec, old);
-        add_raw<T>(raw, old, overwrite, to + v * kVec);
-      }
-    });
+    for (uint32_t v = unit_thread() + 1u; v + 1u < whole; v += kListThreads) {
+      Raw<T> raw;
+      float old[8];
+      raw.load_shifted(from + v * kVecBytes<T>);
+      if (!overwrite) load_acc(to + v * kVec, old);
+      add_raw<T>(raw, old, overwrite, to + v * kVec);
+    }
     if (whole) {
       head += kVec;
       tail = whole > 1u ? tail - kVec : head;
@@ -1160,7 +1183,7 @@ __device__ __forceinline__ void accumulate_rows(const GradUnit& u, float* dst, b
     Raw<T> raw;
     float old[8];
     if (!overwrite && n == kVec) load_acc(dst + e, old);
-    src.load(raw, n, l2_first_out());
+    src.load(raw, n, inside_unit(u, e), l2_first_out());
     src.next_vector();
     if (n == kVec) {
       add_raw<T>(raw, old, overwrite, dst + e);
@@ -1219,7 +1242,7 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
     for (uint32_t b = 0; b < kBatch; ++b) {
       const uint32_t e = (v0 + b * kListThreads) * kVec;
       const uint32_t n = vector_elems(e, u.count);
-      src.load(raw[b], n, l2_first_out());
+      src.load(raw[b], n, inside_unit(u, e), l2_first_out());
       src.next_vector();
 #pragma unroll
       for (uint32_t j = 0; j < kVec; ++j) old[b][j] = 0.0f;
@@ -1313,7 +1336,7 @@ __device__ __forceinline__ void update_grads(const GradUnit& u, const GradListVi
                                              uint32_t e, float (&x)[8]) {
   Raw<T> raw;
   if (kRows && (u.flags & kGradPitched)) {
-    Rows<T>(u, e).load(raw, kVec, l2_first_out());
+    Rows<T>(u, e).load(raw, kVec, inside_unit(u, e), l2_first_out());
   } else {
     const uint8_t* p = static_cast<const uint8_t*>(u.ptr) + e * kSize<T>;
     if (reinterpret_cast<uintptr_t>(p) % kVecBytes<T> == 0u)
