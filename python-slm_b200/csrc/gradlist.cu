@@ -839,8 +839,9 @@ struct ClipState {
 // One unit of the clip, each element read and written by the same thread.
 // Contiguous on both sides: vectors start at the output's boundaries, and the
 // input is shifted where it lies off them.
-// kAligned: no tensor of either list lies off the boundaries.
-template <uint32_t T, uint32_t O, bool kAligned>
+// kAligned: no tensor of either list lies off the boundaries.  kShift: whether the
+// input can lie off them where the output is on them (not in place).
+template <uint32_t T, uint32_t O, bool kAligned, bool kShift>
 __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint32_t count,
                                           float scale, ClipState& state) {
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
@@ -851,7 +852,7 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
   const uint32_t whole = (count - peel) / kVec;
   uint32_t head = peel, tail = peel + whole * kVec;  // left over: [0, head), [tail, count)
   uint32_t v = unit_thread();
-  if (kAligned || reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
+  if (!kShift || reinterpret_cast<uintptr_t>(from) % kVecBytes<T> == 0u) {
     const uint64_t policy = l2_first_out();
     Raw<T> raw[kBatch];
 #pragma unroll
@@ -875,11 +876,18 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
     // The blocks of the first and the last vector can reach beyond the tensor.
     const uint32_t d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
     by_shift(from, [&](auto shift) {
-      for (v += 1u; v + 1u < whole; v += kListThreads) {
-        Raw<T> raw;
-        raw.template load_shifted_by<decltype(shift)::value>(from - d + v * kVecBytes<T>,
-                                                             (d & 2u) * 8u);
-        clip_raw<T, O>(raw, f, to + v * kVecBytes<O>);
+      constexpr uint32_t kShifted = T == kGradF32 ? 1 : 4;
+      for (v += 1u; v + 1u < whole; v += kShifted * kListThreads) {
+        Raw<T> raw[kShifted];
+#pragma unroll
+        for (uint32_t b = 0; b < kShifted; ++b)
+          if (v + b * kListThreads + 1u < whole)
+            raw[b].template load_shifted_by<decltype(shift)::value>(
+                from - d + (v + b * kListThreads) * kVecBytes<T>, (d & 2u) * 8u);
+#pragma unroll
+        for (uint32_t b = 0; b < kShifted; ++b)
+          if (v + b * kListThreads + 1u < whole)
+            clip_raw<T, O>(raw[b], f, to + (v + b * kListThreads) * kVecBytes<O>);
       }
     });
     if (whole) {
@@ -895,27 +903,28 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
 }
 
 // Rows on either side where every vector is one aligned run on both.
-template <uint32_t T, uint32_t O>
+template <uint32_t T, uint32_t O, bool kSame>
 __device__ __forceinline__ void clip_row_vectors(const GradUnit& u, const GradUnit& o, float scale,
                                                  ClipState& state) {
-  constexpr uint32_t kBatch = 2;
+  constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
   if (!state.ready()) return;
   const ClipFactor f(state.clip, scale);
   uint32_t e = unit_thread() * kVec;
   Rows<T> src(u, e);
-  Rows<O> dst(o, e);
+  Rows<O> dst(kSame ? u : o, e);
   for (; e < u.count; e += kBatch * kListThreads * kVec) {
     Raw<T> raw[kBatch];
+    uint8_t* to[kBatch];
 #pragma unroll
     for (uint32_t b = 0; b < kBatch; ++b) {
       if (e + b * (kListThreads * kVec) < u.count) raw[b].load(src.p, l2_first_out());
+      to[b] = kSame ? src.p : dst.p;
       src.next_vector();
+      if (!kSame) dst.next_vector();
     }
 #pragma unroll
-    for (uint32_t b = 0; b < kBatch; ++b) {
-      if (e + b * (kListThreads * kVec) < u.count) clip_raw<T, O>(raw[b], f, dst.p);
-      dst.next_vector();
-    }
+    for (uint32_t b = 0; b < kBatch; ++b)
+      if (e + b * (kListThreads * kVec) < u.count) clip_raw<T, O>(raw[b], f, to[b]);
   }
 }
 
@@ -957,16 +966,17 @@ __device__ __forceinline__ void clip_rows(const GradUnit& u, const GradUnit& o, 
 }
 
 // kRows: kNoRows, kRowVectors, kAnyRows, each with the registers it needs.
-template <uint32_t T, uint32_t O, uint32_t kRows>
+template <uint32_t T, uint32_t O, uint32_t kRows, bool kSame>
 __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
                                           const GradListView& list, const GradListView& out,
                                           float scale, ClipState& state) {
   if (kRows == kRowVectors && ((u.flags | o.flags) & kGradPitched))
-    clip_row_vectors<T, O>(u, o, scale, state);
+    clip_row_vectors<T, O, kSame>(u, o, scale, state);
   else if (kRows == kAnyRows && ((u.flags | o.flags) & kGradPitched))
     clip_rows<T, O>(u, o, scale, state);
   else
-    clip_flat<T, O, kRows == kRowVectors>(static_cast<const uint8_t*>(u.ptr),
+    clip_flat<T, O, kRows == kRowVectors, kRows != kRowVectors && !kSame>(
+        static_cast<const uint8_t*>(u.ptr),
                     static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale,
                     state);
 }
@@ -983,16 +993,17 @@ __device__ __forceinline__ void clip_any(const GradListView& list, const GradLis
   if (!kSame && (o.flags & kGradTypeMask) != kOut) return;
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
-      return clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows>(u, o, list, out, scale, state);
+      return clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows, kSame>(u, o, list, out, scale, state);
     case kGradBf16:
-      return clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows>(u, o, list, out, scale, state);
+      return clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows, kSame>(u, o, list, out, scale, state);
     default:
-      return clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows>(u, o, list, out, scale, state);
+      return clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows, kSame>(u, o, list, out, scale, state);
   }
 }
 
 template <uint32_t kOut, uint32_t kRows>
-__global__ void __launch_bounds__(kListThreads, kRows == kAnyRows ? 3 : 4)
+__global__ void __launch_bounds__(kListThreads,
+                                  kRows == kAnyRows || (kRows && kOut == kOutSame) ? 3 : 4)
     list_clip_kernel(GradListView list, GradListView out, float scale, const float* result) {
   ClipState state{result, 0.0f, 0.0f, false};
   // In place with a loss scale of one there may be nothing to do: look before
@@ -1595,7 +1606,8 @@ cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, fl
                       : list.off_runs || out.off_runs ? list_clip_kernel<kOut, kAnyRows>
                                                       : list_clip_kernel<kOut, kRowVectors>;
   // Where there may be nothing to do, one wave of blocks that walk the units, so
-  // that leaving is quick; else a block per unit, which the hardware balances.
+  // that leaving is quick (135M below the limit: 44.7 us with the norm, against 76
+  // for a block per unit); else a block per unit, which the hardware balances.
   uint32_t grid = list.n_units;
   if (kOut == kOutSame && scale == 1.0f) grid = std::min(grid, wave_blocks(kernel));
   return launch_chained(kernel, grid, kListThreads, 0, stream, list, out, scale, result);
