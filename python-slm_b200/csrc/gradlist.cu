@@ -566,7 +566,8 @@ __device__ __forceinline__ void unit_partial(const GradListView& list, const Gra
 // ---- the norm from the partials ----------------------------------------------------
 // The fixed tree over a run of partials: 1,024 lanes, lane t adds partials t,
 // t + 1024, ... in order; lanes fold by warps of 32, the 32 warps' sums by halves.
-// kThreads threads hold 1,024 / kThreads lanes each, with 8 loads in flight.
+// kThreads threads (thread index t, a barrier of their own) hold 1,024 / kThreads
+// lanes each, with at least 8 loads in flight.  Valid in thread 0.
 constexpr uint32_t kLanes = 1024;
 struct LaneSlot {
   double sum[kLanes / 32];
@@ -574,14 +575,15 @@ struct LaneSlot {
 };
 template <uint32_t kThreads>
 __device__ __forceinline__ void sum_partials(const GradPartial* partials, uint32_t count,
-                                             LaneSlot& slot, double& sum, uint32_t& top) {
+                                             uint32_t t, uint32_t barrier, LaneSlot& slot,
+                                             double& sum, uint32_t& top) {
   constexpr uint32_t kHold = kLanes / kThreads;
   constexpr uint32_t kAhead = kHold < 8 ? 8 / kHold : 1;  // steps of kLanes loaded together
   double v[kHold];
   top = 0u;
 #pragma unroll
   for (uint32_t h = 0; h < kHold; ++h) v[h] = 0.0;
-  for (uint32_t i0 = threadIdx.x; i0 < count; i0 += kAhead * kLanes) {
+  for (uint32_t i0 = t; i0 < count; i0 += kAhead * kLanes) {
     uint4 q[kAhead][kHold];
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) {
@@ -605,18 +607,18 @@ __device__ __forceinline__ void sum_partials(const GradPartial* partials, uint32
 #pragma unroll
   for (uint32_t h = 0; h < kHold; ++h) {
     v[h] = fold_warp(v[h]);
-    const uint32_t warp = (threadIdx.x + h * kThreads) / 32u;
-    if ((threadIdx.x & 31u) == 0u) {
+    const uint32_t warp = (t + h * kThreads) / 32u;
+    if ((t & 31u) == 0u) {
       slot.sum[warp] = v[h];
       slot.top[warp] = top;
     }
   }
-  __syncthreads();
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory");
   sum = 0.0;
-  if (threadIdx.x < 32u) {
+  if (t < 32u) {
     // The halving tree over 32 sums is a shuffle tree over a warp.
-    sum = fold_warp(slot.sum[threadIdx.x]);
-    top = __reduce_max_sync(kFull, slot.top[threadIdx.x]);
+    sum = fold_warp(slot.sum[t]);
+    top = __reduce_max_sync(kFull, slot.top[t]);
   }
 }
 
@@ -694,29 +696,35 @@ __global__ void __launch_bounds__(kListThreads, kRows ? 5 : 8)
                       partials + blockIdx.x);
 }
 
-// Block 0: the list's values; one more block per tensor for the tensors' own.
+// Block 0: the list's values; every further block 8 tensors' own, 128 threads each
+// (a block per tensor took its 1,024 threads' room from the norm's last blocks).
+constexpr uint32_t kTensorThreads = 128, kTensorsPerBlock = kLanes / kTensorThreads;
 __global__ void __launch_bounds__(kLanes)
     list_finalize_kernel(GradListView list, const GradPartial* partials, float scale,
                          float max_norm, int kind, GradListOut out) {
-  __shared__ LaneSlot lanes;
+  __shared__ LaneSlot lanes[kTensorsPerBlock];
   pdl_trigger();
-  uint32_t begin = 0u, count = list.n_units;
-  if (blockIdx.x > 0) {
-    const uint32_t t = blockIdx.x - 1u;
+  const uint32_t group = threadIdx.x / kTensorThreads;
+  const uint32_t t = (blockIdx.x - 1u) * kTensorsPerBlock + group;
+  uint32_t begin = 0u, end = list.n_units;
+  if (blockIdx.x > 0u) {
+    if (t >= list.n_tensors) return;  // its 128 threads together
     begin = __ldg(&list.tensors[t].first_unit);
-    const uint32_t end =
-        t + 1u < list.n_tensors ? __ldg(&list.tensors[t + 1u].first_unit) : list.n_units;
-    count = end - begin;
+    if (t + 1u < list.n_tensors) end = __ldg(&list.tensors[t + 1u].first_unit);
   }
   pdl_wait();
   double sum;
   uint32_t top;
-  sum_partials<kLanes>(partials + begin, count, lanes, sum, top);
-  if (threadIdx.x != 0) return;
-  if (blockIdx.x > 0)
-    write_tensor(out, blockIdx.x - 1u, sum, top, scale, kind);
-  else
-    write_norm(out, norm_values(sum, top, scale, max_norm, kind), unscaled_sum(sum, scale));
+  if (blockIdx.x == 0u) {
+    sum_partials<kLanes>(partials, end, threadIdx.x, 0u, lanes[0], sum, top);
+    if (threadIdx.x == 0u)
+      write_norm(out, norm_values(sum, top, scale, max_norm, kind), unscaled_sum(sum, scale));
+  } else {
+    const uint32_t i = threadIdx.x % kTensorThreads;
+    sum_partials<kTensorThreads>(partials + begin, end - begin, i, 1u + group, lanes[group], sum,
+                                 top);
+    if (i == 0u) write_tensor(out, t, sum, top, scale, kind);
+  }
 }
 
 // The step's decision from the partials.
@@ -728,7 +736,7 @@ __global__ void __launch_bounds__(kLanes)
   pdl_wait();
   double sum;
   uint32_t top;
-  sum_partials<kLanes>(partials, list.n_units, lanes, sum, top);
+  sum_partials<kLanes>(partials, list.n_units, threadIdx.x, 0u, lanes, sum, top);
   if (threadIdx.x == 0) write_step(sum, top, scaler, st, fp);
 }
 
@@ -1076,7 +1084,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   if (kClip || blockIdx.x == 0u) {
     double sum;
     uint32_t top;
-    sum_partials<kSmallThreads>(partials, list.n_units, lanes, sum, top);
+    sum_partials<kSmallThreads>(partials, list.n_units, threadIdx.x, 0u, lanes, sum, top);
     if (threadIdx.x == 0u) {
       if constexpr (kMode == kSmallStep) {
         write_step(sum, top, scaler, st, fp);
@@ -1572,7 +1580,8 @@ cudaError_t launch_list_norm(const GradListView& list, float scale, float max_no
         0, stream, list, scale, static_cast<const DeviceScaler*>(nullptr), partials);
     if (e != cudaSuccess) return e;
   }
-  const uint32_t grid = 1u + (out.tensor_norms || out.tensor_max ? list.n_tensors : 0u);
+  const uint32_t tensors = out.tensor_norms || out.tensor_max ? list.n_tensors : 0u;
+  const uint32_t grid = 1u + (tensors + kTensorsPerBlock - 1u) / kTensorsPerBlock;
   return launch_chained(list_finalize_kernel, grid, kLanes, 0, stream, list,
                         static_cast<const GradPartial*>(partials), scale, max_norm, kind, out);
 }
