@@ -424,7 +424,7 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * row-major order, tensor after tensor.
  *
  * Norm: each tensor is cut into units of consecutive elements (a power of two
- * between 8,192 and 2^30, so that a list has about 16,384 of them at most).
+ * between 8,192 and 2^26, so that a list has about 16,384 of them at most).
  * Within a unit 8 consecutive values are squared and added in f32 (fused
  * multiply-adds), and these sums in f64 by the flat norm's tree; the units'
  * partials are added in f64 in a fixed order and divided by the loss scale
@@ -499,11 +499,12 @@ int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint6
 /* slm_opt_step, slm_opt_norm_pass and slm_opt_norm_pass_accumulate with the
  * gradients in a list whose tensors are the handle's parameters in order and
  * size (E1_PARAMETER_LAYOUT_MISMATCH otherwise).  A ZeRO-1 handle refuses them.
- * After slm_opt_norm_pass_list the list must live, unbound, until the update
- * pass has run. */
+ * The update pass reads the list of the norm pass before it: its tensors must
+ * live, and not be bound anew, until that has run (a list destroyed in between is
+ * kept until then). */
 int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
                       slm_step_result* out, void* stream);
-int slm_opt_norm_pass_list(slm_opt_handle* h, const slm_grad_list* list,
+int slm_opt_norm_pass_list(slm_opt_handle* h, slm_grad_list* list,
                            const slm_step_config* cfg, void* stream);
 int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
                                       const slm_grad_list* list, int overwrite,

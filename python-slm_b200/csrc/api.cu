@@ -600,6 +600,7 @@ int slm_opt_destroy(slm_opt_handle* h) {
   // Work this handle enqueued (on any stream) finishes before its buffers and
   // peer mappings go away; every kernel's waits are bounded.
   cudaDeviceSynchronize();
+  release_pass_list(h);
   zero1_release(h);
   if (h->timer.created)
     for (cudaEvent_t e : h->timer.ev) cudaEventDestroy(e);
@@ -753,7 +754,7 @@ int slm_opt_norm_pass(slm_opt_handle* h, const void* grads, int dtype, int memor
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const void* dev = nullptr;
   h->pass_grads = nullptr;
-  h->pass_is_list = false;
+  release_pass_list(h);
   if ((st = stage_grads(h, grads, dtype, memory, s, &dev))) return st;
   if ((st = enqueue_norm(h, dev, dtype, cfg, s))) return st;
   h->pass_grads = dev;
@@ -829,7 +830,7 @@ int slm_opt_norm_pass_accumulate(slm_opt_handle* h, float* acc_device, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const void* dev = nullptr;
   h->pass_grads = nullptr;
-  h->pass_is_list = false;
+  release_pass_list(h);
   if ((st = stage_grads(h, micro, dtype, memory, s, &dev))) return st;
   const FinalizeParams fp = finalize_params(h, cfg);
   if ((st = h->cuda(launch_accumulate_norm(dtype, acc_device, dev, h->P, overwrite, h->n_chunks,
@@ -845,16 +846,16 @@ int slm_opt_norm_pass_accumulate(slm_opt_handle* h, float* acc_device, const voi
 
 int slm_opt_update_pass(slm_opt_handle* h, const slm_step_config* cfg, void* stream) {
   if (!h) return fail(SLM_ERR_INVALID_ARGUMENT, "NULL handle");
-  if (!h->pass_grads && !h->pass_is_list)
+  if (!h->pass_grads && !h->pass_list)
     return h->err(SLM_ERR_INVALID_ARGUMENT, "slm_opt_update_pass needs a preceding norm pass");
   int st = check_config(h, cfg);
   if (st) return st;
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = h->pass_is_list ? enqueue_list_update(h, h->pass_list, cfg, s)
-                       : enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, s);
+  st = h->pass_list ? enqueue_list_update(h, h->pass_list, cfg, s)
+                    : enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, s);
   h->pass_grads = nullptr;
-  h->pass_is_list = false;
+  release_pass_list(h);
   h->pending = true;
   h->pending_stream = s;
   return st;

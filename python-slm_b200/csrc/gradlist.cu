@@ -1477,18 +1477,6 @@ __global__ void list_bind_units_kernel(const GradTensor* tensors, GradUnit* unit
   units[i].flags = t.flags;
 }
 
-// Blocks of one resident wave on the current device.
-template <typename K>
-uint32_t wave_blocks(K kernel) {
-  int device = 0, sms = 0, per_sm = 0;
-  if (cudaGetDevice(&device) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kListThreads, 0) !=
-          cudaSuccess)
-    return 1u;
-  return uint32_t(std::max(1, sms) * std::max(1, per_sm));
-}
-
 // Launch chained behind the kernel ahead of it on the stream (see pdl_wait).
 template <typename... Args>
 cudaError_t launch_chained(void (*kernel)(Args...), uint32_t grid, uint32_t block, size_t smem,
@@ -1618,7 +1606,8 @@ cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, fl
   // that leaving is quick (135M below the limit: 44.7 us with the norm, against 76
   // for a block per unit); else a block per unit, which the hardware balances.
   uint32_t grid = list.n_units;
-  if (kOut == kOutSame && scale == 1.0f) grid = std::min(grid, wave_blocks(kernel));
+  if (kOut == kOutSame && scale == 1.0f)
+    grid = std::min(grid, list.sms * (list.rows ? 3u : 4u));  // as its launch bounds
   return launch_chained(kernel, grid, kListThreads, 0, stream, list, out, scale, result);
 }
 }  // namespace

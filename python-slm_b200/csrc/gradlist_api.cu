@@ -3,6 +3,7 @@
 #include "handle.h"
 
 #include <algorithm>
+#include <atomic>
 #include <exception>
 #include <new>
 
@@ -30,13 +31,15 @@ struct slm_grad_list {
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
-  uint32_t keep = 0, cluster = 0;  // see GradListView
+  uint32_t keep = 0, cluster = 0, sms = 1;  // see GradListView
   GradTensor* d_tensors = nullptr;
   GradUnit* d_units = nullptr;
+  // The owner, and one for every handle between its norm pass and update pass.
+  std::atomic<int> holders{1};
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        off_runs, off_vectors, types, cluster, keep, elements};
+                        off_runs, off_vectors, types, cluster, sms, keep, elements};
   }
 };
 
@@ -154,6 +157,10 @@ int fill_list(slm_grad_list* l, const slm_grad_view* views, uint32_t n) {
 int upload_list(slm_grad_list* l) {
   l->unit_elems = grad_unit_elems(l->elements);
   l->cluster = list_small_cluster();
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, l->device) == cudaSuccess &&
+      sms > 0)
+    l->sms = uint32_t(sms);
   uint64_t units = 0;
   for (GradTensor& t : l->tensors) {
     t.first_unit = uint32_t(units);
@@ -266,7 +273,23 @@ int check_step_list(slm_opt_handle* h, const slm_grad_list* list) {
   return SLM_OK;
 }
 
+void release(slm_grad_list* list) {
+  if (list->holders.fetch_sub(1) != 1) return;
+  DeviceGuard guard(list->device);
+  // Work enqueued with the list (on any stream) has read its tables, and its
+  // tensors, when this returns.
+  if (list->d_tensors || list->d_units) cudaDeviceSynchronize();
+  cudaFree(list->d_tensors);
+  cudaFree(list->d_units);
+  delete list;
+}
+
 }  // namespace
+
+void slmopt::release_pass_list(slm_opt_handle* h) {
+  if (h->pass_list) release(h->pass_list);
+  h->pass_list = nullptr;
+}
 
 uint64_t slmopt::list_partial_bytes(const std::vector<uint64_t>& offsets) {
   const uint32_t unit = grad_unit_elems(offsets.back());
@@ -284,9 +307,9 @@ int slmopt::enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list,
                  "list norm kernel");
 }
 
-int slmopt::enqueue_list_update(slm_opt_handle* h, const GradListView& list,
+int slmopt::enqueue_list_update(slm_opt_handle* h, const slm_grad_list* list,
                                 const slm_step_config* cfg, cudaStream_t s) {
-  return h->cuda(launch_list_update(list, h->master, h->m1, h->m2, h->w16, h->d_decay,
+  return h->cuda(launch_list_update(list->view(), h->master, h->m1, h->m2, h->w16, h->d_decay,
                                     adamw_params(cfg), h->d_state, s),
                  "list update kernel");
 }
@@ -334,12 +357,9 @@ int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
 int slm_grad_list_destroy(slm_grad_list* list) {
   if (!list) return SLM_OK;
   DeviceGuard guard(list->device);
-  // Work enqueued with the list (on any stream) has read its tables, and its
-  // tensors, when this returns.
+  // The tensors are the caller's again when this returns.
   if (list->d_tensors || list->d_units) cudaDeviceSynchronize();
-  cudaFree(list->d_tensors);
-  cudaFree(list->d_units);
-  delete list;
+  release(list);
   return SLM_OK;
 }
 
@@ -465,13 +485,13 @@ int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_st
   if ((st = phase_begin(h, s))) return st;
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
   if ((st = phase_mark(h, s))) return st;
-  if ((st = enqueue_list_update(h, list->view(), cfg, s))) return st;
+  if ((st = enqueue_list_update(h, list, cfg, s))) return st;
   if ((st = phase_mark(h, s))) return st;
   phase_end(h);
   return finish_step(h, out, s);
 }
 
-int slm_opt_norm_pass_list(slm_opt_handle* h, const slm_grad_list* list,
+int slm_opt_norm_pass_list(slm_opt_handle* h, slm_grad_list* list,
                            const slm_step_config* cfg, void* stream) {
   if (!h || !list) return fail(SLM_ERR_INVALID_ARGUMENT, "NULL argument");
   int st = check_config(h, cfg);
@@ -480,10 +500,10 @@ int slm_opt_norm_pass_list(slm_opt_handle* h, const slm_grad_list* list,
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   h->pass_grads = nullptr;
-  h->pass_is_list = false;
+  release_pass_list(h);
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
-  h->pass_list = list->view();
-  h->pass_is_list = true;
+  list->holders.fetch_add(1);
+  h->pass_list = list;
   h->pending = true;
   h->pending_stream = s;
   return SLM_OK;
@@ -505,7 +525,7 @@ int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   h->pass_grads = nullptr;
-  h->pass_is_list = false;
+  release_pass_list(h);
   const FinalizeParams fp = finalize_params(h, cfg);
   GradPartial* part = static_cast<GradPartial*>(h->d_list_partials);
   const GradListView v = list->view();

@@ -109,8 +109,7 @@ struct slm_opt_handle {
   // Gradients seen by the last norm pass (consumed by the update pass).
   const void* pass_grads = nullptr;
   int pass_dtype = -1;
-  slmopt::GradListView pass_list{};  // of slm_opt_norm_pass_list, when pass_is_list
-  bool pass_is_list = false;
+  slm_grad_list* pass_list = nullptr;  // of slm_opt_norm_pass_list, held until then
   cudaStream_t pending_stream = nullptr;
   bool pending = false;
   std::string last_error = "no error";
@@ -201,8 +200,10 @@ int finish_step(slm_opt_handle* h, slm_step_result* out, cudaStream_t s);
 uint64_t list_partial_bytes(const std::vector<uint64_t>& offsets);
 int enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
                       cudaStream_t s);
-int enqueue_list_update(slm_opt_handle* h, const GradListView& list, const slm_step_config* cfg,
+int enqueue_list_update(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
                         cudaStream_t s);
+// Lets go of the list of a norm pass whose update pass has been enqueued, or never will be.
+void release_pass_list(slm_opt_handle* h);
 void fill_result(const DeviceStepState& s, slm_step_result* out);
 // ZeRO-1 pieces (zero1.cu).
 int zero1_step(slm_opt_handle* h, const void* grads, int dtype, int memory,

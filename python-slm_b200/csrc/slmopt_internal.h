@@ -282,7 +282,7 @@ static_assert(sizeof(GradTensor) == 48 && sizeof(GradUnit) == 48, "list tables")
 // against 23.2 us, clip of 24M f32 62.8 / 53.4, accumulate of 135M 208.7 (16,384)
 // / 204.1.
 constexpr uint32_t kGradUnitMin = 8192;
-constexpr uint32_t kGradUnitMax = 1u << 30;
+constexpr uint32_t kGradUnitMax = 1u << 26;
 constexpr uint64_t kGradUnitsAimed = 16384;
 // How much of the list's end the norm pass leaves in the L2 for the clip, which
 // walks it from there.  Clip of 270 MB of bf16: 132.3 us with none, 129.6 / 128.6 /
@@ -311,6 +311,7 @@ struct GradListView {
   uint32_t off_vectors;  // whether any tensor starts inside a vector of the flat order
   uint32_t types;  // bit per type of a tensor with elements
   uint32_t cluster;  // blocks of the cluster for small lists, see list_small_cluster
+  uint32_t sms;      // of the device
   uint32_t keep;   // units from here on stay in the L2 for a second pass
   uint64_t elements;
 };

@@ -158,8 +158,8 @@ class GradientList:
             raise ValueError("gradients must be on one device")
         if t.dtype not in _dtype_codes():
             raise TypeError("gradients must be float32, bfloat16 or float16")
-        if t.is_conj() or t.is_neg():
-            raise ValueError("gradients must not be lazily negated views")
+        if t.layout != torch.strided or t.is_neg():
+            raise ValueError("gradients must be dense tensors, not lazily negated views")
         return (t.dtype, *_rows(t))
 
     def __len__(self) -> int:

@@ -319,6 +319,55 @@ def test_clip_with_other_scales_and_the_max_norm(torch, scale):
         check_clipped(torch, targets, before, scale, limit / top)
 
 
+@pytest.mark.parametrize("scale, std", [(1e-38, 1e-37), (2.0 ** -140, 2.0 ** -138), (1e38, 1e36),
+                                        (2.0 ** 127, 2.0 ** 120), (2.0 ** 20, 1e4),
+                                        (1.5 * 2.0 ** 20, 1e4), (0.99, 1e-2), (3e38, 1e37)])
+def test_extreme_loss_scales(torch, scale, std):
+    # the stored values, their quotients and the clipped values are all normal f32
+    gen = torch.Generator("cuda").manual_seed(9)
+    x = torch.rand(50_001, generator=gen, device="cuda", dtype=torch.float64) + 0.5
+    x = (x * (torch.arange(50_001, device="cuda") % 2 * 2 - 1) * std).float()
+    total = norms64(torch, [x], scale, "l2")[0]
+    top = norms64(torch, [x], scale, "max")[0]
+    # the quantised values of a subnormal scale: it is the f32 that counts
+    for kind, found in (("l2", total), ("max", top)):
+        for part in (0.5, 2.0):
+            limit = float(np.float32(found * part))
+            y = torch.empty_like(x)
+            with GradientList([x]) as lst, GradientList([y]) as to:
+                r = lst.clip(limit, loss_scale=scale, kind=kind, out=to)
+                check_norm(torch, r, [x], scale, limit, kind)
+                check_clipped(torch, [y], [x], scale, min(1.0, limit / found))
+
+
+LIMITS = [n * 8192 + d for n in (40, 80, 192) for d in (-1, 0, 1)]
+
+
+@pytest.mark.parametrize("n", LIMITS)
+def test_around_the_sizes_where_the_form_changes(torch, n):
+    sizes = [n - 3 * 8192, 8192, 8192, 8192] if n % 8192 else [n]
+    tensors = make(torch, sizes, ["bf16", "f32"], "separate", seed=14)
+    before = [t.clone() for t in tensors]
+    want = tree_sum([t.float().cpu().numpy() for t in tensors], 8192)
+    total = norms64(torch, tensors, 1.0, "l2")[0]
+    targets = [torch.empty_like(t, dtype=torch.float16) for t in tensors]
+    with GradientList(tensors) as lst, GradientList(targets) as to, \
+            B200Adamw(TensorTable.from_sizes(sizes)) as opt:
+        assert float(lst.norm().sum_squares) == want
+        check_norm(torch, lst.norm(per_tensor=True), before, 1.0, 1.0)
+        r = lst.clip(total / 2, out=to, per_tensor=True)
+        assert float(r.sum_squares) == want
+        check_norm(torch, r, before, 1.0, total / 2)
+        check_clipped(torch, targets, before, 1.0, 0.5)
+        start = load(torch, opt, 15)
+        opts = StepOptions(one_based_update=10, max_grad_norm=float(np.float32(total / 2)))
+        assert opt.step(lst, opts).sum_squares == want
+        check_state(torch, opt.state_tensors(), start, before, [True] * len(sizes), opts, 1.0, 0.5)
+        r = lst.clip(total / 2)
+        assert float(r.sum_squares) == want
+        check_clipped(torch, tensors, before, 1.0, 0.5)
+
+
 def test_values_around_a_clipped_tensor_stay(torch):
     wide = torch.randn(64, 100, device="cuda")
     bucket = torch.randn(5001, device="cuda", dtype=torch.bfloat16)
@@ -903,6 +952,77 @@ def test_rebinding_inside_a_captured_graph(torch):
             torch.cuda.synchronize()
             check_norm(torch, a, sets[0], 1.0, 1.0)
             check_norm(torch, b, sets[1], 1.0, 1.0)
+
+
+def test_a_captured_clip_in_place(torch):
+    # small and larger lists, below the limit and above it, as the gradients change
+    for sizes in ([5000, 33], [900_000, 70_001]):
+        tensors = make(torch, sizes, ["bf16", "f32"], "separate", seed=75)
+        keep = [t.clone() for t in tensors]
+        total = norms64(torch, keep, 1.0, "l2")[0]
+        with GradientList(tensors) as lst:
+            g = torch.cuda.CUDAGraph()
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.graph(g, stream=s):
+                r = lst.clip(total, stream=torch.cuda.current_stream())
+            for factor in (0.5, 2.0, 0.25, 4.0):
+                for t, k in zip(tensors, keep):
+                    t.copy_(k * factor)
+                now = [t.clone() for t in tensors]
+                g.replay()
+                torch.cuda.synchronize()
+                check_norm(torch, r, now, 1.0, total)
+                found = norms64(torch, now, 1.0, "l2")[0]
+                check_clipped(torch, tensors, now, 1.0, min(1.0, total / found))
+
+
+def test_a_list_closed_between_the_passes(torch):
+    sizes = [70001, 8192]
+    tensors = make(torch, sizes, ["bf16"], "separate", seed=76)
+    opts = StepOptions(one_based_update=4, max_grad_norm=1e6)
+    with B200Adamw(TensorTable.from_sizes(sizes)) as opt:
+        got = []
+        for close in (False, True):
+            load(torch, opt, 77)
+            lst = GradientList(tensors)
+            opt.norm_pass(lst, opts)
+            if close:
+                lst.close()
+            opt.update_pass(opts)
+            assert opt.read_result().skipped == 0
+            got.append({k: v.clone() for k, v in opt.state_tensors().items()})
+            lst.close()
+        for k in got[0]:
+            assert torch.equal(got[0][k].view(torch.int16), got[1][k].view(torch.int16))
+        lst = GradientList(tensors)
+        opt.norm_pass(lst, opts)
+        lst.close()  # the handle lets go of it when it is closed itself
+
+
+def test_threads_share_a_list(torch):
+    import threading
+
+    tensors = make(torch, [3_000_001, 77], ["f16"], "separate", seed=78)
+    with GradientList(tensors) as lst:
+        want = lst.norm(per_tensor=True).values.tolist()
+        wrong = []
+
+        def work():
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(100):
+                    r = lst.norm(per_tensor=True, stream=s)
+                    if r.values.tolist() != want:
+                        wrong.append(1)
+
+        torch.cuda.synchronize()
+        pool = [threading.Thread(target=work) for _ in range(4)]
+        for t in pool:
+            t.start()
+        for t in pool:
+            t.join()
+        assert not wrong
 
 
 # ---- sizes beyond 32 bits -----------------------------------------------------------
