@@ -827,17 +827,45 @@ __device__ __forceinline__ void clip_raw(const Raw<T>& raw, const ClipFactor& f,
 }
 
 // What the clip needs of the norm, which may still be on its way: it is waited
-// for once per block, after the first loads have been issued.
+// for once per block, after the first loads have been issued.  Lists of few units
+// have no finalize kernel; every block adds the partials for itself (one launch
+// and one hop less: see kGradOwnNorm).
+struct ClipNorm {
+  const float* result;          // of the finalize kernel, or NULL:
+  const GradPartial* partials;  // what to form it from
+  uint32_t count;
+  float max_norm;
+  int kind;
+  GradListOut out;
+};
 struct ClipState {
-  const float* result;  // in global memory, while not `known`
+  const ClipNorm* norm;
+  float scale;
   float clip, bad;
   bool known;
-  // False when a gradient is not finite, which leaves the outputs alone.
+  // False when a gradient is not finite, which leaves the outputs alone.  Called
+  // by the whole block.
   __device__ __forceinline__ bool ready() {
     if (!known) {
       pdl_wait();
-      clip = __ldcg(result + 1);
-      bad = __ldcg(result + 3);
+      if (norm->result) {
+        clip = __ldcg(norm->result + 1);
+        bad = __ldcg(norm->result + 3);
+      } else {
+        __shared__ LaneSlot lanes;
+        __shared__ float2 s_clip;
+        double sum;
+        uint32_t top;
+        sum_partials<kListThreads>(norm->partials, norm->count, threadIdx.x, 0u, lanes, sum, top);
+        if (threadIdx.x == 0u) {
+          const float4 v = norm_values(sum, top, scale, norm->max_norm, norm->kind);
+          s_clip = make_float2(v.y, v.w);
+          if (blockIdx.x == 0u) write_norm(norm->out, v, unscaled_sum(sum, scale));
+        }
+        __syncthreads();
+        clip = s_clip.x;
+        bad = s_clip.y;
+      }
       known = true;
     }
     return bad == 0.0f;
@@ -1012,8 +1040,9 @@ __device__ __forceinline__ void clip_any(const GradListView& list, const GradLis
 template <uint32_t kOut, uint32_t kRows>
 __global__ void __launch_bounds__(kListThreads,
                                   kRows == kAnyRows || (kRows && kOut == kOutSame) ? 3 : 4)
-    list_clip_kernel(GradListView list, GradListView out, float scale, const float* result) {
-  ClipState state{result, 0.0f, 0.0f, false};
+    list_clip_kernel(GradListView list, GradListView out, float scale,
+                     const __grid_constant__ ClipNorm norm) {
+  ClipState state{&norm, scale, 0.0f, 0.0f, false};
   // In place with a loss scale of one there may be nothing to do: look before
   // anything is loaded.
   if (kOut == kOutSame && scale == 1.0f && (!state.ready() || state.clip == 1.0f)) return;
@@ -1109,7 +1138,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   }
   if constexpr (kClip) {
     __syncthreads();
-    ClipState state{nullptr, s_clip.x, s_clip.y, true};
+    ClipState state{nullptr, scale, s_clip.x, s_clip.y, true};
     if (!state.ready() || (kMode == kOutSame && scale == 1.0f && state.clip == 1.0f)) return;
     for (uint32_t i = begin; i < list.n_units; i += step)
       clip_any<kMode, kAnyRows>(list, to, i, scale, state);
@@ -1549,6 +1578,12 @@ bool all_small_fit(uint32_t c) {
          small_fits<kOutSame>(c) && small_fits<kSmallNorm>(c) && small_fits<kSmallStep>(c);
 }
 
+cudaError_t launch_norm_kernel(const GradListView& list, float scale, const DeviceScaler* scaler,
+                               GradPartial* partials, cudaStream_t stream) {
+  return launch_chained(list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units,
+                        kListThreads, 0, stream, list, scale, scaler, partials);
+}
+
 // A list small enough for one cluster, on a device that can hold one.
 bool is_small(const GradListView& list, uint32_t units) {
   return list.cluster != 0u && list.n_units <= units;
@@ -1563,9 +1598,7 @@ cudaError_t launch_list_norm(const GradListView& list, float scale, float max_no
     return launch_small<kSmallNorm>(list, list, scale, max_norm, kind, out, partials, nullptr,
                                     nullptr, FinalizeParams{}, stream);
   if (list.n_units > 0) {
-    const cudaError_t e = launch_chained(
-        list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units, kListThreads,
-        0, stream, list, scale, static_cast<const DeviceScaler*>(nullptr), partials);
+    const cudaError_t e = launch_norm_kernel(list, scale, nullptr, partials, stream);
     if (e != cudaSuccess) return e;
   }
   const uint32_t tensors = out.tensor_norms || out.tensor_max ? list.n_tensors : 0u;
@@ -1580,10 +1613,8 @@ cudaError_t launch_list_norm_decide(const GradListView& list, GradPartial* parti
   if (is_small(list, kGradSmallStep))
     return launch_small<kSmallStep>(list, list, fp.static_scale, 1.0f, 0, GradListOut{}, partials,
                                     scaler, st, fp, stream);
-  const cudaError_t e = launch_chained(
-      list.rows ? list_norm_kernel<true> : list_norm_kernel<false>, list.n_units, kListThreads, 0,
-      stream, list, fp.static_scale, static_cast<const DeviceScaler*>(fp.dynamic ? scaler : nullptr),
-      partials);
+  const cudaError_t e = launch_norm_kernel(list, fp.static_scale, fp.dynamic ? scaler : nullptr,
+                                           partials, stream);
   if (e != cudaSuccess) return e;
   return launch_list_decide(list, partials, scaler, st, fp, stream);
 }
@@ -1598,7 +1629,7 @@ cudaError_t launch_list_decide(const GradListView& list, const GradPartial* part
 namespace {
 template <uint32_t kOut>
 cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, float scale,
-                           const float* result, cudaStream_t stream) {
+                           const ClipNorm& norm, cudaStream_t stream) {
   const auto kernel = !list.rows && !out.rows ? list_clip_kernel<kOut, kNoRows>
                       : list.off_runs || out.off_runs ? list_clip_kernel<kOut, kAnyRows>
                                                       : list_clip_kernel<kOut, kRowVectors>;
@@ -1608,7 +1639,7 @@ cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, fl
   uint32_t grid = list.n_units;
   if (kOut == kOutSame && scale == 1.0f)
     grid = std::min(grid, list.sms * (list.rows ? 3u : 4u));  // as its launch bounds
-  return launch_chained(kernel, grid, kListThreads, 0, stream, list, out, scale, result);
+  return launch_chained(kernel, grid, kListThreads, 0, stream, list, out, scale, norm);
 }
 }  // namespace
 
@@ -1624,15 +1655,22 @@ cudaError_t launch_list_clip(const GradListView& list, const GradListView& to, b
     return launch(list, to, scale, max_norm, kind, out, partials, nullptr, nullptr,
                   FinalizeParams{}, stream);
   }
-  cudaError_t e = launch_list_norm(list, scale, max_norm, kind, out, partials, stream);
+  ClipNorm norm{out.result, partials, list.n_units, max_norm, kind, out};
+  cudaError_t e = cudaSuccess;
+  if (one_type && list.n_units > 0u && list.n_units <= kGradOwnNorm && !out.tensor_norms &&
+      !out.tensor_max) {
+    norm.result = nullptr;
+    e = launch_norm_kernel(list, scale, nullptr, partials, stream);
+  } else {
+    e = launch_list_norm(list, scale, max_norm, kind, out, partials, stream);
+  }
   if (e != cudaSuccess || list.n_units == 0) return e;
-  if (in_place) return launch_clip_to<kOutSame>(list, list, scale, out.result, stream);
-  if (to.types & (1u << kGradF32))
-    e = launch_clip_to<kGradF32>(list, to, scale, out.result, stream);
+  if (in_place) return launch_clip_to<kOutSame>(list, list, scale, norm, stream);
+  if (to.types & (1u << kGradF32)) e = launch_clip_to<kGradF32>(list, to, scale, norm, stream);
   if (e == cudaSuccess && (to.types & (1u << kGradBf16)))
-    e = launch_clip_to<kGradBf16>(list, to, scale, out.result, stream);
+    e = launch_clip_to<kGradBf16>(list, to, scale, norm, stream);
   if (e == cudaSuccess && (to.types & (1u << kGradF16)))
-    e = launch_clip_to<kGradF16>(list, to, scale, out.result, stream);
+    e = launch_clip_to<kGradF16>(list, to, scale, norm, stream);
   return e;
 }
 

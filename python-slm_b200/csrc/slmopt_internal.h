@@ -296,6 +296,10 @@ constexpr uint64_t kGradKeepBytes = uint64_t(24) << 20;
 // 10.2 / 10.4 / 10.2 / 11.9; clip of 0.25 / 0.5 / 1M 7.8 / 10.5 / 14.8 against 12.4 /
 // 12.6 / 12.4; step on 0.03 / 0.25 / 0.5M 7.2 / 8.0 / 10.3 against 8.2 / 8.4 / 8.7.
 constexpr uint32_t kGradSmallNorm = 192, kGradSmallClip = 80, kGradSmallStep = 40;
+// Up to so many units the clip kernel's blocks add the partials themselves instead
+// of waiting for a kernel that does: 2 / 4 / 8 / 16M bf16 elements 10.4 / 12.3 / 12.3 /
+// 24.6 us a call against 12.9 / 14.7 / 14.6 / 23.1.
+constexpr uint32_t kGradOwnNorm = 1024;
 inline uint32_t grad_unit_elems(uint64_t total) {
   uint32_t u = kGradUnitMin;
   while (u < kGradUnitMax && total / u > kGradUnitsAimed) u *= 2;

@@ -46,22 +46,11 @@ class StepOptions:
     growth_interval: int = 2000
 
     def to_c(self) -> _lib.StepConfig:
-        c = _lib.StepConfig()
-        c.learning_rate = self.learning_rate
-        c.one_based_update = self.one_based_update
-        c.beta1 = self.beta1
-        c.beta2 = self.beta2
-        c.epsilon = self.epsilon
-        c.decay_weight = self.decay_weight
-        c.no_decay_weight = self.no_decay_weight
-        c.max_grad_norm = self.max_grad_norm
-        c.apply_clip = 1 if self.apply_clip else 0
-        c.min_clip_accept = self.min_clip_accept
-        c.nonfinite_policy = self.nonfinite_policy
-        c.loss_scale_mode = self.loss_scale_mode
-        c.static_loss_scale = self.static_loss_scale
-        c.growth_interval = self.growth_interval
-        return c
+        return _lib.StepConfig(
+            self.learning_rate, self.one_based_update, self.beta1, self.beta2, self.epsilon,
+            self.decay_weight, self.no_decay_weight, self.max_grad_norm,
+            1 if self.apply_clip else 0, self.min_clip_accept, self.nonfinite_policy,
+            self.loss_scale_mode, self.static_loss_scale, self.growth_interval)
 
 
 def _grad_pointer(grads):

@@ -340,7 +340,7 @@ def test_extreme_loss_scales(torch, scale, std):
                 check_clipped(torch, [y], [x], scale, min(1.0, limit / found))
 
 
-LIMITS = [n * 8192 + d for n in (40, 80, 192) for d in (-1, 0, 1)]
+LIMITS = [n * 8192 + d for n in (40, 80, 192, 1024) for d in (-1, 0, 1)]
 
 
 @pytest.mark.parametrize("n", LIMITS)
@@ -355,10 +355,11 @@ def test_around_the_sizes_where_the_form_changes(torch, n):
             B200Adamw(TensorTable.from_sizes(sizes)) as opt:
         assert float(lst.norm().sum_squares) == want
         check_norm(torch, lst.norm(per_tensor=True), before, 1.0, 1.0)
-        r = lst.clip(total / 2, out=to, per_tensor=True)
-        assert float(r.sum_squares) == want
-        check_norm(torch, r, before, 1.0, total / 2)
-        check_clipped(torch, targets, before, 1.0, 0.5)
+        for per_tensor in (True, False):
+            r = lst.clip(total / 2, out=to, per_tensor=per_tensor)
+            assert float(r.sum_squares) == want
+            check_norm(torch, r, before, 1.0, total / 2)
+            check_clipped(torch, targets, before, 1.0, 0.5)
         start = load(torch, opt, 15)
         opts = StepOptions(one_based_update=10, max_grad_norm=float(np.float32(total / 2)))
         assert opt.step(lst, opts).sum_squares == want
