@@ -1,19 +1,22 @@
 // Kernels over gradient lists: tensors that lie where the backward pass left
 // them, in f32, bf16 or f16, contiguous or as rows with a pitch.
 //
-//   list_norm_kernel        -- one block per unit: unscale, squares, the unit's
-//                              f64 partial and largest magnitude.
-//   list_finalize_kernel    -- block 0: norm, clip scale, non-finite flag; one
-//                              more block per tensor for the tensors' own norms.
+//   list_norm_kernel        -- one block per unit: squares, the unit's f64 partial
+//                              and largest magnitude.
+//   list_finalize_kernel    -- norm, clip scale, non-finite flag; the tensors' own.
 //   list_clip_kernel        -- one block per unit: unscale, clip, write.
-//   list_accumulate_kernel  -- one block per unit: into the flat f32 accumulator
-//                              (and the partials of the sums, last micro-batch).
+//   list_small_kernel       -- norm, clip or the step's decision of a small list.
+//   list_accumulate_kernel, list_accumulate_norm_kernel -- into the flat f32
+//                              accumulator (and the partials of the sums, for the
+//                              last micro-batch).
 //   list_decide_kernel, list_update_kernel -- the optimizer step on a list.
 //
-// All of them stream; nothing is a contraction.  The kernels of one call are
+// All of them stream; nothing is a contraction, so no tensor cores.  What each is
+// bound by and measured stands at the kernel.  The kernels of one call are
 // chained by programmatic dependent launch: each lets the next one become
 // resident at once and the next one waits for its results (pdl_wait) after it
-// has issued what loads do not depend on them.
+// has issued what loads do not depend on them.  A kernel triggers only after its
+// own wait, so whatever has started early sees the gradients' producers finished.
 #include "step_device.cuh"
 
 #include <cuda_bf16.h>
@@ -340,6 +343,14 @@ __device__ __forceinline__ GradUnit load_unit(const GradUnit* units, uint32_t i)
 }
 
 // ---- norm ----------------------------------------------------------------------
+// One read of the gradients: 2 or 4 bytes an element, so DRAM should bound it; a
+// first form (unscaling and squaring each value, 66 warp instructions an 8-element
+// vector) was bound by issue at 71 % instead.  Squares by packed fused multiply-adds of the
+// stored values take 40, 32 registers keep 8 blocks of 256 threads a SM resident
+// with 64 bytes a thread on their way: 135M bf16 in 41.8 us with the finalize
+// (6.5 TB/s; a kernel that only reads the same bytes takes 39.4-42.7), 49 us at
+// the start.  Off the vector boundaries a vector costs two loads and a shift:
+// 120M bf16 in odd-sized packed tensors 54.7 us against 39.2.
 // Squares are formed of the stored values times a power of two: 1 for loss
 // scales of 1 to 2^20, else the one next to 1 / scale, so that they are in the
 // range of the unscaled values' (within 2^40) without a division per element;
@@ -741,6 +752,11 @@ __global__ void __launch_bounds__(kLanes)
 }
 
 // ---- clip ----------------------------------------------------------------------
+// y = round(x * (clip / scale)): a second read and the write behind the norm's
+// read.  DRAM bounds it: 135M bf16 read, mostly read again (the L2 keeps the last
+// 24 MB, see kGradKeepBytes) and written are 790 MB, 120 us at 6.57 TB/s; measured
+// 125 us.  Keeping more on chip than the L2 does was not tried: 30 MB of shared
+// memory would save 4.6 us.
 constexpr uint32_t kNoRows = 0u, kRowVectors = 1u, kAnyRows = 2u;
 template <uint32_t T>
 __device__ __forceinline__ uint32_t to_bits(float y) {
@@ -1060,7 +1076,9 @@ __global__ void __launch_bounds__(kListThreads,
 // One launch of one thread-block cluster for lists whose time is latency: the
 // partials, a cluster barrier, and the norm (every block for itself where it
 // goes on to clip) from the same tree.  A block works on 4 units at a time; unit
-// i goes to block i % cluster first.
+// i goes to block i % cluster first.  16 blocks (8 where 16 do not fit) of 1,024
+// threads: 0.1M bf16 in 9 tensors 7.6 us a call, of which 5.0 on the GPU, against
+// 10.2 us for the two kernels; 8 blocks are slower from 0.25M on, 4 much.
 constexpr uint32_t kSmallThreads = 1024;
 constexpr uint32_t kSmallGroups = kSmallThreads / kListThreads;
 constexpr uint32_t kSmallNorm = 4u, kSmallStep = 5u;  // kMode; 0..3: clip to kOut
@@ -1146,6 +1164,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
 }
 
 // ---- accumulate ------------------------------------------------------------------
+// acc = micro or acc + micro, one f32 rounding an element: 10 bytes an element from
+// bf16 (6 to start an update), so DRAM alone bounds it.  32-byte loads and stores
+// of the accumulator, everything first to leave the L2, 8,192 elements a block:
+// 135M from bf16 in 199.5 us (6.78 TB/s; a plain copy reaches 6.57), 216 us with
+// 2,048 a block, 204 with 16,384.
+constexpr uint32_t kAccElems = 8192;
 __device__ __forceinline__ void load_acc(const float* p, float (&y)[8]) {
   asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]), "=f"(y[4]), "=f"(y[5]),
@@ -1248,8 +1272,7 @@ __device__ __forceinline__ void accumulate_rows(const GradUnit& u, float* dst, b
 }
 
 template <uint32_t T, bool kRows>
-__device__ __forceinline__ void accumulate_unit(const GradUnit& u, const GradListView& list,
-                                                float* acc, bool overwrite) {
+__device__ __forceinline__ void accumulate_unit(const GradUnit& u, float* acc, bool overwrite) {
   float* dst = acc + u.offset;
   if (kRows && (u.flags & kGradPitched))
     accumulate_rows<T>(u, dst, overwrite);
@@ -1257,16 +1280,39 @@ __device__ __forceinline__ void accumulate_unit(const GradUnit& u, const GradLis
     accumulate_flat<T>(static_cast<const uint8_t*>(u.ptr), dst, u.count, overwrite);
 }
 
+// Elements [begin, begin + n) of a unit as a unit of their own.
+template <bool kRows>
+__device__ __forceinline__ void slice_unit(GradUnit& u, uint32_t begin, uint32_t n) {
+  uint64_t at = begin;
+  if (kRows && (u.flags & kGradPitched)) {
+    const uint32_t k = u.column + begin;
+    const uint32_t row = k / u.columns;
+    const uint32_t column = k - row * u.columns;
+    at = row * u.row_stride + column - u.column;
+    u.column = column;
+  }
+  u.ptr = static_cast<const uint8_t*>(u.ptr) + at * elem_bytes(u.flags & kGradTypeMask);
+  u.offset += begin;
+  u.count = u.count - begin < n ? u.count - begin : n;
+  if (begin > 0u) u.index = 1u;  // not at the tensor's start
+}
+
+// A block per kAccElems elements of a unit.
 template <bool kRows>
 __global__ void __launch_bounds__(kListThreads, 4)
-    list_accumulate_kernel(GradListView list, float* acc, int overwrite) {
-  const GradUnit u = load_unit<kRows>(list.units, blockIdx.x);
+    list_accumulate_kernel(GradListView list, uint32_t blocks_per_unit, float* acc,
+                           int overwrite) {
+  const uint32_t unit = blockIdx.x / blocks_per_unit;
+  const uint32_t begin = (blockIdx.x - unit * blocks_per_unit) * kAccElems;
+  GradUnit u = load_unit<kRows>(list.units, unit);
   pdl_wait();
   pdl_trigger();  // whoever starts early waits for this kernel before it reads
+  if (begin >= u.count) return;
+  slice_unit<kRows>(u, begin, kAccElems);
   switch (u.flags & kGradTypeMask) {
-    case kGradF32: return accumulate_unit<kGradF32, kRows>(u, list, acc, overwrite != 0);
-    case kGradBf16: return accumulate_unit<kGradBf16, kRows>(u, list, acc, overwrite != 0);
-    default: return accumulate_unit<kGradF16, kRows>(u, list, acc, overwrite != 0);
+    case kGradF32: return accumulate_unit<kGradF32, kRows>(u, acc, overwrite != 0);
+    case kGradBf16: return accumulate_unit<kGradBf16, kRows>(u, acc, overwrite != 0);
+    default: return accumulate_unit<kGradF16, kRows>(u, acc, overwrite != 0);
   }
 }
 
@@ -1369,12 +1415,12 @@ __global__ void __launch_bounds__(kListThreads)
 // not whole within the tensor goes element by element, and a gradient off the
 // boundaries is shifted.
 //
-// All loads are in flight before the norm is finished (pdl_wait), 64 registers
-// and 128 threads a block keep 112 KB a SM on their way, and the hardware
-// balances the blocks.  135M elements, bf16: 607 us (6.24 TB/s of 28 bytes an
-// element) against 625 us for tiles through shared memory by bulk copies (2 stages,
-// 3 blocks a SM); with 256 / 512 threads a block 620 / 645 us, with two vectors a
-// thread 719 us.
+// 28 bytes an element (bf16 gradients), bound by DRAM: all loads are in flight
+// before the norm is finished (pdl_wait), 62 registers and 128 threads a block keep
+// 112 KB a SM on their way, and the hardware balances the blocks.  135M elements:
+// step 615-630 us, of which the update 570-585 (6.5 TB/s).  The flat step's form
+// (2,048-element tiles by bulk copies into shared memory, 3 blocks a SM) took
+// 667 us here; 256 / 512 threads a block 663 / 688, two vectors a thread 761.
 constexpr uint32_t kUpdateBlock = 128;
 constexpr uint32_t kUpdateElems = kUpdateBlock * kVec;
 
@@ -1677,8 +1723,11 @@ cudaError_t launch_list_clip(const GradListView& list, const GradListView& to, b
 cudaError_t launch_list_accumulate(const GradListView& list, float* acc, int overwrite,
                                    cudaStream_t stream) {
   if (list.n_units == 0) return cudaSuccess;
-  return launch_chained(list.rows ? list_accumulate_kernel<true> : list_accumulate_kernel<false>, list.n_units, kListThreads, 0, stream, list, acc,
-                        overwrite);
+  const uint32_t per_unit = list.unit_elems / kAccElems;
+  const uint64_t blocks = uint64_t(list.n_units) * per_unit;
+  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+  return launch_chained(list.rows ? list_accumulate_kernel<true> : list_accumulate_kernel<false>,
+                        uint32_t(blocks), kListThreads, 0, stream, list, per_unit, acc, overwrite);
 }
 
 cudaError_t launch_list_accumulate_norm(const GradListView& list, float* acc, int overwrite,

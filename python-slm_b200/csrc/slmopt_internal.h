@@ -277,10 +277,10 @@ struct __align__(16) GradUnit {
 };
 static_assert(sizeof(GradTensor) == 48 && sizeof(GradUnit) == 48, "list tables");
 // The smallest and largest unit; between them a list has at most about
-// kGradUnitsAimed, which bounds the partials that its norm has to add.  4,096 and
-// 16,384 elements were slower than 8,192: the norm of 30M values in 257 tensors 26.9
-// against 23.2 us, clip of 24M f32 62.8 / 53.4, accumulate of 135M 208.7 (16,384)
-// / 204.1.
+// kGradUnitsAimed, which bounds the partials that its norm has to add.  Units of
+// 4,096 / 8,192: the norm of 30M values in 257 tensors 26.9 / 23.2 us, clip of 24M
+// f32 in columns 62.8 / 53.4; of 8,192 / 16,384 / 32,768: norm of 135M bf16 44.6 / 41.8 /
+// 42.8 us, its clip 137 / 126 / 127.
 constexpr uint32_t kGradUnitMin = 8192;
 constexpr uint32_t kGradUnitMax = 1u << 26;
 constexpr uint64_t kGradUnitsAimed = 16384;
@@ -310,13 +310,13 @@ struct GradListView {
   const GradTensor* tensors;
   uint32_t n_units, n_tensors;
   uint32_t unit_elems;
-  uint32_t rows;   // whether any tensor is pitched
+  uint32_t rows;         // whether any tensor is pitched
   uint32_t off_runs;     // whether any tensor is not kGradVector
   uint32_t off_vectors;  // whether any tensor starts inside a vector of the flat order
-  uint32_t types;  // bit per type of a tensor with elements
-  uint32_t cluster;  // blocks of the cluster for small lists, see list_small_cluster
-  uint32_t sms;      // of the device
-  uint32_t keep;   // units from here on stay in the L2 for a second pass
+  uint32_t types;        // bit per type of a tensor with elements
+  uint32_t cluster;      // blocks of the cluster for small lists, see list_small_cluster
+  uint32_t sms;          // of the device
+  uint32_t keep;         // units from here on stay in the L2 for a second pass
   uint64_t elements;
 };
 struct GradListOut {
