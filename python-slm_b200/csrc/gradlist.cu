@@ -23,6 +23,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace slmopt {
@@ -1636,7 +1637,19 @@ bool is_small(const GradListView& list, uint32_t units) {
 }
 }  // namespace
 
-uint32_t list_small_cluster() { return all_small_fit(16u) ? 16u : all_small_fit(8u) ? 8u : 0u; }
+uint32_t list_small_cluster() {
+  // Looked up once per device (the answer, plus one).
+  constexpr int kMaxDevices = 64;
+  static std::atomic<uint32_t> known[kMaxDevices];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return 0u;
+  uint32_t c = known[device].load(std::memory_order_acquire);
+  if (c == 0u) {
+    c = 1u + (all_small_fit(16u) ? 16u : all_small_fit(8u) ? 8u : 0u);
+    known[device].store(c, std::memory_order_release);
+  }
+  return c - 1u;
+}
 
 cudaError_t launch_list_norm(const GradListView& list, float scale, float max_norm, int kind,
                              const GradListOut& out, GradPartial* partials, cudaStream_t stream) {

@@ -249,7 +249,7 @@ bool collides(const slm_grad_list& list, const slm_grad_list& out) {
       const uint32_t a = list.extents[j].tensor, b = o.tensor;
       const GradTensor &x = list.tensors[a], &y = out.tensors[b];
       if (a == b && x.ptr == y.ptr && x.flags == y.flags &&
-          (!(x.flags & kGradPitched) || x.row_stride == y.row_stride))
+          (!(x.flags & kGradPitched) || (x.row_stride == y.row_stride && x.columns == y.columns)))
         continue;
       if (share_elements(x, y)) return true;
     }
@@ -480,6 +480,7 @@ int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_st
   int st = check_config(h, cfg);
   if (!st) st = check_step_list(h, list);
   if (st) return st;
+  if (h->broken) return h->err(SLM_ERR_INTERNAL, "a previous step failed inside a kernel");
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if ((st = phase_begin(h, s))) return st;

@@ -17,11 +17,17 @@ _SHARED_BYTES = 4096
 _KINDS = {"l2": _lib.NORM_L2, "max": _lib.NORM_MAX}
 
 
-def _dtype_codes():
-    import torch
+_CODES: dict = {}
 
-    return {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
-            torch.float16: _lib.DTYPE_F16}
+
+def _dtype_codes() -> dict:
+    """slm_dtype by torch dtype."""
+    if not _CODES:
+        import torch
+
+        _CODES.update({torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
+                       torch.float16: _lib.DTYPE_F16})
+    return _CODES
 
 
 def _rows(tensor) -> tuple[int, int, int]:
@@ -126,19 +132,15 @@ class GradientList:
         self.tensors = tuple(tensors)
         if not self.tensors:
             raise ValueError("the list contains no tensors")
-        views = (_lib.GradView * len(self.tensors))()
-        codes = _dtype_codes()
-        self._shapes = []
         first = self.tensors[0]
         if not isinstance(first, torch.Tensor) or not first.is_cuda:
             raise ValueError("gradients must be CUDA tensors")
         self.device = first.device
-        for view, t in zip(views, self.tensors):
-            layout = self._layout(t)
-            view.data = t.data_ptr()
-            view.rows, view.columns, view.row_stride = layout[1:]
-            view.dtype = codes[t.dtype]
-            self._shapes.append(layout)
+        self._shapes = [self._layout(t) for t in self.tensors]
+        codes = _dtype_codes()
+        views = (_lib.GradView * len(self.tensors))(
+            *[(t.data_ptr(), rows, columns, stride, codes[dtype])
+              for t, (dtype, rows, columns, stride) in zip(self.tensors, self._shapes)])
         h = ctypes.c_void_p()
         _lib.check(self.lib.slm_grad_list_create(views, len(self.tensors), self.device.index,
                                                  ctypes.byref(h)))
@@ -150,6 +152,7 @@ class GradientList:
         self._norm_call, self._clip_call = self.lib.slm_grad_list_norm, self.lib.slm_grad_list_clip
 
     def _layout(self, t):
+        """(dtype, rows, columns, row stride) of a tensor that the list can take."""
         import torch
 
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -160,6 +163,9 @@ class GradientList:
             raise TypeError("gradients must be float32, bfloat16 or float16")
         if t.layout != torch.strided or t.is_neg():
             raise ValueError("gradients must be dense tensors, not lazily negated views")
+        if t.is_contiguous():
+            n = t.numel()
+            return t.dtype, 1, n, n
         return (t.dtype, *_rows(t))
 
     def __len__(self) -> int:

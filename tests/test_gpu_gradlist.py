@@ -418,6 +418,8 @@ def test_clip_refuses_outputs_that_share_elements(torch):
         ([a[:500], a[500:]], [a[500:], a[:500]]),
         ([a], [torch.ones(999, device="cuda")]),
         ([a], [a[:500], a[500:]]),
+        ([w[:6, :4]], [w[:4, :6]]),           # as many elements from the same one on, other rows
+        ([w[:, :30]], [w[:, 1:31]]),
     ]
     for tensors, targets in refused:
         with GradientList(tensors) as lst:
