@@ -149,6 +149,7 @@ class GradientList:
         self._work_bytes = int(self.lib.slm_grad_list_workspace_bytes(h))
         # What every call needs, looked up once.
         self._empty, self._f32, self._index = torch.empty, torch.float32, self.device.index
+        self._tensor_type, self._strided = torch.Tensor, torch.strided
         self._norm_call, self._clip_call = self.lib.slm_grad_list_norm, self.lib.slm_grad_list_clip
 
     def _layout(self, t):
@@ -167,6 +168,14 @@ class GradientList:
             n = t.numel()
             return t.dtype, 1, n, n
         return (t.dtype, *_rows(t))
+
+    def _is(self, t, shape) -> bool:
+        """Whether t has this layout (the common case, contiguous, without detours)."""
+        if type(t) is self._tensor_type and t.get_device() == self._index and \
+                t.dtype is shape[0] and shape[1] == 1 and t.layout is self._strided and \
+                t.is_contiguous() and t.numel() == shape[2]:
+            return not t.is_neg()
+        return self._layout(t) == shape
 
     def __len__(self) -> int:
         return len(self.tensors)
@@ -197,7 +206,8 @@ class GradientList:
     def bind(self, tensors, stream=None) -> None:
         """Take other tensors of the same types, sizes and strides, in order."""
         tensors = tuple(tensors)
-        if [self._layout(t) for t in tensors] != self._shapes:
+        if len(tensors) != len(self._shapes) or \
+                not all(self._is(t, shape) for t, shape in zip(tensors, self._shapes)):
             raise ValueError("other tensors than the list's: types, sizes and strides must agree")
         ptrs = (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
         _lib.check(self.lib.slm_grad_list_bind(self.handle, ptrs, len(tensors),

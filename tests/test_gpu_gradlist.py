@@ -1058,3 +1058,54 @@ def test_column_offsets_beyond_32_bits(torch):
         lst.accumulate(acc, overwrite=True)
         assert torch.equal(acc, torch.cat([aligned.reshape(-1), odd.reshape(-1)]).float())
     del wide
+
+
+def test_bind_takes_only_what_the_list_was_made_of(torch):
+    a = [torch.ones(100, device="cuda"), torch.ones(6, 20, device="cuda").bfloat16()[:, :10]]
+    same = [torch.full((100,), 2.0, device="cuda"),
+            torch.full((6, 20), 2.0, device="cuda").bfloat16()[:, 5:15]]
+    other = [
+        [same[0]], [same[0], same[1], same[0]],
+        [same[0].bfloat16(), same[1]],               # another type
+        [same[0][:99], same[1]],                      # another size
+        [same[0], same[1].contiguous()],              # another layout
+        [same[0], torch.ones(6, 30, device="cuda").bfloat16()[:, :10]],
+        [torch.ones(200, device="cuda")[::2], same[1]],
+    ]
+    with GradientList(a) as lst:
+        before = lst.norm().read().norm
+        for tensors in other:
+            with pytest.raises(ValueError):
+                lst.bind(tensors)
+        with pytest.raises(ValueError):
+            lst.bind([same[0].cpu(), same[1]])
+        assert lst.norm().read().norm == before and lst.tensors == tuple(a)
+        # the same elements in another shape are the same run in memory
+        lst.bind([same[0].view(10, 10), same[1]])
+        near(lst.norm().read().norm, 2.0 * math.sqrt(160), 4 * U, "norm")
+
+
+def test_closed_lists_are_refused_and_a_list_is_its_own_output(torch):
+    x, y = torch.full((9000,), 2.0, device="cuda"), torch.empty(9000, device="cuda")
+    closed, lst = GradientList([y]), GradientList([x])
+    closed.close()
+    closed.close()
+    for call in (closed.norm, closed.clip, lambda: closed.accumulate(y),
+                 lambda: closed.bind([y]), lambda: lst.clip(out=closed)):
+        with pytest.raises(ValueError):
+            call()
+    lst.clip(1.0, out=lst)
+    near(float(x[77]), 1.0 / math.sqrt(9000), 8 * U, "clipped")
+    lst.close()
+
+
+def test_phase_times_of_a_step_on_a_list(torch):
+    sizes = [70001, 8192]
+    tensors = make(torch, sizes, ["bf16"], "separate", seed=90)
+    with B200Adamw(TensorTable.from_sizes(sizes)) as opt, GradientList(tensors) as lst:
+        load(torch, opt, 91)
+        opt.phase_timing(True)
+        for t in (1, 2, 3):
+            opt.step(lst, StepOptions(one_based_update=t))
+        times, steps = opt.phase_times()
+        assert len(times) == 2 and steps == 3 and all(v > 0.0 for v in times.values())
