@@ -492,8 +492,8 @@ int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, floa
                        double* sum_squares_device, void* workspace_device,
                        uint64_t workspace_bytes, void* stream);
 /* slm_grad_accumulate from a list: acc_device (n == the list's elements, f32,
- * 16-byte aligned) += the list's values, tensor after tensor, or with overwrite
- * = them. */
+ * 16-byte aligned, NULL only for a list without elements) += the list's values,
+ * tensor after tensor, or with overwrite = them. */
 int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint64_t n,
                              int overwrite, void* stream);
 /* slm_opt_step, slm_opt_norm_pass and slm_opt_norm_pass_accumulate with the

@@ -459,7 +459,9 @@ int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, floa
 
 int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint64_t n,
                              int overwrite, void* stream) {
-  if (!list || !acc_device) return fail(SLM_ERR_INVALID_ARGUMENT, "NULL argument");
+  // An accumulator without elements may have no address.
+  if (!list || (!acc_device && list->elements))
+    return fail(SLM_ERR_INVALID_ARGUMENT, "NULL argument");
   if (n != list->elements)
     return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator needs one value per list element");
   if (reinterpret_cast<uintptr_t>(acc_device) % 16 != 0)

@@ -232,6 +232,18 @@ def test_norm_of_zeros_and_of_nothing(torch):
             lst.clip()
 
 
+def test_accumulate_of_nothing(torch):
+    with GradientList([torch.zeros(0, device="cuda"), torch.zeros(0, 4, device="cuda")]) as lst:
+        lst.accumulate(torch.zeros(0, device="cuda"))
+        lst.accumulate(torch.zeros(0, device="cuda"), overwrite=True)
+        with pytest.raises(ValueError):
+            lst.accumulate(torch.zeros(1, device="cuda"))
+    with GradientList([torch.zeros(3, device="cuda")]) as lst:
+        with pytest.raises(SlmError):  # elements, but no accumulator
+            _lib.check(lst.lib.slm_grad_list_accumulate(lst.handle, None, 3, 0, None))
+    torch.cuda.synchronize()
+
+
 def test_squares_that_overflow_count_as_non_finite(torch):
     with GradientList([torch.full((100,), 1e20, device="cuda")]) as lst:
         v = lst.norm().values.tolist()
