@@ -54,41 +54,55 @@ def _rows(tensor) -> tuple[int, int, int]:
 
 
 class GradientNorm:
-    """What a norm or clip call found, in device memory (reading a property that
-    is a tensor does not wait; ``read`` does).
+    """What a norm or clip call found, in device memory.  The properties are
+    tensors: taking one does not wait on the host, it orders torch's current stream
+    behind the call's stream; ``read`` waits.  (Inside a capture nothing is ordered:
+    a call is captured on the capture's own stream.  A replay of a captured call
+    renews the values in the replay's stream order.)
 
     ``values`` is one f32 tensor: the norm of all gradients divided by the loss
     scale, the clip scale, the largest magnitude, 1.0 if a gradient or the norm
     is not finite (the clip scale is then 0.0) else 0.0; and with per_tensor each
     tensor's norm, then each tensor's largest magnitude."""
 
-    __slots__ = ("_buffer", "_count", "_tensors")
+    __slots__ = ("_buffer", "_count", "_tensors", "_index", "_stream", "_after")
 
-    def __init__(self, buffer, count: int, tensors: int):
+    def __init__(self, buffer, count: int, tensors: int, index: int, stream: int):
         # f32: the values, the f64 sum of squares, and scratch of the call.
         self._buffer = buffer
         self._count = count
         self._tensors = tensors
+        self._index = index     # of the device
+        self._stream = stream   # the call's
+        self._after = stream    # the last one ordered behind it
+
+    def _ready(self):
+        """The buffer, with the current stream behind the call."""
+        current = _current_stream(self._index)
+        if current != self._after and current != self._stream and \
+                _order_behind(self._buffer, self._index, self._stream):
+            self._after = current
+        return self._buffer
 
     @property
     def values(self):
-        return self._buffer.as_strided((self._count,), (1,))
+        return self._ready().as_strided((self._count,), (1,))
 
     @property
     def norm(self):
-        return self._buffer[0]
+        return self._ready()[0]
 
     @property
     def clip_scale(self):
-        return self._buffer[1]
+        return self._ready()[1]
 
     @property
     def max_abs(self):
-        return self._buffer[2]
+        return self._ready()[2]
 
     @property
     def nonfinite(self):
-        return self._buffer[3]
+        return self._ready()[3]
 
     @property
     def sum_squares(self):
@@ -96,23 +110,23 @@ class GradientNorm:
         tensors add up."""
         import torch
 
-        return self._buffer[self._count:self._count + 2].view(torch.float64)[0]
+        return self._ready()[self._count:self._count + 2].view(torch.float64)[0]
 
     @property
     def tensor_norms(self):
         if self._count == 4:
             raise ValueError("the call was made without per_tensor")
-        return self._buffer[4:4 + self._tensors]
+        return self._ready()[4:4 + self._tensors]
 
     @property
     def tensor_max(self):
         if self._count == 4:
             raise ValueError("the call was made without per_tensor")
-        return self._buffer[4 + self._tensors:self._count]
+        return self._ready()[4 + self._tensors:self._count]
 
     def read(self) -> _lib.ListNorm:
         """The four values on the host; waits for them."""
-        return _lib.ListNorm(*self._buffer[:4].tolist())
+        return _lib.ListNorm(*self._ready()[:4].tolist())
 
 
 class GradientList:
@@ -259,7 +273,7 @@ class GradientList:
                                  self._work_bytes, s)
         if st:
             _lib.check(st)
-        return GradientNorm(buffer, count, n)
+        return GradientNorm(buffer, count, n, self._index, s or 0)
 
     def accumulate(self, acc, overwrite: bool = False, stream=None) -> None:
         """acc (f32, one value per element, tensor after tensor) += the
@@ -285,11 +299,31 @@ def _current_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _torch_stream(stream: int | None, index: int):
+    """torch's object for a stream handle (None or 0: the legacy default stream)."""
+    import torch
+
+    if not stream:
+        return torch.cuda.default_stream(index)
+    return torch.cuda.ExternalStream(stream, device=index)
+
+
 def _use_on(tensor, stream: int | None) -> None:
     """Tells torch's allocator that memory it gave for the current stream is used
     on another one."""
+    tensor.record_stream(_torch_stream(stream, tensor.device.index))
+
+
+def _order_behind(tensor, index: int, stream: int) -> bool:
+    """Lets torch's current stream wait for what is on ``stream``, where ``tensor``
+    was written, and tells the allocator that it is read there.  False inside a
+    capture, which cannot wait for work outside of it."""
     import torch
 
-    handle = stream or 0
-    tensor.record_stream(torch.cuda.ExternalStream(handle, device=tensor.device) if handle else
-                         torch.cuda.default_stream(tensor.device))
+    with torch.cuda.device(index):
+        if torch.cuda.is_current_stream_capturing():
+            return False
+        current = torch.cuda.current_stream()
+        current.wait_stream(_torch_stream(stream, index))
+        tensor.record_stream(current)
+    return True

@@ -1,0 +1,93 @@
+"""Gradient lists and streams without a GPU: in which order the wrapper allocates,
+calls, waits and reads.  The library and torch's streams are stand-ins."""
+from __future__ import annotations
+
+import ctypes
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from slmopt import GradientList, gradlist
+
+CURRENT, OTHER = 5, 7  # stream handles
+
+
+@pytest.fixture
+def log(monkeypatch):
+    """What happens to streams, in order; torch's current stream is CURRENT."""
+    events = []
+    now = SimpleNamespace(stream=CURRENT)
+    monkeypatch.setattr(gradlist, "_current_stream", lambda index: now.stream)
+    monkeypatch.setattr(gradlist, "_use_on", lambda t, s: events.append(("use", s or 0)),
+                        raising=False)
+
+    def order(tensor, index, stream):
+        events.append(("wait", now.stream, stream))
+        return True
+
+    monkeypatch.setattr(gradlist, "_order_behind", order, raising=False)
+    return SimpleNamespace(events=events, now=now)
+
+
+def a_list(log, work_bytes=64):
+    """A GradientList of two tensors whose library and allocator are stand-ins."""
+    lst = GradientList.__new__(GradientList)
+    lst._h = ctypes.c_void_p(1)
+    lst.tensors = (torch.ones(3), torch.ones(2))
+    lst.device, lst._index = torch.device("cpu"), 0
+    lst.elements, lst._work_bytes, lst._f32 = 5, work_bytes, torch.float32
+
+    def empty(n, dtype, device):
+        log.events.append(("allocate", log.now.stream))
+        return torch.zeros(n, dtype=dtype)
+
+    def call(h, *args):
+        # The kernel is a stand-in: the norm of these tensors, written at once.
+        log.events.append(("call", args[-1] or 0))
+        values = args[-7]
+        ctypes.memmove(values, (ctypes.c_float * 4)(5.0 ** 0.5, 0.25, 1.0, 0.0), 16)
+        return 0
+
+    lst._empty, lst._norm_call, lst._clip_call = empty, call, call
+    lst.lib = SimpleNamespace(slm_grad_list_destroy=lambda h: 0)
+    return lst
+
+
+READS = {
+    "read": lambda r: r.read().norm,
+    "norm": lambda r: r.norm.item(),
+    "clip_scale": lambda r: r.clip_scale.item(),
+    "max_abs": lambda r: r.max_abs.item(),
+    "nonfinite": lambda r: r.nonfinite.item(),
+    "values": lambda r: r.values.tolist(),
+    "sum_squares": lambda r: r.sum_squares.item(),
+    "tensor_norms": lambda r: r.tensor_norms.tolist(),
+    "tensor_max": lambda r: r.tensor_max.tolist(),
+}
+
+
+@pytest.mark.parametrize("stream", [OTHER, None])
+@pytest.mark.parametrize("take", READS.values(), ids=READS.keys())
+def test_results_are_read_behind_the_call(log, take, stream):
+    lst = a_list(log)
+    r = lst.norm(per_tensor=True, stream=stream)
+    assert ("call", stream or 0) in log.events and not any(e[0] == "wait" for e in log.events)
+    take(r)
+    assert log.events[-1] == ("wait", CURRENT, stream or 0)
+    take(r)  # once is enough
+    assert sum(e[0] == "wait" for e in log.events) == 1
+    log.now.stream = 9
+    take(r)
+    assert log.events[-1] == ("wait", 9, stream or 0)
+
+
+def test_results_of_the_current_stream_wait_for_nothing(log):
+    r = a_list(log).norm(stream=CURRENT)
+    assert r.read().norm == pytest.approx(5.0 ** 0.5)
+    r.values
+    assert not any(e[0] == "wait" for e in log.events)
+    log.now.stream = 0
+    r = a_list(log).norm()  # None is the legacy default stream, torch's stream 0
+    r.read()
+    assert not any(e[0] == "wait" for e in log.events)
