@@ -79,7 +79,7 @@ class GradientNorm:
     def _ready(self):
         """The buffer, with the current stream behind the call."""
         current = _current_stream(self._index)
-        if current != self._after and current != self._stream and \
+        if current != self._stream and current != self._after and \
                 _order_behind(self._buffer, self._index, self._stream):
             self._after = current
         return self._buffer
@@ -251,16 +251,19 @@ class GradientList:
         # A small workspace shares the results' allocation; a large one is freed
         # with the call instead of living as long as the results.
         head = (count + 5) & ~3
+        # Both come from the memory of the stream that the call runs on: another
+        # stream's may still be in use by what is queued there.
         small = self._work_bytes <= _SHARED_BYTES
-        buffer = self._empty(head + self._work_bytes // 4 if small else head, dtype=self._f32,
-                             device=self.device)
-        work = buffer if small else self._empty(self._work_bytes // 4, dtype=self._f32,
-                                                device=self.device)
-        s = stream if stream is None or type(stream) is int else _stream_handle(stream)
-        if _current_stream(self._index) != (s or 0):
-            _use_on(buffer, s)
-            if not small:
-                _use_on(work, s)
+        s = None if stream is None else _stream_handle(stream)
+        on = s or 0
+        if _current_stream(self._index) != on:
+            with _on_stream(self._index, s):
+                buffer, work = self._room(head, small)
+        elif small:
+            buffer = work = self._empty(head + self._work_bytes // 4, dtype=self._f32,
+                                        device=self.device)
+        else:
+            buffer, work = self._room(head, False)
         v = buffer.data_ptr()
         w = v + 4 * head if small else work.data_ptr()
         norms, tops = (v + 16, v + 16 + 4 * n) if per_tensor else (None, None)
@@ -273,7 +276,15 @@ class GradientList:
                                  self._work_bytes, s)
         if st:
             _lib.check(st)
-        return GradientNorm(buffer, count, n, self._index, s or 0)
+        return GradientNorm(buffer, count, n, self._index, on)
+
+    def _room(self, head: int, small: bool):
+        """Results and workspace of a call, from the current stream's memory."""
+        buffer = self._empty(head + self._work_bytes // 4 if small else head, dtype=self._f32,
+                             device=self.device)
+        if small:
+            return buffer, buffer
+        return buffer, self._empty(self._work_bytes // 4, dtype=self._f32, device=self.device)
 
     def accumulate(self, acc, overwrite: bool = False, stream=None) -> None:
         """acc (f32, one value per element, tensor after tensor) += the
@@ -288,15 +299,20 @@ class GradientList:
 
 
 def _stream_handle(stream) -> int | None:
-    if stream is None or isinstance(stream, int):
-        return stream
-    return int(stream.cuda_stream)  # torch.cuda.Stream
+    """The handle of a torch stream or a handle; None or 0: the legacy default stream."""
+    if stream is None:
+        return None
+    handle = stream if isinstance(stream, int) else int(stream.cuda_stream)
+    return 0 if handle == 1 else handle  # 1: cudaStreamLegacy, the same stream
 
 
 def _current_stream(index: int) -> int:
+    """The handle of a device's current stream; from the first call on torch's own lookup."""
+    global _current_stream
     import torch
 
-    return torch._C._cuda_getCurrentRawStream(index)
+    _current_stream = torch._C._cuda_getCurrentRawStream
+    return _current_stream(index)
 
 
 def _torch_stream(stream: int | None, index: int):
@@ -308,10 +324,11 @@ def _torch_stream(stream: int | None, index: int):
     return torch.cuda.ExternalStream(stream, device=index)
 
 
-def _use_on(tensor, stream: int | None) -> None:
-    """Tells torch's allocator that memory it gave for the current stream is used
-    on another one."""
-    tensor.record_stream(_torch_stream(stream, tensor.device.index))
+def _on_stream(index: int, stream: int | None):
+    """Context in which a stream is torch's current one."""
+    import torch
+
+    return torch.cuda.stream(_torch_stream(stream, index))
 
 
 def _order_behind(tensor, index: int, stream: int) -> bool:

@@ -66,3 +66,38 @@ def test_a_result_is_read_behind_its_call(torch, sizes, take, how):
             with torch.cuda.stream(reader):
                 r = lst.norm(stream=side if on is side else None)
                 near(take(r), want * 2.0 ** k, 4 * U, "norm")
+
+
+# ---- memory of calls on other streams -------------------------------------------------
+@pytest.mark.parametrize("call", ["norm", "clip"])
+@pytest.mark.parametrize("how", ["another stream", "the default stream beside a side stream"])
+@pytest.mark.parametrize("sizes", [[3000, 33], [2_000_003, 70_001]], ids=["small", "large"])
+def test_a_call_takes_no_memory_that_another_stream_still_uses(torch, sizes, how, call):
+    """Blocks that were given back on the current stream, where kernels that use
+    them are still queued, are not what a call on another stream writes to."""
+    tensors = make(torch, sizes, seed=2)
+    want = norm64(tensors)
+    side = torch.cuda.Stream()
+    with GradientList(tensors) as lst, \
+            GradientList([torch.empty_like(t) for t in tensors]) as out:
+        on = side if how == "another stream" else torch.cuda.default_stream()
+        current = torch.cuda.default_stream() if how == "another stream" else side
+        elements = [128, 256, 512, 1024, 4096, 16384]  # f32: blocks of results and workspaces
+        with torch.cuda.stream(current):
+            warm = [torch.empty(n, device="cuda") for n in elements for _ in range(8)]
+            del warm
+            torch.cuda.synchronize()
+            for _ in range(3):
+                blocks = [torch.full((n,), 3.0, device="cuda") for n in elements for _ in range(8)]
+                kept = torch.empty(len(blocks), device="cuda")
+                torch.cuda._sleep(BUSY)
+                for k, b in enumerate(blocks):  # queued behind the sleep: reads, then writes
+                    kept[k] = b.sum() / b.numel()
+                    b.fill_(5.0)
+                del blocks, b
+                kw = dict(stream=side if on is side else None, per_tensor=True)
+                r = lst.norm(**kw) if call == "norm" else lst.clip(want / 2, out=out, **kw)
+                torch.cuda.synchronize()
+                near(r.read().norm, want, 4 * U, "norm")
+                near(float(r.tensor_max[0]), float(tensors[0].abs().max()), U, "largest")
+                assert bool((kept == 3.0).all())

@@ -2,6 +2,7 @@
 calls, waits and reads.  The library and torch's streams are stand-ins."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from types import SimpleNamespace
 
@@ -19,8 +20,15 @@ def log(monkeypatch):
     events = []
     now = SimpleNamespace(stream=CURRENT)
     monkeypatch.setattr(gradlist, "_current_stream", lambda index: now.stream)
-    monkeypatch.setattr(gradlist, "_use_on", lambda t, s: events.append(("use", s or 0)),
-                        raising=False)
+    monkeypatch.setattr(gradlist, "_use_on", lambda t, s: None, raising=False)
+
+    @contextlib.contextmanager
+    def on_stream(index, stream):
+        before, now.stream = now.stream, stream or 0
+        yield
+        now.stream = before
+
+    monkeypatch.setattr(gradlist, "_on_stream", on_stream, raising=False)
 
     def order(tensor, index, stream):
         events.append(("wait", now.stream, stream))
@@ -91,3 +99,14 @@ def test_results_of_the_current_stream_wait_for_nothing(log):
     r = a_list(log).norm()  # None is the legacy default stream, torch's stream 0
     r.read()
     assert not any(e[0] == "wait" for e in log.events)
+
+
+@pytest.mark.parametrize("work_bytes", [64, 1 << 20], ids=["small", "large"])
+@pytest.mark.parametrize("stream", [OTHER, None, CURRENT, 1])
+@pytest.mark.parametrize("call", ["norm", "clip"])
+def test_results_and_workspace_come_from_the_calls_stream(log, call, stream, work_bytes):
+    lst = a_list(log, work_bytes)
+    getattr(lst, call)(stream=stream)
+    on = 0 if stream in (None, 1) else stream
+    assert log.events == [("allocate", on)] * (1 if work_bytes == 64 else 2) + [("call", on)]
+    assert log.now.stream == CURRENT
