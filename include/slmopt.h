@@ -466,7 +466,11 @@ uint64_t slm_grad_list_elements(const slm_grad_list* list);
 uint64_t slm_grad_list_workspace_bytes(const slm_grad_list* list);
 /* Points the list at new addresses (same sizes, types and strides), in stream
  * order: for gradients that are allocated anew every step.  Calls enqueued
- * on other streams must be ordered against it by the caller. */
+ * on other streams must be ordered against it by the caller.  Captured calls
+ * read the addresses that are bound when they run: a replay works on those of
+ * the last bind ahead of it, captured or not, of any alignment.  What is checked
+ * on the host (shared elements, overlaps) goes by the last slm_grad_list_bind
+ * call; where replays change the addresses, that is the caller's to see to. */
 int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n, void* stream);
 
 /* The norm of the list.  result_device, and where they are not NULL

@@ -892,7 +892,7 @@ struct ClipState {
 // One unit of the clip, each element read and written by the same thread.
 // Contiguous on both sides: vectors start at the output's boundaries, and the
 // input is shifted where it lies off them.
-// kAligned: no tensor of either list lies off the boundaries.  kShift: whether the
+// kAligned: both units lie on the boundaries (kGradVector).  kShift: whether the
 // input can lie off them where the output is on them (not in place).
 template <uint32_t T, uint32_t O, bool kAligned, bool kShift>
 __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint32_t count,
@@ -1034,6 +1034,31 @@ __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
                     state);
 }
 
+// Unit i in any layout and type on either side, element by element.  The launch
+// chooses the form for vectors by the addresses that the host knows; a bind in a
+// replayed graph, or one behind a captured clip, may have brought others by the
+// time the kernel runs.  A call of its own, for the registers of that form's sake.
+__device__ __noinline__ void clip_elements(const GradUnit* units, const GradUnit* outs, uint32_t i,
+                                           float scale, float clip) {
+  const GradUnit u = load_unit<true>(units, i), o = load_unit<true>(outs, i);
+  const ClipFactor f(clip, scale);
+  const uint32_t from = u.flags & kGradTypeMask, to = o.flags & kGradTypeMask;
+#pragma unroll 1
+  for (uint32_t e = unit_thread(); e < u.count; e += kListThreads) {
+    const void* p = from == kGradF32 ? Rows<kGradF32>(u, e).p : Rows<kGradF16>(u, e).p;
+    void* q = to == kGradF32 ? Rows<kGradF32>(o, e).p : Rows<kGradF16>(o, e).p;
+    const float y = f(from == kGradF32    ? from_bits<kGradF32>(elem_bits<kGradF32>(p, 0))
+                      : from == kGradBf16 ? from_bits<kGradBf16>(elem_bits<kGradBf16>(p, 0))
+                                          : from_bits<kGradF16>(elem_bits<kGradF16>(p, 0)));
+    if (to == kGradF32)
+      store1<kGradF32>(q, 0, y);
+    else if (to == kGradBf16)
+      store1<kGradBf16>(q, 0, y);
+    else
+      store1<kGradF16>(q, 0, y);
+  }
+}
+
 // kOut: the output type (units written in another one are left to the launch for
 // theirs), or in place.  All nine pairs of types in one kernel would spill.
 constexpr uint32_t kOutSame = 3u;
@@ -1044,6 +1069,11 @@ __device__ __forceinline__ void clip_any(const GradListView& list, const GradLis
   const GradUnit u = load_unit<kRows != kNoRows>(list.units, i);
   const GradUnit o = kSame ? u : load_unit<kRows != kNoRows>(out.units, i);
   if (!kSame && (o.flags & kGradTypeMask) != kOut) return;
+  if (kRows == kRowVectors && !(u.flags & o.flags & kGradVector)) {
+    if (state.ready())
+      clip_elements(list.units, kSame ? list.units : out.units, i, scale, state.clip);
+    return;
+  }
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
       return clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows, kSame>(u, o, list, out, scale, state);

@@ -101,3 +101,102 @@ def test_a_call_takes_no_memory_that_another_stream_still_uses(torch, sizes, how
                 near(r.read().norm, want, 4 * U, "norm")
                 near(float(r.tensor_max[0]), float(tensors[0].abs().max()), U, "largest")
                 assert bool((kept == 3.0).all())
+
+
+# ---- clipped rows whose alignment changes ----------------------------------------------
+def rows_of(torch, kind, first, columns=256, rows=3000, seed=0, width=328):
+    """A column slice of a wider matrix; on vector boundaries when first % 8 == 0."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    wide = (1e-2 * torch.randn(rows, width, generator=gen, device="cuda")).to(getattr(torch, kind))
+    return wide, wide[:, first:first + columns]
+
+
+def half_step(torch, kind):
+    return {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[kind]
+
+
+def check_clipped(torch, got, before, factor):
+    """round(x * (clip / scale)): clip 5u (sum to f32 6u, its root 3u + 1u, quotient 1u), over the
+    scale 1u, product 1u: 7u, 7.5u are checked; and half a step of the output's type."""
+    for y, x in zip(got, before):
+        want = x.double() * factor
+        off = (y.double() - want).abs()
+        tol = (7.5 * U + half_step(torch, y.dtype)) * want.abs()
+        if y.dtype == torch.float16:
+            tol += 2.0 ** -25
+        assert bool((off <= tol).all()), float((off - tol).max())
+
+
+def outside_kept(torch, wide, keep, part):
+    """Nothing but the slice has changed."""
+    mask = torch.ones_like(wide, dtype=torch.bool)
+    at = part.storage_offset() - wide.storage_offset()
+    mask[:, at:at + part.shape[1]] = False
+    return bool((wide[mask] == keep[mask]).all())
+
+
+def captured(torch, call):
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=s):
+        r = call(torch.cuda.current_stream())
+    return g, r
+
+
+@pytest.mark.parametrize("scale", [1.0, 8.0])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "float16"])
+def test_a_captured_clip_in_place_follows_rows_off_the_boundaries(torch, kind, scale):
+    wides, parts = zip(*[rows_of(torch, kind, first, seed=first) for first in (64, 61, 8, 3)])
+    keeps = [w.clone() for w in wides]
+    total = norm64(parts[:1]) / scale
+    with GradientList([parts[0]]) as lst:
+        g, r = captured(torch, lambda s: lst.clip(total / 2, loss_scale=scale, stream=s))
+        for k in (1, 2, 3, 0):
+            lst.bind([parts[k]])
+            before = parts[k].clone()
+            found = norm64([before]) / scale
+            g.replay()
+            torch.cuda.synchronize()
+            near(r.read().norm, found, 4 * U, "norm")
+            check_clipped(torch, [parts[k]], [before], total / 2 / found / scale)
+            assert outside_kept(torch, wides[k], keeps[k], parts[k])
+
+
+@pytest.mark.parametrize("out", ["bfloat16", "float32", "float16", "contiguous"])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_a_captured_clip_into_rows_follows_both_lists(torch, kind, out):
+    ins = [rows_of(torch, kind, first, seed=first) for first in (64, 61)]
+    outs = [rows_of(torch, "float32" if out == "contiguous" else out, first, seed=9)
+            for first in (8, 5)]
+    keeps = [w.clone() for w, _ in outs]
+    targets = [p for _, p in outs]
+    if out == "contiguous":
+        room = torch.zeros(3000 * 256 + 8, device="cuda")
+        targets = [room[a:a + 3000 * 256].view(3000, 256) for a in (0, 1)]
+    with GradientList([ins[0][1]]) as lst, GradientList([targets[0]]) as to:
+        g, _ = captured(torch, lambda s: lst.clip(0.25, loss_scale=8.0, out=to, stream=s))
+        for i, o in ((1, 0), (0, 1), (1, 1), (0, 0)):
+            lst.bind([ins[i][1]])
+            to.bind([targets[o]])
+            g.replay()
+            torch.cuda.synchronize()
+            found = norm64([ins[i][1]]) / 8.0
+            check_clipped(torch, [targets[o]], [ins[i][1]], 0.25 / found / 8.0)
+            if out != "contiguous":
+                assert outside_kept(torch, outs[o][0], keeps[o], targets[o])
+
+
+def test_calls_behind_a_replayed_bind_work_on_its_addresses(torch):
+    wides, parts = zip(*[rows_of(torch, "bfloat16", first, seed=first) for first in (64, 61)])
+    keeps = [w.clone() for w in wides]
+    with GradientList([parts[0]]) as lst:
+        g, _ = captured(torch, lambda s: lst.bind([parts[1]], stream=s))
+        lst.bind([parts[0]])  # the host goes by this one
+        g.replay()
+        before = parts[1].clone()
+        r = lst.clip(1.0, loss_scale=2.0)
+        found = norm64([before]) / 2.0
+        near(r.read().norm, found, 4 * U, "norm")
+        check_clipped(torch, [parts[1]], [before], 1.0 / found / 2.0)
+        assert torch.equal(wides[0], keeps[0])
+        assert outside_kept(torch, wides[1], keeps[1], parts[1])
