@@ -699,11 +699,12 @@ __global__ void __launch_bounds__(kListThreads, kRows ? 5 : 8)
     list_norm_kernel(GradListView list, float scale, const DeviceScaler* scaler,
                      GradPartial* partials) {
   __shared__ UnitSlot slot;
-  const GradUnit u = load_unit<kRows>(list.units, blockIdx.x);
   // The kernels behind may start to read gradients once all blocks are here, so
-  // their producers must be done by then: wait first.
+  // their producers must be done by then: wait first.  A bind just ahead writes
+  // the unit's record, so that is read behind the wait too.
   pdl_wait();
   pdl_trigger();
+  const GradUnit u = load_unit<kRows>(list.units, blockIdx.x);
   unit_partial<kRows>(list, u, square_factor(scaler ? scaler->scale : scale), slot, 1u,
                       partials + blockIdx.x);
 }
@@ -1335,9 +1336,9 @@ __global__ void __launch_bounds__(kListThreads, 4)
                            int overwrite) {
   const uint32_t unit = blockIdx.x / blocks_per_unit;
   const uint32_t begin = (blockIdx.x - unit * blocks_per_unit) * kAccElems;
-  GradUnit u = load_unit<kRows>(list.units, unit);
-  pdl_wait();
+  pdl_wait();  // a bind just ahead writes the unit's record
   pdl_trigger();  // whoever starts early waits for this kernel before it reads
+  GradUnit u = load_unit<kRows>(list.units, unit);
   if (begin >= u.count) return;
   slice_unit<kRows>(u, begin, kAccElems);
   switch (u.flags & kGradTypeMask) {
@@ -1427,8 +1428,8 @@ __global__ void __launch_bounds__(kListThreads)
     list_accumulate_norm_kernel(GradListView list, float* acc, int overwrite, float scale,
                                 const DeviceScaler* scaler, GradPartial* partials) {
   __shared__ UnitSlot slot;
+  pdl_wait();  // a bind just ahead writes the unit's record
   const GradUnit u = load_unit<true>(list.units, blockIdx.x);
-  pdl_wait();
   const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
   const double sum = factor == 1.0f

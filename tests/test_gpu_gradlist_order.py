@@ -200,3 +200,29 @@ def test_calls_behind_a_replayed_bind_work_on_its_addresses(torch):
         check_clipped(torch, [parts[1]], [before], 1.0 / found / 2.0)
         assert torch.equal(wides[0], keeps[0])
         assert outside_kept(torch, wides[1], keeps[1], parts[1])
+
+
+# ---- calls right behind a bind -----------------------------------------------------------
+@pytest.mark.parametrize("sizes", [[3000, 33], [2_000_003, 70_001, 8192]], ids=["small", "large"])
+def test_calls_right_behind_a_bind_read_the_new_addresses(torch, sizes):
+    """No host synchronisation between binding and the calls, many times over."""
+    sets = [make(torch, sizes, seed=20 + k, std=1e-2 * 2.0 ** k) for k in range(4)]
+    wants = [norm64(s) for s in sets]
+    flats = [torch.cat([t.float() for t in s]) for s in sets]
+    n = sum(sizes)
+    opts = StepOptions(one_based_update=3, max_grad_norm=1e6)
+    with GradientList(sets[0]) as lst, B200Adamw(TensorTable.from_sizes(sizes)) as opt:
+        room = -(-n // 4) * 4  # rows of the accumulators on 16-byte boundaries
+        acc = [a[:n] for a in torch.empty(4, room, device="cuda")]
+        for rep in range(20):
+            norms = []
+            for k in range(4):
+                lst.bind(sets[k])
+                norms.append(lst.norm())
+                lst.bind(sets[(k + 1) % 4])
+                lst.accumulate(acc[k], overwrite=True)
+                lst.bind(sets[(k + 2) % 4])
+                opt.norm_pass_accumulate(acc[k], lst, opts)
+            for k in range(4):
+                near(norms[k].read().norm, wants[k], 4 * U, "norm")
+                assert torch.equal(acc[k], flats[(k + 1) % 4] + flats[(k + 2) % 4])
