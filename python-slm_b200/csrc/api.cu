@@ -384,12 +384,13 @@ int enqueue_norm(slm_opt_handle* h, const void* dev_grads, int dtype, const slm_
                  "norm kernel");
 }
 
+// chained: behind a norm pass over dev_grads in the same call (see launch_adamw_update).
 int enqueue_update(slm_opt_handle* h, const void* dev_grads, int dtype,
-                   const slm_step_config* cfg, cudaStream_t s) {
+                   const slm_step_config* cfg, bool chained, cudaStream_t s) {
   const AdamwParams p = adamw_params(cfg);
   return h->cuda(launch_adamw_update(dtype, dev_grads, h->P, 0, h->master, h->m1, h->m2, h->w16,
                                      h->d_offsets, h->d_decay, h->d_tile_first, p, h->d_state,
-                                     h->grid_update[dtype == SLM_DTYPE_F32 ? 0 : 1], s),
+                                     h->grid_update[dtype == SLM_DTYPE_F32 ? 0 : 1], chained, s),
                  "update kernel");
 }
 
@@ -852,8 +853,10 @@ int slm_opt_update_pass(slm_opt_handle* h, const slm_step_config* cfg, void* str
   if (st) return st;
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = h->pass_list ? enqueue_list_update(h, h->pass_list, cfg, s)
-                    : enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, s);
+  // Not chained: the kernel ahead may be the caller's, or the accumulating norm
+  // pass, which writes the gradients that the update reads.
+  st = h->pass_list ? enqueue_list_update(h, h->pass_list, cfg, false, s)
+                    : enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, false, s);
   h->pass_grads = nullptr;
   release_pass_list(h);
   h->pending = true;
@@ -876,7 +879,7 @@ int run_step(slm_opt_handle* h, const void* grads, int dtype, int memory,
     if ((st = phase_begin(h, s))) return st;
     if ((st = enqueue_norm(h, dev, dtype, cfg, s))) return st;
     if ((st = phase_mark(h, s))) return st;
-    if ((st = enqueue_update(h, dev, dtype, cfg, s))) return st;
+    if ((st = enqueue_update(h, dev, dtype, cfg, true, s))) return st;
     if ((st = phase_mark(h, s))) return st;
   }
   phase_end(h);
@@ -1146,7 +1149,7 @@ int slm_opt_apply_update(slm_opt_handle* h, const float* grads_host, uint64_t n,
                   "AdamW received a learning rate that differs from the frozen schedule");
   cfg.learning_rate = learning_rate;
   cfg.one_based_update = uint32_t(one_based_update);
-  if ((st = enqueue_update(h, dev, SLM_DTYPE_F32, &cfg, s))) return st;
+  if ((st = enqueue_update(h, dev, SLM_DTYPE_F32, &cfg, false, s))) return st;
   if ((st = phase_mark(h, s))) return st;
   phase_end(h, kApplyUpdateCall);
   if ((st = read_state(h, s, &ds))) return st;

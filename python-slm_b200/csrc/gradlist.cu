@@ -15,8 +15,13 @@
 // bound by and measured stands at the kernel.  The kernels of one call are
 // chained by programmatic dependent launch: each lets the next one become
 // resident at once and the next one waits for its results (pdl_wait) after it
-// has issued what loads do not depend on them.  A kernel triggers only after its
-// own wait, so whatever has started early sees the gradients' producers finished.
+// has issued what loads do not depend on them.  The first kernel of a call waits
+// before it reads or writes anything that another call may have written, and
+// triggers only then, so what the kernels behind it in the call read ahead of
+// their own waits (gradients, state, unit records) was complete and visible
+// already.  Those behind it (finalize, decide) may therefore trigger at once;
+// whatever comes behind a call starts with a wait again, or is launched without
+// the attribute (the update pass).
 #include "step_device.cuh"
 
 #include <cuda_bf16.h>
@@ -1784,14 +1789,19 @@ cudaError_t launch_list_accumulate_norm(const GradListView& list, float* acc, in
 
 cudaError_t launch_list_update(const GradListView& list, float* master, float* moment,
                                float* variance, uint16_t* w16, const uint8_t* decay,
-                               const AdamwParams& p, DeviceStepState* st, cudaStream_t stream) {
+                               const AdamwParams& p, DeviceStepState* st, bool chained,
+                               cudaStream_t stream) {
   // One block more where a unit can start inside a vector of the state.
   const uint32_t per_unit = list.unit_elems / kUpdateElems + (list.off_vectors ? 1u : 0u);
   const uint64_t blocks = uint64_t(list.n_units) * per_unit;
   if (blocks == 0 || blocks > 0x7fffffffull) return cudaErrorInvalidValue;
-  return launch_chained(list.rows ? list_update_kernel<true> : list_update_kernel<false>,
-                        uint32_t(blocks), kUpdateBlock, 0, stream, list, per_unit,
-                        list.keep > 0u, master, moment, variance, w16, decay, p, st);
+  const auto kernel = list.rows ? list_update_kernel<true> : list_update_kernel<false>;
+  if (chained)
+    return launch_chained(kernel, uint32_t(blocks), kUpdateBlock, 0, stream, list, per_unit,
+                          list.keep > 0u, master, moment, variance, w16, decay, p, st);
+  kernel<<<uint32_t(blocks), kUpdateBlock, 0, stream>>>(list, per_unit, list.keep > 0u, master,
+                                                        moment, variance, w16, decay, p, st);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_list_bind(GradTensor* tensors, GradUnit* units, uint32_t n_units,

@@ -308,9 +308,9 @@ int slmopt::enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list,
 }
 
 int slmopt::enqueue_list_update(slm_opt_handle* h, const slm_grad_list* list,
-                                const slm_step_config* cfg, cudaStream_t s) {
+                                const slm_step_config* cfg, bool chained, cudaStream_t s) {
   return h->cuda(launch_list_update(list->view(), h->master, h->m1, h->m2, h->w16, h->d_decay,
-                                    adamw_params(cfg), h->d_state, s),
+                                    adamw_params(cfg), h->d_state, chained, s),
                  "list update kernel");
 }
 
@@ -488,7 +488,7 @@ int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_st
   if ((st = phase_begin(h, s))) return st;
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
   if ((st = phase_mark(h, s))) return st;
-  if ((st = enqueue_list_update(h, list, cfg, s))) return st;
+  if ((st = enqueue_list_update(h, list, cfg, true, s))) return st;
   if ((st = phase_mark(h, s))) return st;
   phase_end(h);
   return finish_step(h, out, s);

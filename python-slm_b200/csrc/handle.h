@@ -201,7 +201,7 @@ uint64_t list_partial_bytes(const std::vector<uint64_t>& offsets);
 int enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
                       cudaStream_t s);
 int enqueue_list_update(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
-                        cudaStream_t s);
+                        bool chained, cudaStream_t s);
 // Lets go of the list of a norm pass whose update pass has been enqueued, or never will be.
 void release_pass_list(slm_opt_handle* h);
 void fill_result(const DeviceStepState& s, slm_step_result* out);

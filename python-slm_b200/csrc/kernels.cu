@@ -2328,17 +2328,19 @@ cudaError_t launch_update_typed(const void* grads, uint64_t n, uint64_t elem_bas
                                 float* moment, float* variance, uint16_t* w16,
                                 const uint64_t* offsets, const uint8_t* decay,
                                 const uint32_t* tile_first, const AdamwParams& p,
-                                DeviceStepState* st, int grid, cudaStream_t stream) {
+                                DeviceStepState* st, int grid, bool chained,
+                                cudaStream_t stream) {
   const GT* g = static_cast<const GT*>(grads);
   if constexpr (kUpdateBulk) {
     const uint64_t tiles = n / kBulkTile;
     const unsigned blocks =
         static_cast<unsigned>(tiles == 0 ? 1 : (uint64_t(grid) < tiles ? uint64_t(grid) : tiles));
     // Programmatic stream serialization: may start before the kernel ahead of
-    // it on the stream completes, if that kernel triggers (the norm pass does).
+    // it on the stream completes, if that kernel triggers (the norm pass does),
+    // and without its writes being visible if it does not.
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = chained ? 1 : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(kBulkThreads);
@@ -2397,13 +2399,15 @@ cudaError_t launch_adamw_update(int dtype, const void* grads, uint64_t n, uint64
                                 float* master, float* moment, float* variance, uint16_t* w16,
                                 const uint64_t* offsets, const uint8_t* decay,
                                 const uint32_t* tile_first_tensor, const AdamwParams& p,
-                                DeviceStepState* st, int grid, cudaStream_t stream) {
+                                DeviceStepState* st, int grid, bool chained,
+                                cudaStream_t stream) {
   if (n == 0) return cudaSuccess;
   if (dtype == 0)
     return launch_update_typed<float>(grads, n, elem_base, master, moment, variance, w16, offsets,
-                                      decay, tile_first_tensor, p, st, grid, stream);
+                                      decay, tile_first_tensor, p, st, grid, chained, stream);
   return launch_update_typed<uint16_t>(grads, n, elem_base, master, moment, variance, w16,
-                                       offsets, decay, tile_first_tensor, p, st, grid, stream);
+                                       offsets, decay, tile_first_tensor, p, st, grid, chained,
+                                       stream);
 }
 
 cudaError_t launch_zero1_reduce(int dtype, const void* recv, uint32_t ranks, uint64_t stride,

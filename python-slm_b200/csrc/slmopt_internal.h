@@ -148,12 +148,16 @@ cudaError_t launch_norm_partials(int dtype, const void* grads, uint64_t n, uint6
                                  cudaStream_t stream);
 // Updates local elements [0, n); element i is global flat index elem_base + i
 // (the tensor table holds global offsets).  grads/master/moment/variance/w16
-// are all indexed by the local i.
+// are all indexed by the local i.  chained: the launch may start while the kernel
+// ahead on the stream runs and reads g / master / m / v before it has waited for it.
+// Only for a kernel of the same call ahead that was itself launched behind, or has
+// waited for, whatever wrote them.
 cudaError_t launch_adamw_update(int dtype, const void* grads, uint64_t n, uint64_t elem_base,
                                 float* master, float* moment, float* variance, uint16_t* w16,
                                 const uint64_t* offsets, const uint8_t* decay,
                                 const uint32_t* tile_first_tensor, const AdamwParams& p,
-                                DeviceStepState* st, int grid, cudaStream_t stream);
+                                DeviceStepState* st, int grid, bool chained,
+                                cudaStream_t stream);
 // ZeRO-1 over peer memory (see zero1.cu): two kernels per step.
 // The reduce: gradient barrier, rank-ordered sum of this shard's slices of
 // every rank's gradient buffer (bulk copies over NVLink), unscale, chunk
@@ -357,10 +361,11 @@ cudaError_t launch_list_decide(const GradListView& list, const GradPartial* part
                                DeviceScaler* scaler, DeviceStepState* st,
                                const FinalizeParams& fp, cudaStream_t stream);
 // AdamW over the flat state with the gradients read from the list's tensors,
-// which are the state's tensors in order.
+// which are the state's tensors in order.  chained: see launch_adamw_update.
 cudaError_t launch_list_update(const GradListView& list, float* master, float* moment,
                                float* variance, uint16_t* w16, const uint8_t* decay,
-                               const AdamwParams& p, DeviceStepState* st, cudaStream_t stream);
+                               const AdamwParams& p, DeviceStepState* st, bool chained,
+                               cudaStream_t stream);
 // Points the list's tables at new first elements (tensors [begin, begin + n)).
 constexpr uint32_t kGradBindBatch = 256;
 struct GradBind {

@@ -417,7 +417,7 @@ int zero1_step(slm_opt_handle* h, const void* grads, int dtype, int memory,
   if ((st = h->cuda(launch_adamw_update(SLM_DTYPE_F32, h->d_gsum, h->shard_len, h->shard_begin,
                                         h->master, h->m1, h->m2, h->w16 + h->shard_begin,
                                         h->d_offsets, h->d_decay, h->d_tile_first, p, h->d_state,
-                                        h->grid_update[0], s),
+                                        h->grid_update[0], true, s),
                     "update kernel")))
     return st;
   if ((st = phase_mark(h, s))) return st;

@@ -226,3 +226,47 @@ def test_calls_right_behind_a_bind_read_the_new_addresses(torch, sizes):
             for k in range(4):
                 near(norms[k].read().norm, wants[k], 4 * U, "norm")
                 assert torch.equal(acc[k], flats[(k + 1) % 4] + flats[(k + 2) % 4])
+
+
+# ---- the update pass behind other work -----------------------------------------------------
+def load(torch, opt, seed):
+    st = synth.optimizer_state(opt.P, seed)
+    opt.load_state(st["master"], st["moment"], st["variance"], st["bf16"])
+
+
+def same_bits(torch, a, b):
+    return all(torch.equal(a[k].view(torch.int16), b[k].view(torch.int16)) for k in a)
+
+
+@pytest.mark.parametrize("form", ["list", "flat", "list accumulated", "flat accumulated"])
+def test_an_update_pass_sees_what_ran_ahead_of_it(torch, form):
+    """The norm pass, work on the state, then the update pass, without waiting in
+    between, give what they give with a wait after each."""
+    sizes = [2_000_003, 70_001, 8192]
+    tensors = make(torch, sizes, ("float32",), seed=30)
+    flat = torch.cat(tensors)
+    opts = StepOptions(one_based_update=3, max_grad_norm=0.5)
+    with B200Adamw(TensorTable.from_sizes(sizes)) as opt, GradientList(tensors) as lst:
+        grads = lst if form.startswith("list") else flat
+        start = torch.randn(opt.P, device="cuda")
+        got = []
+        for wait in (True, False, False, False):
+            pause = torch.cuda.synchronize if wait else lambda: None
+            load(torch, opt, 31)
+            state, acc = opt.state_tensors(), start.clone()
+            torch.cuda.synchronize()
+            for k in range(8):
+                if "accumulated" in form:
+                    opt.norm_pass_accumulate(acc, grads, opts)
+                else:
+                    opt.norm_pass(grads, opts)
+                pause()
+                if k % 2:
+                    state["moment"].mul_(0.5)
+                    state["variance"].add_(1e-6)
+                    pause()
+                opt.update_pass(opts)
+                pause()
+            assert opt.read_result().skipped == 0
+            got.append({k: v.clone() for k, v in state.items()})
+        assert all(same_bits(torch, got[0], g) for g in got[1:])
