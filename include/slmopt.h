@@ -245,7 +245,9 @@ const char* slm_opt_phase_name(const slm_opt_handle* h, uint32_t phase);
  *   slm_opt_update_pass -- AdamW + bf16 weight write over the gradients the
  *                          norm pass saw (CanonicalAdamw's loop, trainer.rs:274-293).
  * The gradient buffer must stay valid until the update pass has run; cfg must
- * be the same for both.  Lets a caller overlap the norm pass with other work
+ * be the same for both.  A whole step or slm_opt_apply_update in between ends the
+ * norm pass: the update pass then has none ahead of it and is refused
+ * (SLM_ERR_INVALID_ARGUMENT).  Lets a caller overlap the norm pass with other work
  * or time each pass with its own events. */
 int slm_opt_norm_pass(slm_opt_handle* h, const void* grads, int dtype, int memory,
                       const slm_step_config* cfg, void* stream);

@@ -286,7 +286,8 @@ void release(slm_grad_list* list) {
 
 }  // namespace
 
-void slmopt::release_pass_list(slm_opt_handle* h) {
+void slmopt::drop_norm_pass(slm_opt_handle* h) {
+  h->pass_grads = nullptr;
   if (h->pass_list) release(h->pass_list);
   h->pass_list = nullptr;
 }
@@ -485,6 +486,7 @@ int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_st
   if (h->broken) return h->err(SLM_ERR_INTERNAL, "a previous step failed inside a kernel");
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  drop_norm_pass(h);
   if ((st = phase_begin(h, s))) return st;
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
   if ((st = phase_mark(h, s))) return st;
@@ -502,8 +504,7 @@ int slm_opt_norm_pass_list(slm_opt_handle* h, slm_grad_list* list,
   if (st) return st;
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  h->pass_grads = nullptr;
-  release_pass_list(h);
+  drop_norm_pass(h);
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
   list->holders.fetch_add(1);
   h->pass_list = list;
@@ -527,8 +528,7 @@ int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
       return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  h->pass_grads = nullptr;
-  release_pass_list(h);
+  drop_norm_pass(h);
   const FinalizeParams fp = finalize_params(h, cfg);
   GradPartial* part = static_cast<GradPartial*>(h->d_list_partials);
   const GradListView v = list->view();

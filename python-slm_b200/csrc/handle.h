@@ -202,8 +202,9 @@ int enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list, const slm_st
                       cudaStream_t s);
 int enqueue_list_update(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
                         bool chained, cudaStream_t s);
-// Lets go of the list of a norm pass whose update pass has been enqueued, or never will be.
-void release_pass_list(slm_opt_handle* h);
+// Forgets a norm pass whose update pass has been enqueued, or never will be (its
+// decision is about to be overwritten), and lets go of its list.
+void drop_norm_pass(slm_opt_handle* h);
 void fill_result(const DeviceStepState& s, slm_step_result* out);
 // ZeRO-1 pieces (zero1.cu).
 int zero1_step(slm_opt_handle* h, const void* grads, int dtype, int memory,

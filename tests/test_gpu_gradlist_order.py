@@ -11,6 +11,7 @@ import math
 import pytest
 
 from slmopt import B200Adamw, GradientList, SlmError, StepOptions, TensorTable, _lib, synth
+from slmopt.trainer import canonical_learning_rate
 
 pytestmark = pytest.mark.gpu
 
@@ -270,3 +271,36 @@ def test_an_update_pass_sees_what_ran_ahead_of_it(torch, form):
             assert opt.read_result().skipped == 0
             got.append({k: v.clone() for k, v in state.items()})
         assert all(same_bits(torch, got[0], g) for g in got[1:])
+
+
+@pytest.mark.parametrize("ahead", ["list", "flat", "list accumulated"])
+@pytest.mark.parametrize("between", ["list step", "flat step", "uploaded step", "apply_update"])
+def test_a_step_between_the_passes_ends_the_norm_pass(torch, ahead, between):
+    """The decision of the norm pass is gone, so there is nothing to update by."""
+    sizes = [70_001, 8192]
+    tensors, other = (make(torch, sizes, ("float32",), seed=40 + k, std=1e-6) for k in (0, 1))
+    opts = StepOptions(one_based_update=3)
+    with B200Adamw(TensorTable.from_sizes(sizes)) as opt, GradientList(tensors) as lst, \
+            GradientList(other) as lst2:
+        load(torch, opt, 41)
+        if ahead == "list":
+            opt.norm_pass(lst, opts)
+        elif ahead == "flat":
+            keep = opt.norm_pass(torch.cat(tensors), opts)
+        else:
+            opt.norm_pass_accumulate(torch.zeros(opt.P, device="cuda"), lst, opts)
+        flat = torch.cat(other)
+        if between == "list step":
+            opt.step(lst2, opts)
+        elif between == "flat step":
+            opt.step(flat, opts)
+        elif between == "uploaded step":
+            opt.step_uploaded(opt.upload(flat.cpu().pin_memory()), opts)
+        else:
+            opt.apply_normalized_clipped_gradients(flat.cpu().numpy(), canonical_learning_rate(1), 1)
+        with pytest.raises(SlmError) as e:
+            opt.update_pass(opts)
+        assert e.value.status == _lib.SLM_ERR_INVALID_ARGUMENT
+        opt.norm_pass(lst, opts)  # and with one of its own it goes on
+        opt.update_pass(opts)
+        assert opt.read_result().skipped == 0
