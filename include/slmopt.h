@@ -419,7 +419,8 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * never written.
  *
  * A list borrows its tensors: they must stay allocated while the list or work
- * enqueued with it uses them.  It is immutable but for slm_grad_list_bind, so
+ * enqueued with it uses them.  A captured call reads the list's tables at every
+ * replay, so the list must outlive the graph.  It is immutable but for slm_grad_list_bind, so
  * calls with it may run at the same time on several streams or in several
  * captured graphs, each with its own workspace and results; all but
  * slm_grad_list_create and _destroy may be captured.  Elements are counted in
@@ -461,7 +462,9 @@ typedef struct slm_list_norm {
  * (SLM_ERR_INVALID_ARGUMENT otherwise). */
 int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
                          slm_grad_list** out);
-/* Waits for the device's outstanding work, then frees the list. */
+/* Waits for the device's outstanding work, then frees the list.  Graphs that have
+ * captured a call with the list must not be replayed any more.  While a stream
+ * is captured it fails (SLM_ERR_CUDA; the list lives on). */
 int slm_grad_list_destroy(slm_grad_list* list);
 uint64_t slm_grad_list_elements(const slm_grad_list* list);
 /* Bytes of device workspace of one norm or clip call. */

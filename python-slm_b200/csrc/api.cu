@@ -601,7 +601,8 @@ int slm_opt_destroy(slm_opt_handle* h) {
   // Work this handle enqueued (on any stream) finishes before its buffers and
   // peer mappings go away; every kernel's waits are bounded.
   cudaDeviceSynchronize();
-  drop_norm_pass(h);
+  drop_norm_pass(h, nullptr);
+  free_parked_lists(h);
   zero1_release(h);
   if (h->timer.created)
     for (cudaEvent_t e : h->timer.ev) cudaEventDestroy(e);
@@ -754,7 +755,7 @@ int slm_opt_norm_pass(slm_opt_handle* h, const void* grads, int dtype, int memor
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const void* dev = nullptr;
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   if ((st = stage_grads(h, grads, dtype, memory, s, &dev))) return st;
   if ((st = enqueue_norm(h, dev, dtype, cfg, s))) return st;
   h->pass_grads = dev;
@@ -829,7 +830,7 @@ int slm_opt_norm_pass_accumulate(slm_opt_handle* h, float* acc_device, const voi
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const void* dev = nullptr;
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   if ((st = stage_grads(h, micro, dtype, memory, s, &dev))) return st;
   const FinalizeParams fp = finalize_params(h, cfg);
   if ((st = h->cuda(launch_accumulate_norm(dtype, acc_device, dev, h->P, overwrite, h->n_chunks,
@@ -855,7 +856,7 @@ int slm_opt_update_pass(slm_opt_handle* h, const slm_step_config* cfg, void* str
   // pass, which writes the gradients that the update reads.
   st = h->pass_list ? enqueue_list_update(h, h->pass_list, cfg, false, s)
                     : enqueue_update(h, h->pass_grads, h->pass_dtype, cfg, false, s);
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   h->pending = true;
   h->pending_stream = s;
   return st;
@@ -868,7 +869,7 @@ namespace {
 int run_step(slm_opt_handle* h, const void* grads, int dtype, int memory,
              const slm_step_config* cfg, slm_step_result* out, cudaStream_t s) {
   int st = SLM_OK;
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   if (h->sharded()) {
     if ((st = zero1_step(h, grads, dtype, memory, cfg, s))) return st;
   } else {
@@ -1085,7 +1086,7 @@ int slm_opt_apply_update(slm_opt_handle* h, const float* grads_host, uint64_t n,
   DeviceGuard guard(h->device);
   cudaStream_t s = nullptr;
   const void* dev = nullptr;
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   int st = phase_begin(h, s);
   if (st) return st;
   // Re-verification first (trainer.rs:250-260), with the reference's own

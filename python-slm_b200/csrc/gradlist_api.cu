@@ -273,12 +273,9 @@ int check_step_list(slm_opt_handle* h, const slm_grad_list* list) {
   return SLM_OK;
 }
 
-void release(slm_grad_list* list) {
-  if (list->holders.fetch_sub(1) != 1) return;
+// A list without holders, whose work has been waited for.
+void free_list(slm_grad_list* list) {
   DeviceGuard guard(list->device);
-  // Work enqueued with the list (on any stream) has read its tables, and its
-  // tensors, when this returns.
-  if (list->d_tensors || list->d_units) cudaDeviceSynchronize();
   cudaFree(list->d_tensors);
   cudaFree(list->d_units);
   delete list;
@@ -286,10 +283,27 @@ void release(slm_grad_list* list) {
 
 }  // namespace
 
-void slmopt::drop_norm_pass(slm_opt_handle* h) {
+void slmopt::drop_norm_pass(slm_opt_handle* h, cudaStream_t s) {
   h->pass_grads = nullptr;
-  if (h->pass_list) release(h->pass_list);
+  slm_grad_list* list = h->pass_list;
   h->pass_list = nullptr;
+  if (!list || list->holders.fetch_sub(1) != 1) return;
+  // Its owner has destroyed it, which waited for what was enqueued then: an update
+  // pass on s at most has come since.  A graph that captures that goes on to read
+  // the list, which is kept as long as the handle.
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &status) != cudaSuccess) cudaGetLastError();
+  if (status != cudaStreamCaptureStatusNone) {
+    h->parked_lists.push_back(list);
+    return;
+  }
+  cudaStreamSynchronize(s);
+  free_list(list);
+}
+
+void slmopt::free_parked_lists(slm_opt_handle* h) {
+  for (slm_grad_list* list : h->parked_lists) free_list(list);
+  h->parked_lists.clear();
 }
 
 uint64_t slmopt::list_partial_bytes(const std::vector<uint64_t>& offsets) {
@@ -357,10 +371,19 @@ int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
 
 int slm_grad_list_destroy(slm_grad_list* list) {
   if (!list) return SLM_OK;
+  if (!list->d_tensors && !list->d_units) {  // never came to a device
+    delete list;
+    return SLM_OK;
+  }
   DeviceGuard guard(list->device);
-  // The tensors are the caller's again when this returns.
-  if (list->d_tensors || list->d_units) cudaDeviceSynchronize();
-  release(list);
+  // Work enqueued with the list (on any stream) has read its tables, and its
+  // tensors, when this returns; an update pass to come may still read them.
+  const cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaErrorStreamCaptureUnsupported) {
+    cudaGetLastError();
+    return fail(SLM_ERR_CUDA, "a gradient list cannot be destroyed while a stream is captured");
+  }
+  if (list->holders.fetch_sub(1) == 1) free_list(list);
   return SLM_OK;
 }
 
@@ -486,7 +509,7 @@ int slm_opt_step_list(slm_opt_handle* h, const slm_grad_list* list, const slm_st
   if (h->broken) return h->err(SLM_ERR_INTERNAL, "a previous step failed inside a kernel");
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   if ((st = phase_begin(h, s))) return st;
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
   if ((st = phase_mark(h, s))) return st;
@@ -504,7 +527,7 @@ int slm_opt_norm_pass_list(slm_opt_handle* h, slm_grad_list* list,
   if (st) return st;
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   if ((st = enqueue_list_norm(h, list, cfg, s))) return st;
   list->holders.fetch_add(1);
   h->pass_list = list;
@@ -528,7 +551,7 @@ int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
       return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  drop_norm_pass(h);
+  drop_norm_pass(h, s);
   const FinalizeParams fp = finalize_params(h, cfg);
   GradPartial* part = static_cast<GradPartial*>(h->d_list_partials);
   const GradListView v = list->view();

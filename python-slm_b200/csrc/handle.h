@@ -110,6 +110,7 @@ struct slm_opt_handle {
   const void* pass_grads = nullptr;
   int pass_dtype = -1;
   slm_grad_list* pass_list = nullptr;  // of slm_opt_norm_pass_list, held until then
+  std::vector<slm_grad_list*> parked_lists;  // destroyed by their owners, read by a captured update
   cudaStream_t pending_stream = nullptr;
   bool pending = false;
   std::string last_error = "no error";
@@ -203,8 +204,10 @@ int enqueue_list_norm(slm_opt_handle* h, const slm_grad_list* list, const slm_st
 int enqueue_list_update(slm_opt_handle* h, const slm_grad_list* list, const slm_step_config* cfg,
                         bool chained, cudaStream_t s);
 // Forgets a norm pass whose update pass has been enqueued, or never will be (its
-// decision is about to be overwritten), and lets go of its list.
-void drop_norm_pass(slm_opt_handle* h);
+// decision is about to be overwritten by work on s), and lets go of its list.
+void drop_norm_pass(slm_opt_handle* h, cudaStream_t s);
+// The lists that drop_norm_pass has kept for captured update passes.
+void free_parked_lists(slm_opt_handle* h);
 void fill_result(const DeviceStepState& s, slm_step_result* out);
 // ZeRO-1 pieces (zero1.cu).
 int zero1_step(slm_opt_handle* h, const void* grads, int dtype, int memory,

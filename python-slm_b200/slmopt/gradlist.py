@@ -136,12 +136,14 @@ class GradientList:
     addresses of the last construction or ``bind``: after ``tensor.data = ...``
     or a new backward pass that allocated new gradients, ``bind`` the new ones.
     Work runs on ``stream`` (None: the legacy default stream) and is ordered
-    with the rest of that stream; the tensors must be ready there."""
+    with the rest of that stream; the tensors must be ready there.  A list must
+    outlive the CUDA graphs that have captured its calls."""
 
     def __init__(self, tensors):
         import torch
 
         self.lib = _lib.load()
+        _free_retired()
         self._h = None
         self.tensors = tuple(tensors)
         if not self.tensors:
@@ -195,9 +197,13 @@ class GradientList:
         return len(self.tensors)
 
     def close(self) -> None:
-        if getattr(self, "_h", None):
-            self.lib.slm_grad_list_destroy(self._h)
-            self._h = None
+        """Frees the list, once the device's outstanding work is done.  During a
+        capture, which cannot be waited in (a list may be collected at any time),
+        that is left to the next creation or ``close`` of a list outside."""
+        h, self._h = getattr(self, "_h", None), None
+        if h:
+            _RETIRED.append((self.lib, h, self.tensors))
+        _free_retired()
 
     def __del__(self):
         try:
@@ -296,6 +302,23 @@ class GradientList:
         _lib.check(self.lib.slm_grad_list_accumulate(self.handle, acc.data_ptr(), self.elements,
                                                      1 if overwrite else 0,
                                                      _stream_handle(stream)))
+
+
+_RETIRED: list = []  # (library, handle, tensors) of closed lists that are still to be freed
+
+
+def _free_retired() -> None:
+    while _RETIRED and not _capturing():
+        lib, handle, tensors = _RETIRED.pop()
+        if lib.slm_grad_list_destroy(handle):
+            _RETIRED.append((lib, handle, tensors))  # another thread captures
+            return
+
+
+def _capturing() -> bool:
+    import torch
+
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 def _stream_handle(stream) -> int | None:

@@ -304,3 +304,49 @@ def test_a_step_between_the_passes_ends_the_norm_pass(torch, ahead, between):
         opt.norm_pass(lst, opts)  # and with one of its own it goes on
         opt.update_pass(opts)
         assert opt.read_result().skipped == 0
+
+
+# ---- lists that end around captures --------------------------------------------------------
+def test_a_list_collected_inside_a_capture_does_not_break_it(torch):
+    tensors, other = make(torch, [70_001, 33], seed=50), make(torch, [5000], seed=51)
+    with GradientList(tensors) as lst:
+        spare = [GradientList(other), GradientList(other)]
+
+        def call(s):
+            r = lst.norm(stream=s)
+            spare.pop()          # collected
+            spare[0].close()
+            lst.norm(stream=s)
+            return r
+
+        g, r = captured(torch, call)
+        g.replay()
+        torch.cuda.synchronize()
+        near(r.read().norm, norm64(tensors), 4 * U, "norm")
+        GradientList(other).close()
+        near(lst.norm().read().norm, norm64(tensors), 4 * U, "norm")
+
+
+def test_a_captured_update_pass_keeps_a_list_that_is_closed_ahead_of_it(torch):
+    sizes = [70_001, 8192]
+    tensors = make(torch, sizes, seed=52)
+    opts = StepOptions(one_based_update=4, max_grad_norm=1e6)
+    with B200Adamw(TensorTable.from_sizes(sizes)) as opt, GradientList(tensors) as lst:
+        load(torch, opt, 53)
+        opt.norm_pass(lst, opts)
+        for _ in range(3):  # update passes by one decision, as the replays below
+            opt.update_pass(opts)
+            want = {k: v.clone() for k, v in opt.state_tensors().items()}
+            opt.norm_pass(lst, opts)
+        load(torch, opt, 53)
+        gone = GradientList(tensors)
+        opt.norm_pass(gone, opts)
+        gone.close()
+        g, _ = captured(torch, lambda s: opt.update_pass(opts, stream=s))
+        for _ in range(3):
+            g.replay()
+        torch.cuda.synchronize()
+        assert same_bits(torch, want, opt.state_tensors())
+        opt.norm_pass(lst, opts)
+        opt.update_pass(opts)
+        assert opt.read_result().skipped == 0

@@ -110,3 +110,36 @@ def test_results_and_workspace_come_from_the_calls_stream(log, call, stream, wor
     on = 0 if stream in (None, 1) else stream
     assert log.events == [("allocate", on)] * (1 if work_bytes == 64 else 2) + [("call", on)]
     assert log.now.stream == CURRENT
+
+
+def test_a_list_closed_inside_a_capture_is_freed_after_it(log, monkeypatch):
+    freed, capturing, failing = [], [True], [0]
+
+    def destroy(h):
+        if failing[0]:
+            return 1
+        freed.append(h.value)
+        return 0
+
+    monkeypatch.setattr(gradlist, "_capturing", lambda: capturing[0], raising=False)
+    lists = []
+    for k in range(4):
+        lst = a_list(log)
+        lst._h = ctypes.c_void_p(10 + k)
+        lst.lib = SimpleNamespace(slm_grad_list_destroy=destroy)
+        lists.append(lst)
+    lists[0].close()
+    lists.pop(1).__del__()
+    assert freed == []
+    for call in (lists[0].norm, lists[0].clip, lambda: lists[0].handle):
+        with pytest.raises(ValueError):
+            call()
+    capturing[0] = False
+    lists[1].close()
+    assert sorted(freed) == [10, 11, 12]
+    failing[0] = 1  # another thread captures: the list is not lost
+    lists[2].close()
+    failing[0] = 0
+    lists[2].close()
+    lists[0].close()
+    assert sorted(freed) == [10, 11, 12, 13]
