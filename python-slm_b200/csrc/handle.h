@@ -30,18 +30,15 @@ inline uint32_t f32_bits(float v) {
 
 inline bool finite_f32(float v) { return std::isfinite(v); }
 
-// Restores the caller's current device on scope exit.
+// Restores the caller's current device on scope exit.  The device is set even where
+// its ordinal is current already: the caller's thread may be in a driver-API
+// context of its own on it, and the handle's memory is in the primary one.
 struct DeviceGuard {
   int prev = -1;
   bool ok = false;
   explicit DeviceGuard(int device) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev == device) {  // nothing to switch, nothing to restore
-      prev = -1;
-      ok = true;
-    } else {
-      ok = cudaSetDevice(device) == cudaSuccess;
-    }
+    ok = cudaSetDevice(device) == cudaSuccess;
   }
   ~DeviceGuard() {
     if (prev >= 0) cudaSetDevice(prev);

@@ -350,3 +350,36 @@ def test_a_captured_update_pass_keeps_a_list_that_is_closed_ahead_of_it(torch):
         opt.norm_pass(lst, opts)
         opt.update_pass(opts)
         assert opt.read_result().skipped == 0
+
+
+# ---- the caller's context --------------------------------------------------------------------
+@pytest.mark.parametrize("call", ["handle", "list"])
+def test_calls_from_a_context_of_the_callers_own_run_in_the_primary_one(torch, call):
+    """No kernel is launched here: copies of the loss scale, and the end of a list."""
+    import ctypes
+
+    cuda = ctypes.CDLL("libcuda.so.1")
+
+    def ok(status):
+        assert status == 0, status
+
+    with B200Adamw(TensorTable.from_sizes([100])) as opt, \
+            GradientList([torch.ones(100, device="cuda")]) as lst:
+        primary, own, now = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+        torch.cuda.synchronize()
+        ok(cuda.cuCtxGetCurrent(ctypes.byref(primary)))
+        ok(cuda.cuCtxCreate_v2(ctypes.byref(own), 0, 0))
+        try:
+            ok(cuda.cuCtxGetCurrent(ctypes.byref(now)))
+            assert now.value == own.value != primary.value
+            if call == "handle":
+                opt.set_loss_scale(512.0)
+                assert opt.loss_scale() == (512.0, 0)
+            else:
+                handle, lst._h = lst._h, None
+                assert lst.lib.slm_grad_list_destroy(handle) == _lib.SLM_OK
+            ok(cuda.cuCtxGetCurrent(ctypes.byref(now)))
+            assert now.value == primary.value
+        finally:
+            ok(cuda.cuCtxDestroy_v2(own))
+            ok(cuda.cuCtxSetCurrent(primary))
