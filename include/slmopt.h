@@ -434,9 +434,9 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  * squared.  The result does not depend on the device or the run, only on the
  * tensors' sizes.  It is within 3e-7 relative of the exact sum, as the flat
  * norm's is, but not the same bits (the tree restarts at every tensor).  The
- * values are squared as they are stored for loss scales from 1 to 2^20, else
- * times the power of two next to 1 / loss_scale; a square above 3e38 is
- * infinite and counts as a non-finite gradient, one below 1e-38 loses bits. */
+ * values are squared times the largest power of two not above 1 / loss_scale, so
+ * in the flat norm's range: an unscaled square above 3e38 is infinite and counts as a
+ * non-finite gradient, one below 1e-37 loses bits. */
 typedef struct slm_grad_view {
   const void* data;     /* device memory, aligned to the element */
   uint64_t rows, columns; /* at most 2^30 columns where rows have a pitch */

@@ -6,6 +6,7 @@ The norm's tolerance counts roundings (u = 2^-24): the sum of squares is within
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -356,8 +357,6 @@ def test_a_captured_update_pass_keeps_a_list_that_is_closed_ahead_of_it(torch):
 @pytest.mark.parametrize("call", ["handle", "list"])
 def test_calls_from_a_context_of_the_callers_own_run_in_the_primary_one(torch, call):
     """No kernel is launched here: copies of the loss scale, and the end of a list."""
-    import ctypes
-
     cuda = ctypes.CDLL("libcuda.so.1")
 
     def ok(status):
@@ -383,3 +382,51 @@ def test_calls_from_a_context_of_the_callers_own_run_in_the_primary_one(torch, c
         finally:
             ok(cuda.cuCtxDestroy_v2(own))
             ok(cuda.cuCtxSetCurrent(primary))
+
+
+# ---- gradients as large as the flat step takes them ------------------------------------------
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("accumulated", [False, True], ids=["step", "accumulated"])
+@pytest.mark.parametrize("scale", [1.0, 1.5, 1024.0, 37888.0, 65536.0, 2.0 ** 20, 3e6])
+def test_a_list_step_takes_large_gradients_as_the_flat_step(torch, scale, accumulated, kind):
+    # the unscaled values' squares are f32 (up to 1e38), the stored ones' are not
+    sizes = [4097, 33]
+    scale = ctypes.c_float(scale).value
+    tensors = make(torch, sizes, ("float32",), seed=60)
+    for t in tensors:
+        t.mul_(2.0 ** 20 * scale)
+    tensors[0][5], tensors[1][32] = 3e18 * scale, -7e18 * scale
+    tensors = [t.to(getattr(torch, kind)) for t in tensors]
+    want = norm64(tensors) / scale
+    opts = StepOptions(one_based_update=3, max_grad_norm=1.0, static_loss_scale=scale)
+    with B200Adamw(TensorTable.from_sizes(sizes)) as opt, GradientList(tensors) as lst:
+        load(torch, opt, 61)
+        for grads in (torch.cat(tensors), lst):
+            if accumulated:
+                opt.norm_pass_accumulate(torch.empty(opt.P, device="cuda"), grads, opts,
+                                         overwrite=True)
+                opt.update_pass(opts)
+                res = opt.read_result()
+            else:
+                res = opt.step(grads, opts)
+            assert (res.skipped, res.nonfinite) == (0, 0)
+            near(res.grad_norm, want, 4 * U, "norm")
+        r = lst.norm(loss_scale=scale, per_tensor=True).values.tolist()
+        near(r[0], want, 4 * U, "norm")
+        assert r[3] == 0.0
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -149, 2.0 ** -127, 2.0 ** -126, 1.7 * 2.0 ** -126, 0.5,
+                                   0.75, 1.0 - 2.0 ** -24, 1.0, 1.0 + 2.0 ** -23, 1.9, 2.0,
+                                   1.5 * 2.0 ** 125, 2.0 ** 126, 1.5 * 2.0 ** 126, 2.0 ** 127,
+                                   3.4e38])
+def test_the_norm_at_any_loss_scale(torch, scale):
+    """Unscaled values from 1 to 2, as far as the stored ones are normal numbers."""
+    scale = ctypes.c_float(scale).value
+    gen = torch.Generator("cuda").manual_seed(62)
+    x = (torch.rand(20_001, generator=gen, device="cuda", dtype=torch.float64) + 1.0)
+    x = (x * max(scale, 2.0 ** -126)).clamp(max=3.4e38).float()
+    with GradientList([x]) as lst:
+        r = lst.norm(loss_scale=scale, max_norm=3e38).values.tolist()
+    near(r[0], norm64([x]) / scale, 4 * U, "norm")
+    assert r[3] == 0.0
