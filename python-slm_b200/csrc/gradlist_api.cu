@@ -6,6 +6,7 @@
 #include <atomic>
 #include <exception>
 #include <new>
+#include <utility>
 
 using namespace slmopt;
 
@@ -16,6 +17,13 @@ struct Extent {
   uint32_t tensor;
 };
 
+// What depends on the tensors' addresses.
+struct Addresses {
+  std::vector<Extent> extents;  // non-empty tensors by address
+  bool overlapping = false;     // two tensors share an element
+  uint32_t off_runs = 0;        // see GradListView
+};
+
 uint32_t type_bytes(uint32_t type) { return type == kGradF32 ? 4u : 2u; }
 
 }  // namespace
@@ -24,10 +32,9 @@ struct slm_grad_list {
   int device = 0;
   std::vector<GradTensor> tensors;
   std::vector<uint64_t> rows;  // 1 for contiguous tensors
-  std::vector<Extent> extents;  // non-empty tensors by address
-  bool overlapping = false;     // two tensors share an element
-  uint32_t pitched = 0;         // whether any tensor is rows with a pitch
-  uint32_t off_runs = 0, off_vectors = 0, types = 0;  // see GradListView; bit per type of a tensor with elements
+  Addresses at;
+  uint32_t pitched = 0;  // whether any tensor is rows with a pitch
+  uint32_t off_vectors = 0, types = 0;  // see GradListView; bit per type of a tensor with elements
   uint64_t elements = 0;
   uint32_t unit_elems = kGradUnitMin;
   uint32_t n_units = 0;
@@ -39,7 +46,7 @@ struct slm_grad_list {
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        off_runs, off_vectors, types, cluster, sms, keep, elements};
+                        at.off_runs, off_vectors, types, cluster, sms, keep, elements};
   }
 };
 
@@ -75,26 +82,24 @@ bool share_elements(const GradTensor& a, const GradTensor& b) {
   return col < x.columns * sx || col + y.columns * sy > pitch;
 }
 
-// What depends on the tensors' addresses.
-void look_at_addresses(slm_grad_list* l) {
-  l->extents.clear();
-  l->off_runs = 0;
-  for (const GradTensor& t : l->tensors)
-    if (t.elements && !(t.flags & kGradVector)) l->off_runs = 1;
-  for (uint32_t k = 0; k < l->tensors.size(); ++k) {
-    const GradTensor& t = l->tensors[k];
-    if (t.elements)
-      l->extents.push_back(Extent{uintptr_t(t.ptr), uintptr_t(t.ptr) + span_bytes(t, l->rows[k]), k});
+Addresses look_at_addresses(const std::vector<GradTensor>& tensors,
+                            const std::vector<uint64_t>& rows) {
+  Addresses at;
+  for (uint32_t k = 0; k < tensors.size(); ++k) {
+    const GradTensor& t = tensors[k];
+    if (!t.elements) continue;
+    if (!(t.flags & kGradVector)) at.off_runs = 1;
+    at.extents.push_back(Extent{uintptr_t(t.ptr), uintptr_t(t.ptr) + span_bytes(t, rows[k]), k});
   }
-  std::sort(l->extents.begin(), l->extents.end(),
+  std::sort(at.extents.begin(), at.extents.end(),
             [](const Extent& a, const Extent& b) { return a.lo < b.lo; });
-  l->overlapping = false;
-  for (size_t i = 0; i < l->extents.size() && !l->overlapping; ++i)
-    for (size_t j = i + 1; j < l->extents.size() && l->extents[j].lo < l->extents[i].hi; ++j)
-      if (share_elements(l->tensors[l->extents[i].tensor], l->tensors[l->extents[j].tensor])) {
-        l->overlapping = true;
+  for (size_t i = 0; i < at.extents.size() && !at.overlapping; ++i)
+    for (size_t j = i + 1; j < at.extents.size() && at.extents[j].lo < at.extents[i].hi; ++j)
+      if (share_elements(tensors[at.extents[i].tensor], tensors[at.extents[j].tensor])) {
+        at.overlapping = true;
         break;
       }
+  return at;
 }
 
 // Device memory of the list's device, aligned to its element size.
@@ -242,11 +247,11 @@ int check_norm_call(const slm_grad_list* list, float loss_scale, float max_norm,
 // same tensor in the same layout and type, itself.
 bool collides(const slm_grad_list& list, const slm_grad_list& out) {
   size_t i = 0;
-  for (const Extent& o : out.extents) {
-    while (i < list.extents.size() && list.extents[i].hi <= o.lo) ++i;
-    for (size_t j = i; j < list.extents.size() && list.extents[j].lo < o.hi; ++j) {
-      if (list.extents[j].hi <= o.lo) continue;
-      const uint32_t a = list.extents[j].tensor, b = o.tensor;
+  for (const Extent& o : out.at.extents) {
+    while (i < list.at.extents.size() && list.at.extents[i].hi <= o.lo) ++i;
+    for (size_t j = i; j < list.at.extents.size() && list.at.extents[j].lo < o.hi; ++j) {
+      if (list.at.extents[j].hi <= o.lo) continue;
+      const uint32_t a = list.at.extents[j].tensor, b = o.tensor;
       const GradTensor &x = list.tensors[a], &y = out.tensors[b];
       if (a == b && x.ptr == y.ptr && x.flags == y.flags &&
           (!(x.flags & kGradPitched) || (x.row_stride == y.row_stride && x.columns == y.columns)))
@@ -353,7 +358,7 @@ int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
         st = check_pointer(l->tensors[k].ptr, l->tensors[k].flags & kGradTypeMask, device);
     if (!st) {
       l->device = device;
-      look_at_addresses(l);
+      l->at = look_at_addresses(l->tensors, l->rows);
       DeviceGuard guard(device);
       st = guard.ok ? upload_list(l) : fail(SLM_ERR_CUDA, "cudaSetDevice failed");
     }
@@ -401,14 +406,18 @@ int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n,
     if (list->tensors[k].elements)
       if (int st = check_pointer(data[k], list->tensors[k].flags & kGradTypeMask, list->device))
         return st;
+  // The list's own tables change only once the device's are going to.
+  std::vector<GradTensor> tensors;
+  Addresses at;
   try {
+    tensors = list->tensors;
     for (uint32_t k = 0; k < n; ++k) {
-      GradTensor& t = list->tensors[k];
+      GradTensor& t = tensors[k];
       t.ptr = data[k];
       t.flags = layout_flags(t.flags & kGradTypeMask, (t.flags & kGradPitched) != 0u, t.ptr,
                              t.columns, t.row_stride);
     }
-    look_at_addresses(list);
+    at = look_at_addresses(tensors, list->rows);
   } catch (const std::exception&) {
     return fail(SLM_ERR_OUT_OF_MEMORY, "host allocation failed");
   }
@@ -417,8 +426,8 @@ int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n,
     GradBind b;
     const uint32_t m = std::min(kGradBindBatch, n - begin);
     for (uint32_t i = 0; i < kGradBindBatch; ++i) {
-      b.ptr[i] = i < m ? list->tensors[begin + i].ptr : nullptr;
-      b.flags[i] = i < m ? list->tensors[begin + i].flags : 0u;
+      b.ptr[i] = i < m ? tensors[begin + i].ptr : nullptr;
+      b.flags[i] = i < m ? tensors[begin + i].flags : 0u;
     }
     if (int st = cuda_status(launch_list_bind(list->d_tensors, list->d_units, list->n_units,
                                               list->unit_elems, b, begin, m,
@@ -426,6 +435,8 @@ int slm_grad_list_bind(slm_grad_list* list, const void* const* data, uint32_t n,
                              "list bind kernel"))
       return st;
   }
+  list->tensors.swap(tensors);
+  std::swap(list->at, at);
   return SLM_OK;
 }
 
@@ -459,7 +470,7 @@ int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, floa
   const slm_grad_list* to = in_place ? list : out;
   if (to->device != list->device)
     return fail(SLM_ERR_INVALID_ARGUMENT, "the output list is on another device");
-  if (to->overlapping)
+  if (to->at.overlapping)
     return fail(SLM_ERR_INVALID_ARGUMENT,
                 "tensors of the list that is written share elements, which would be clipped twice");
   if (!in_place) {
@@ -491,7 +502,7 @@ int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint6
   if (reinterpret_cast<uintptr_t>(acc_device) % 16 != 0)
     return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator must be 16-byte aligned");
   const uintptr_t lo = reinterpret_cast<uintptr_t>(acc_device), hi = lo + n * sizeof(float);
-  for (const Extent& x : list->extents)
+  for (const Extent& x : list->at.extents)
     if (x.lo < hi && lo < x.hi)
       return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
   DeviceGuard guard(list->device);
@@ -546,7 +557,7 @@ int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
   if (reinterpret_cast<uintptr_t>(acc_device) % 16 != 0)
     return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator must be 16-byte aligned");
   const uintptr_t lo = reinterpret_cast<uintptr_t>(acc_device), hi = lo + h->P * sizeof(float);
-  for (const Extent& x : list->extents)
+  for (const Extent& x : list->at.extents)
     if (x.lo < hi && lo < x.hi)
       return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
   DeviceGuard guard(h->device);

@@ -430,3 +430,30 @@ def test_the_norm_at_any_loss_scale(torch, scale):
         r = lst.norm(loss_scale=scale, max_norm=3e38).values.tolist()
     near(r[0], norm64([x]) / scale, 4 * U, "norm")
     assert r[3] == 0.0
+
+
+# ---- binds that fail -----------------------------------------------------------------------
+def test_a_bind_that_fails_leaves_the_list_as_it_was(torch):
+    """The launch is refused because a stream that the default stream waits for is
+    being captured: an error from the runtime, nothing runs."""
+    n = 4096
+    old, new = torch.full((n,), 2.0, device="cuda"), torch.full((n,), 3.0, device="cuda")
+    runtime = ctypes.CDLL("libcudart.so.12")
+    blocking, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    with GradientList([old]) as lst:
+        torch.cuda.synchronize()
+        assert runtime.cudaStreamCreate(ctypes.byref(blocking)) == 0
+        assert runtime.cudaStreamBeginCapture(blocking, 2) == 0  # relaxed
+        with pytest.raises(SlmError) as e:
+            lst.bind([new])
+        assert e.value.status == _lib.SLM_ERR_CUDA
+        runtime.cudaStreamEndCapture(blocking, ctypes.byref(graph))  # invalidated
+        runtime.cudaGetLastError()
+        assert runtime.cudaStreamDestroy(blocking) == 0
+        assert lst.tensors == (old,)
+        near(lst.norm().read().norm, 2.0 * math.sqrt(n), 4 * U, "norm")
+        lst.accumulate(new)  # not one of the list's tensors
+        torch.cuda.synchronize()
+        assert bool((new == 5.0).all()) and bool((old == 2.0).all())
+        lst.bind([new])
+        near(lst.norm().read().norm, 5.0 * math.sqrt(n), 4 * U, "norm")
