@@ -6,6 +6,7 @@
 #include <atomic>
 #include <exception>
 #include <new>
+#include <numeric>
 #include <utility>
 
 using namespace slmopt;
@@ -67,19 +68,22 @@ uint32_t layout_flags(uint32_t type, bool pitched, const void* ptr, uint64_t col
   return f;
 }
 
-// Whether two tensors whose extents overlap share an element.  Rows of one pitch
-// are compared column by column; other pairs count as sharing.
+// Whether two tensors whose extents overlap share an element.  In rows as far
+// apart as the two pitches allow (their greatest common divisor; a contiguous tensor
+// is one row and goes with any pitch) they do not when their columns differ;
+// other pairs count as sharing.
 bool share_elements(const GradTensor& a, const GradTensor& b) {
   const bool ordered = uintptr_t(a.ptr) <= uintptr_t(b.ptr);
   const GradTensor &x = ordered ? a : b, &y = ordered ? b : a;
   const uint64_t sx = type_bytes(x.flags & kGradTypeMask), sy = type_bytes(y.flags & kGradTypeMask);
-  if (!(x.flags & kGradPitched) || !(y.flags & kGradPitched) ||
-      x.row_stride * sx != y.row_stride * sy)
-    return true;
-  const uint64_t pitch = x.row_stride * sx;
+  const bool px = x.flags & kGradPitched, py = y.flags & kGradPitched;
+  const uint64_t pitch = std::gcd(px ? x.row_stride * sx : 0u, py ? y.row_stride * sy : 0u);
+  const uint64_t wide_x = (px ? x.columns : x.elements) * sx;  // of a row
+  const uint64_t wide_y = (py ? y.columns : y.elements) * sy;
+  if (pitch == 0u) return true;
   const uint64_t delta = uintptr_t(y.ptr) - uintptr_t(x.ptr);
   const uint64_t col = delta % pitch;  // y's first column within x's rows
-  return col < x.columns * sx || col + y.columns * sy > pitch;
+  return col < wide_x || col + wide_y > pitch;
 }
 
 Addresses look_at_addresses(const std::vector<GradTensor>& tensors,
@@ -259,6 +263,18 @@ bool collides(const slm_grad_list& list, const slm_grad_list& out) {
       if (share_elements(x, y)) return true;
     }
   }
+  return false;
+}
+
+// Whether one of n contiguous f32 values lies on an element of `list`.
+bool collides(const slm_grad_list& list, const float* values, uint64_t n) {
+  GradTensor run{};
+  run.ptr = values;
+  run.elements = n;
+  run.flags = kGradF32;
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(values), hi = lo + n * sizeof(float);
+  for (const Extent& x : list.at.extents)
+    if (x.lo < hi && lo < x.hi && share_elements(list.tensors[x.tensor], run)) return true;
   return false;
 }
 
@@ -501,10 +517,8 @@ int slm_grad_list_accumulate(const slm_grad_list* list, float* acc_device, uint6
     return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator needs one value per list element");
   if (reinterpret_cast<uintptr_t>(acc_device) % 16 != 0)
     return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator must be 16-byte aligned");
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(acc_device), hi = lo + n * sizeof(float);
-  for (const Extent& x : list->at.extents)
-    if (x.lo < hi && lo < x.hi)
-      return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
+  if (collides(*list, acc_device, n))
+    return fail(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
   DeviceGuard guard(list->device);
   return cuda_status(launch_list_accumulate(list->view(), acc_device, overwrite,
                                             static_cast<cudaStream_t>(stream)),
@@ -556,10 +570,8 @@ int slm_opt_norm_pass_accumulate_list(slm_opt_handle* h, float* acc_device,
   if (st) return st;
   if (reinterpret_cast<uintptr_t>(acc_device) % 16 != 0)
     return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator must be 16-byte aligned");
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(acc_device), hi = lo + h->P * sizeof(float);
-  for (const Extent& x : list->at.extents)
-    if (x.lo < hi && lo < x.hi)
-      return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
+  if (collides(*list, acc_device, h->P))
+    return h->err(SLM_ERR_INVALID_ARGUMENT, "the accumulator overlaps a gradient tensor");
   DeviceGuard guard(h->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   drop_norm_pass(h, s);

@@ -457,3 +457,42 @@ def test_a_bind_that_fails_leaves_the_list_as_it_was(torch):
         assert bool((new == 5.0).all()) and bool((old == 2.0).all())
         lst.bind([new])
         near(lst.norm().read().norm, 5.0 * math.sqrt(n), 4 * U, "norm")
+
+
+# ---- tensors between the rows of others ----------------------------------------------------
+def test_tensors_between_the_rows_of_others_are_no_overlap(torch):
+    w = torch.randn(64, 96, device="cuda")
+    keep = w.clone()
+    apart = [
+        ([w[:, :40], w[5, 40:96]], None),                       # a run in one gap
+        ([w[:, 32:64], w[0, :32], w[63, 64:]], None),           # ahead of, behind the rows
+        ([w[::2, :40], w[:, 40:50], w[1::2, :40]], None),       # rows of two pitches
+        ([w[:, :8], w[:4, 8:]], [w[:, :8], w[:4, 8:]]),
+        ([w[:, :8]], [w[3, 40:40 + 8 * 5].new_empty(64, 8)]),
+    ]
+    for tensors, targets in apart:
+        before = [t.clone() for t in tensors]
+        found = norm64(before)
+        with GradientList(tensors) as lst:
+            to = GradientList(targets) if targets else None
+            lst.clip(found / 2, out=to)
+            check_clipped(torch, targets or tensors, before, 0.5)
+            if to:
+                to.close()
+        inside = torch.zeros_like(w, dtype=torch.bool)
+        for t in tensors:
+            at = t.storage_offset()
+            inside.view(-1).as_strided(t.shape, t.stride(), at).fill_(True)
+        assert bool((w[~inside] == keep[~inside]).all())
+        w.copy_(keep)
+    with GradientList([w[:2, :4]]) as lst:  # an accumulator in the gap
+        lst.accumulate(w[0, 8:16], overwrite=True)
+        assert torch.equal(w[0, 8:16], w[:2, :4].reshape(-1))
+    together = [[w[:, :40], w[5, 39:96]], [w[:, :40], w.view(-1)[5 * 96 + 50:6 * 96 + 1]],
+                [w[::2, :40], w[:, 39:50]], [w[:, 32:64], w[0, :33]], [w[0], w[0, 5:6]],
+                [w[:, :40], w[2:4].view(-1)]]
+    for tensors in together:
+        with GradientList(tensors) as lst, pytest.raises(SlmError):
+            lst.clip(1.0)
+    with GradientList([w[:2, :4]]) as lst, pytest.raises(SlmError):
+        lst.accumulate(w.view(-1)[92:100])
