@@ -302,6 +302,8 @@ class B200Adamw:
         """acc (device f32[P]) += micro (device f32 or bf16 [P], or a
         GradientList), or acc = micro."""
         if isinstance(micro, GradientList):
+            if micro.elements != self.P:
+                raise ValueError(f"expected {self.P} elements")
             micro.accumulate(acc, overwrite, stream)
             return
         ptr, dt, mem, n, keep = _grad_pointer(micro)

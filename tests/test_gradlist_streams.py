@@ -9,7 +9,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from slmopt import GradientList, gradlist
+from slmopt import B200Adamw, GradientList, gradlist
 
 CURRENT, OTHER = 5, 7  # stream handles
 
@@ -143,3 +143,19 @@ def test_a_list_closed_inside_a_capture_is_freed_after_it(log, monkeypatch):
     lists[2].close()
     lists[0].close()
     assert sorted(freed) == [10, 11, 12, 13]
+
+
+@pytest.mark.parametrize("parameters", [4, 5, 6])
+def test_a_handle_accumulates_lists_of_its_size_alone(log, parameters):
+    opt = B200Adamw.__new__(B200Adamw)
+    opt.P, opt._h = parameters, None
+    lst = a_list(log)  # of 5 elements
+    lst.lib.slm_grad_list_accumulate = lambda h, acc, n, overwrite, s: log.events.append(n) or 0
+    acc = torch.zeros(5)
+    if parameters == 5:
+        opt.accumulate(acc, lst)
+        assert log.events == [5]
+        return
+    with pytest.raises(ValueError):
+        opt.accumulate(acc, lst)
+    assert log.events == []
