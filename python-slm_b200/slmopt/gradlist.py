@@ -161,6 +161,7 @@ class GradientList:
         _lib.check(self.lib.slm_grad_list_create(views, len(self.tensors), self.device.index,
                                                  ctypes.byref(h)))
         self._h = h
+        self._streams: set = set()  # where the bound tensors are in use
         self.elements = int(self.lib.slm_grad_list_elements(h))
         self._work_bytes = int(self.lib.slm_grad_list_workspace_bytes(h))
         # What every call needs, looked up once.
@@ -224,7 +225,9 @@ class GradientList:
         return self._h
 
     def bind(self, tensors, stream=None) -> None:
-        """Take other tensors of the same types, sizes and strides, in order."""
+        """Take other tensors of the same types, sizes and strides, in order.  The
+        old ones are let go; torch's allocator learns which streams calls of the
+        list have used them on."""
         tensors = tuple(tensors)
         if len(tensors) != len(self._shapes) or \
                 not all(self._is(t, shape) for t, shape in zip(tensors, self._shapes)):
@@ -232,7 +235,12 @@ class GradientList:
         ptrs = (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
         _lib.check(self.lib.slm_grad_list_bind(self.handle, ptrs, len(tensors),
                                                _stream_handle(stream)))
-        self.tensors = tensors
+        old, self.tensors = self.tensors, tensors
+        self._streams.discard(_current_stream(self._index))  # ordered as it is
+        while self._streams:
+            on = _torch_stream(self._streams.pop(), self._index)
+            for t in old:
+                t.record_stream(on)
 
     def norm(self, loss_scale: float = 1.0, max_norm: float = 1.0, kind: str = "l2",
              per_tensor: bool = False, stream=None) -> GradientNorm:
@@ -262,6 +270,9 @@ class GradientList:
         small = self._work_bytes <= _SHARED_BYTES
         s = None if stream is None else _stream_handle(stream)
         on = s or 0
+        self._streams.add(on)
+        if out is not None:
+            out._streams.add(on)
         if _current_stream(self._index) != on:
             with _on_stream(self._index, s):
                 buffer, work = self._room(head, small)
@@ -299,9 +310,15 @@ class GradientList:
                 acc.numel() != self.elements:
             raise ValueError("acc must be a contiguous f32 tensor on the list's device with one "
                              "value per element")
+        s = self._use(stream)
         _lib.check(self.lib.slm_grad_list_accumulate(self.handle, acc.data_ptr(), self.elements,
-                                                     1 if overwrite else 0,
-                                                     _stream_handle(stream)))
+                                                     1 if overwrite else 0, s))
+
+    def _use(self, stream) -> int | None:
+        """The handle of a stream that a call of the list runs on."""
+        s = _stream_handle(stream)
+        self._streams.add(s or 0)
+        return s
 
 
 _RETIRED: list = []  # (library, handle, tensors) of closed lists that are still to be freed

@@ -496,3 +496,42 @@ def test_tensors_between_the_rows_of_others_are_no_overlap(torch):
             lst.clip(1.0)
     with GradientList([w[:2, :4]]) as lst, pytest.raises(SlmError):
         lst.accumulate(w.view(-1)[92:100])
+
+
+# ---- tensors that a bind lets go -----------------------------------------------------------
+@pytest.mark.parametrize("call", ["norm", "clip", "accumulate", "step"])
+def test_tensors_let_go_by_a_bind_are_not_given_out_too_soon(torch, call):
+    sizes = [2_000_003, 70_001]
+    keep = make(torch, sizes, ("float32",), seed=70)
+    new = make(torch, sizes, ("float32",), seed=71)
+    want = norm64(keep)
+    side = torch.cuda.Stream()
+    acc = torch.zeros(sum(sizes), device="cuda")
+    opts = StepOptions(one_based_update=3, max_grad_norm=1e6)
+    out = [torch.empty_like(t) for t in keep]
+    with GradientList(new) as lst, GradientList(out) as to, \
+            B200Adamw(TensorTable.from_sizes(sizes)) as opt:
+        load(torch, opt, 72)
+        for _ in range(3):
+            lst.bind([t.clone() for t in keep])
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(BUSY)
+            if call == "norm":
+                r = lst.norm(stream=side)
+            elif call == "clip":
+                r = lst.clip(want / 2, out=to, stream=side)
+            elif call == "accumulate":
+                lst.accumulate(acc, overwrite=True, stream=side)
+            else:
+                opt.step(lst, opts, stream=side, wait=False)
+            lst.bind(new, stream=side)
+            junk = [torch.full((n,), 100.0, device="cuda") for n in sizes for _ in range(4)]
+            torch.cuda.synchronize()
+            del junk
+            if call in ("norm", "clip"):
+                near(r.read().norm, want, 4 * U, "norm")
+            elif call == "accumulate":
+                assert torch.equal(acc, torch.cat(keep))
+            else:
+                near(opt.read_result().grad_norm, want, 4 * U, "norm")

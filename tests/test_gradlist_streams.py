@@ -44,6 +44,7 @@ def a_list(log, work_bytes=64):
     lst._h = ctypes.c_void_p(1)
     lst.tensors = (torch.ones(3), torch.ones(2))
     lst.device, lst._index = torch.device("cpu"), 0
+    lst._streams = set()
     lst.elements, lst._work_bytes, lst._f32 = 5, work_bytes, torch.float32
 
     def empty(n, dtype, device):
@@ -159,3 +160,55 @@ def test_a_handle_accumulates_lists_of_its_size_alone(log, parameters):
     with pytest.raises(ValueError):
         opt.accumulate(acc, lst)
     assert log.events == []
+
+
+def test_tensors_let_go_by_a_bind_stay_until_their_streams_are_done(log, monkeypatch):
+    monkeypatch.setattr(gradlist, "_torch_stream", lambda stream, index: stream or 0)
+
+    class Tensor:
+        def __init__(self, name):
+            self.name = name
+
+        def data_ptr(self):
+            return 4096
+
+        def record_stream(self, stream):
+            log.events.append((self.name, stream))
+
+    lst, out = a_list(log), a_list(log)
+    for one in (lst, out):
+        one._is = lambda t, shape: True
+        one._shapes = [None, None]
+        one.lib.slm_grad_list_bind = lambda h, ptrs, n, s: 0
+        one.lib.slm_grad_list_accumulate = lambda h, acc, n, overwrite, s: 0
+        one.bind([Tensor("a"), Tensor("b")])
+
+    def released(which):
+        log.events.clear()
+        which.bind([Tensor("a"), Tensor("b")])
+        return sorted(log.events)
+
+    assert released(lst) == []
+    lst.norm(stream=CURRENT)  # torch's current stream: in order by itself
+    assert released(lst) == []
+    lst.norm(stream=OTHER)
+    lst.norm()
+    assert released(lst) == [("a", 0), ("a", OTHER), ("b", 0), ("b", OTHER)]
+    assert released(lst) == []
+    lst.clip(out=out, stream=OTHER)
+    assert released(out) == released(lst) == [("a", OTHER), ("b", OTHER)]
+    lst.accumulate(torch.zeros(5), stream=OTHER)
+    assert released(lst) == [("a", OTHER), ("b", OTHER)]
+
+    class Stub:
+        def __getattr__(self, name):
+            return lambda *args: 0
+
+    opt = B200Adamw.__new__(B200Adamw)
+    opt.P, opt.device, opt._h, opt.lib, opt._check = 5, 0, None, Stub(), lambda status: None
+    monkeypatch.setattr("slmopt.optimizer._check_accumulator", lambda acc, n, device: None)
+    for call in (lambda: opt.step(lst, stream=OTHER, wait=False),
+                 lambda: opt.norm_pass(lst, stream=OTHER),
+                 lambda: opt.norm_pass_accumulate(torch.zeros(5), lst, stream=OTHER)):
+        call()
+        assert released(lst) == [("a", OTHER), ("b", OTHER)]
