@@ -13,6 +13,7 @@ import pytest
 
 from slmopt import B200Adamw, GradientList, SlmError, StepOptions, TensorTable, _lib, synth
 from slmopt.trainer import canonical_learning_rate
+from test_gpu_gradlist import check_state
 
 pytestmark = pytest.mark.gpu
 
@@ -535,3 +536,98 @@ def test_tensors_let_go_by_a_bind_are_not_given_out_too_soon(torch, call):
                 assert torch.equal(acc, torch.cat(keep))
             else:
                 near(opt.read_result().grad_norm, want, 4 * U, "norm")
+
+
+# ---- rows on the boundaries, and units beyond the smallest -----------------------------------
+@pytest.mark.parametrize("rows", [3000, 40_000], ids=["0.8M", "10M"])
+@pytest.mark.parametrize("scale", [1.0, 8.0])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "float16"])
+def test_clip_of_rows_on_the_boundaries(torch, kind, scale, rows):
+    """Beyond the lists that one cluster takes: in place, into rows of every type and
+    into contiguous memory, with what lies beside the columns left as it was."""
+    wide, part = rows_of(torch, kind, 64, rows=rows, seed=80)
+    more = rows_of(torch, kind, 8, columns=64, rows=333, seed=81)[1]
+    keep = wide.clone()
+    before = [part.clone(), more.clone()]
+    total = norm64(before) / scale
+    for limit in (total / 3, total * 3):
+        factor = min(1.0, limit / total)
+        with GradientList([part, more]) as lst:
+            for out in ("bfloat16", "float32", "float16"):
+                room, target = rows_of(torch, out, 8, rows=rows, seed=82)
+                room_keep = room.clone()
+                flat = [torch.zeros(p.shape, device="cuda", dtype=room.dtype) for p in before]
+                for targets in ([target, flat[1]], flat):
+                    with GradientList(targets) as to:
+                        r = lst.clip(limit, loss_scale=scale, out=to, per_tensor=rows > 3000)
+                        near(r.read().norm, total, 4 * U, "norm")
+                    check_clipped(torch, targets, before, factor / scale)
+                assert outside_kept(torch, room, room_keep, target)
+            r = lst.clip(limit, loss_scale=scale)
+            near(r.read().norm, total, 4 * U, "norm")
+            check_clipped(torch, [part, more], before, factor / scale)
+            assert outside_kept(torch, wide, keep, part)
+            if scale == 1.0 and limit > total:
+                assert torch.equal(part, before[0])
+        part.copy_(before[0]), more.copy_(before[1])
+
+
+def test_units_beyond_the_smallest_over_mixed_layouts(torch):
+    """141M elements (units of 16,384) in contiguous memory off the boundaries, rows with
+    an odd pitch and rows on the boundaries: norm, clip, accumulate and the step."""
+    gen = torch.Generator("cuda").manual_seed(90)
+
+    def values(*shape, kind):
+        return (1e-3 * torch.randn(shape, generator=gen, device="cuda")).to(kind)
+
+    odd = values(30_000, 1003, kind=torch.float32)
+    even = values(50_000, 1032, kind=torch.bfloat16)
+    tensors = [values(60_000_002, kind=torch.bfloat16)[1:], odd[:, 1:1002], even[:, 8:],
+               values(777, kind=torch.float16)]
+    sizes = [t.numel() for t in tensors]
+    n = sum(sizes)
+    assert n // 8192 > 16384
+    keeps = [odd.clone(), even.clone()]
+    before = [t.clone() for t in tensors]
+    flat = torch.cat([t.reshape(-1).float() for t in tensors])
+    total = norm64(before)
+    limit = ctypes.c_float(total / 2).value
+    opts = StepOptions(learning_rate=3e-4, one_based_update=10, max_grad_norm=limit)
+    decay = [True, False, True, False]
+    with GradientList(tensors) as lst, B200Adamw(TensorTable.from_sizes(sizes, decay)) as opt:
+        r = lst.norm(per_tensor=True)
+        near(r.read().norm, total, 4 * U, "norm")
+        for k, t in enumerate(before):
+            near(float(r.tensor_norms[k]), norm64([t]), 4 * U, f"norm of tensor {k}")
+            assert float(r.tensor_max[k]) == float(t.abs().max())
+        acc = torch.randn(n, generator=gen, device="cuda")
+        old = acc.clone()
+        lst.accumulate(acc)
+        assert torch.equal(acc, old + flat)
+        lst.accumulate(acc, overwrite=True)
+        assert torch.equal(acc, flat)
+        opt.norm_pass_accumulate(acc, lst, opts)
+        assert torch.equal(acc, flat + flat)
+        near(opt.read_result().grad_norm, 2.0 * total, 4 * U, "accumulated norm")
+        del acc, old
+        state = opt.state_tensors()
+        state["master"].copy_(0.02 * torch.randn(n, generator=gen, device="cuda"))
+        state["moment"].copy_(1e-4 * torch.randn(n, generator=gen, device="cuda"))
+        state["variance"].copy_((1e-3 * torch.randn(n, generator=gen, device="cuda")).square())
+        state["bf16"].copy_(state["master"].bfloat16())
+        start = {k: v.clone() for k, v in state.items()}
+        res = opt.step(lst, opts)
+        near(res.grad_norm, total, 4 * U, "norm of the step")
+        check_state(torch, state, start, before, decay, opts, 1.0, 0.5)
+        del start
+        wide = torch.zeros(30_000, 1008, device="cuda")
+        targets = [torch.empty(sizes[0], device="cuda", dtype=torch.float16), wide[:, 3:1004],
+                   torch.empty(50_000, 1024, device="cuda"), torch.empty(777, device="cuda")]
+        with GradientList(targets) as to:
+            lst.clip(limit, out=to)
+            check_clipped(torch, targets, before, 0.5)
+        assert not bool(wide[:, :3].any()) and not bool(wide[:, 1004:].any())
+        lst.clip(limit)
+        check_clipped(torch, tensors, before, 0.5)
+        assert outside_kept(torch, odd, keeps[0], tensors[1])
+        assert outside_kept(torch, even, keeps[1], tensors[2])
