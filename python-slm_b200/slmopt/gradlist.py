@@ -65,22 +65,23 @@ class GradientNorm:
     is not finite (the clip scale is then 0.0) else 0.0; and with per_tensor each
     tensor's norm, then each tensor's largest magnitude."""
 
-    __slots__ = ("_buffer", "_count", "_tensors", "_index", "_stream", "_after")
+    __slots__ = ("_buffer", "_count", "_tensors", "_index", "_stream", "_event", "_after")
 
-    def __init__(self, buffer, count: int, tensors: int, index: int, stream: int):
+    def __init__(self, buffer, count: int, tensors: int, index: int, stream: int, event):
         # f32: the values, the f64 sum of squares, and scratch of the call.
         self._buffer = buffer
         self._count = count
         self._tensors = tensors
         self._index = index     # of the device
         self._stream = stream   # the call's
+        self._event = event     # behind the call, if that stream was not the current one
         self._after = stream    # the last one ordered behind it
 
     def _ready(self):
         """The buffer, with the current stream behind the call."""
         current = _current_stream(self._index)
         if current != self._stream and current != self._after and \
-                _order_behind(self._buffer, self._index, self._stream):
+                _order_behind(self._buffer, self._index, self._stream, self._event):
             self._after = current
         return self._buffer
 
@@ -161,7 +162,9 @@ class GradientList:
         _lib.check(self.lib.slm_grad_list_create(views, len(self.tensors), self.device.index,
                                                  ctypes.byref(h)))
         self._h = h
-        self._streams: set = set()  # where the bound tensors are in use
+        # Streams that the bound tensors are in use on: None, or for one that the
+        # caller owns (and may destroy) an event behind the last call there.
+        self._streams: dict = {}
         self.elements = int(self.lib.slm_grad_list_elements(h))
         self._work_bytes = int(self.lib.slm_grad_list_workspace_bytes(h))
         # What every call needs, looked up once.
@@ -236,9 +239,13 @@ class GradientList:
         _lib.check(self.lib.slm_grad_list_bind(self.handle, ptrs, len(tensors),
                                                _stream_handle(stream)))
         old, self.tensors = self.tensors, tensors
-        self._streams.discard(_current_stream(self._index))  # ordered as it is
+        self._streams.pop(_current_stream(self._index), None)  # ordered as it is
         while self._streams:
-            on = _torch_stream(self._streams.pop(), self._index)
+            handle, event = self._streams.popitem()
+            if event is not None:
+                event.synchronize()
+                continue
+            on = _torch_stream(handle, self._index)
             for t in old:
                 t.record_stream(on)
 
@@ -270,10 +277,8 @@ class GradientList:
         small = self._work_bytes <= _SHARED_BYTES
         s = None if stream is None else _stream_handle(stream)
         on = s or 0
-        self._streams.add(on)
-        if out is not None:
-            out._streams.add(on)
-        if _current_stream(self._index) != on:
+        away = _current_stream(self._index) != on
+        if away:
             with _on_stream(self._index, s):
                 buffer, work = self._room(head, small)
         elif small:
@@ -293,7 +298,15 @@ class GradientList:
                                  self._work_bytes, s)
         if st:
             _lib.check(st)
-        return GradientNorm(buffer, count, n, self._index, on)
+        event = None
+        if away:
+            event = _event_on(self._index, on)
+            self._streams[on] = event if isinstance(stream, int) else None
+        else:
+            self._streams[on] = None
+        if out is not None:
+            out._streams[on] = self._streams[on]
+        return GradientNorm(buffer, count, n, self._index, on, event)
 
     def _room(self, head: int, small: bool):
         """Results and workspace of a call, from the current stream's memory."""
@@ -310,15 +323,16 @@ class GradientList:
                 acc.numel() != self.elements:
             raise ValueError("acc must be a contiguous f32 tensor on the list's device with one "
                              "value per element")
-        s = self._use(stream)
         _lib.check(self.lib.slm_grad_list_accumulate(self.handle, acc.data_ptr(), self.elements,
-                                                     1 if overwrite else 0, s))
+                                                     1 if overwrite else 0,
+                                                     _stream_handle(stream)))
+        self._used(stream)
 
-    def _use(self, stream) -> int | None:
-        """The handle of a stream that a call of the list runs on."""
-        s = _stream_handle(stream)
-        self._streams.add(s or 0)
-        return s
+    def _used(self, stream) -> None:
+        """Takes note of the stream that a call with the list has run on."""
+        on = _stream_handle(stream) or 0
+        away = isinstance(stream, int) and _current_stream(self._index) != on
+        self._streams[on] = _event_on(self._index, on) if away else None
 
 
 _RETIRED: list = []  # (library, handle, tensors) of closed lists that are still to be freed
@@ -371,16 +385,32 @@ def _on_stream(index: int, stream: int | None):
     return torch.cuda.stream(_torch_stream(stream, index))
 
 
-def _order_behind(tensor, index: int, stream: int) -> bool:
-    """Lets torch's current stream wait for what is on ``stream``, where ``tensor``
-    was written, and tells the allocator that it is read there.  False inside a
-    capture, which cannot wait for work outside of it."""
+def _event_on(index: int, stream: int):
+    """An event behind what is on a stream now; None where that is being captured
+    (there is nothing to wait for outside of the graph)."""
+    import torch
+
+    with _on_stream(index, stream):
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        event = torch.cuda.Event()
+        event.record()
+    return event
+
+
+def _order_behind(tensor, index: int, stream: int, event) -> bool:
+    """Lets torch's current stream wait for the event, or without one for what is on
+    ``stream``, where ``tensor`` was written, and tells the allocator that it is read
+    there.  False inside a capture, which cannot wait for work outside of it."""
     import torch
 
     with torch.cuda.device(index):
         if torch.cuda.is_current_stream_capturing():
             return False
         current = torch.cuda.current_stream()
-        current.wait_stream(_torch_stream(stream, index))
+        if event is not None:
+            current.wait_event(event)
+        else:
+            current.wait_stream(_torch_stream(stream, index))
         tensor.record_stream(current)
     return True

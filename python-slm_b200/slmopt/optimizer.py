@@ -235,7 +235,8 @@ class B200Adamw:
             res = _lib.StepResult() if wait else None
             self._check(self.lib.slm_opt_step_list(self._h, grads.handle, ctypes.byref(cfg),
                                                    ctypes.byref(res) if wait else None,
-                                                   grads._use(stream)))
+                                                   _stream_handle(stream)))
+            grads._used(stream)
             return res
         ptr, dt, mem, n, keep = _grad_pointer(grads)
         if n != self.P:
@@ -288,7 +289,8 @@ class B200Adamw:
         if isinstance(grads, GradientList):
             cfg = (options or StepOptions()).to_c()
             self._check(self.lib.slm_opt_norm_pass_list(self._h, grads.handle, ctypes.byref(cfg),
-                                                        grads._use(stream)))
+                                                        _stream_handle(stream)))
+            grads._used(stream)
             return grads
         ptr, dt, mem, n, keep = _grad_pointer(grads)
         if n != self.P:
@@ -323,7 +325,8 @@ class B200Adamw:
             cfg = (options or StepOptions()).to_c()
             self._check(self.lib.slm_opt_norm_pass_accumulate_list(
                 self._h, acc.data_ptr(), micro.handle, 1 if overwrite else 0, ctypes.byref(cfg),
-                micro._use(stream)))
+                _stream_handle(stream)))
+            micro._used(stream)
             return micro
         ptr, dt, mem, n, keep = _grad_pointer(micro)
         if n != self.P or acc.numel() != self.P:

@@ -631,3 +631,23 @@ def test_units_beyond_the_smallest_over_mixed_layouts(torch):
         check_clipped(torch, tensors, before, 0.5)
         assert outside_kept(torch, odd, keeps[0], tensors[1])
         assert outside_kept(torch, even, keeps[1], tensors[2])
+
+
+def test_streams_of_the_callers_own_may_end_before_results_are_read(torch):
+    tensors, new = make(torch, [70_001, 33], seed=100), make(torch, [70_001, 33], seed=101)
+    want = norm64(tensors)
+    acc = torch.zeros(70_034, device="cuda")
+    runtime = ctypes.CDLL("libcudart.so.12")
+    with GradientList(tensors) as lst:
+        torch.cuda.synchronize()
+        for k in range(3):
+            own = ctypes.c_void_p()
+            assert runtime.cudaStreamCreateWithFlags(ctypes.byref(own), 1) == 0  # non-blocking
+            r = lst.norm(stream=own.value)
+            lst.accumulate(acc, overwrite=True, stream=own.value)
+            assert runtime.cudaStreamSynchronize(own) == 0
+            assert runtime.cudaStreamDestroy(own) == 0
+            near(r.read().norm, want, 4 * U, "norm")
+            del r
+            lst.bind(new)
+            lst.bind(tensors)

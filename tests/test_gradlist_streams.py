@@ -30,11 +30,19 @@ def log(monkeypatch):
 
     monkeypatch.setattr(gradlist, "_on_stream", on_stream, raising=False)
 
-    def order(tensor, index, stream):
+    def order(tensor, index, stream, event):
+        # Behind the call's event where there is one: its stream may be gone by then.
+        assert event is None or event.stream == stream
         events.append(("wait", now.stream, stream))
         return True
 
     monkeypatch.setattr(gradlist, "_order_behind", order, raising=False)
+
+    def event_on(index, stream):
+        return SimpleNamespace(stream=stream,
+                               synchronize=lambda: events.append(("synchronize", stream)))
+
+    monkeypatch.setattr(gradlist, "_event_on", event_on, raising=False)
     return SimpleNamespace(events=events, now=now)
 
 
@@ -44,7 +52,7 @@ def a_list(log, work_bytes=64):
     lst._h = ctypes.c_void_p(1)
     lst.tensors = (torch.ones(3), torch.ones(2))
     lst.device, lst._index = torch.device("cpu"), 0
-    lst._streams = set()
+    lst._streams = {}
     lst.elements, lst._work_bytes, lst._f32 = 5, work_bytes, torch.float32
 
     def empty(n, dtype, device):
@@ -175,6 +183,9 @@ def test_tensors_let_go_by_a_bind_stay_until_their_streams_are_done(log, monkeyp
         def record_stream(self, stream):
             log.events.append((self.name, stream))
 
+    class Stream:  # torch's, which outlive every use
+        cuda_stream = OTHER
+
     lst, out = a_list(log), a_list(log)
     for one in (lst, out):
         one._is = lambda t, shape: True
@@ -188,27 +199,29 @@ def test_tensors_let_go_by_a_bind_stay_until_their_streams_are_done(log, monkeyp
         which.bind([Tensor("a"), Tensor("b")])
         return sorted(log.events)
 
-    assert released(lst) == []
-    lst.norm(stream=CURRENT)  # torch's current stream: in order by itself
-    assert released(lst) == []
-    lst.norm(stream=OTHER)
-    lst.norm()
-    assert released(lst) == [("a", 0), ("a", OTHER), ("b", 0), ("b", OTHER)]
-    assert released(lst) == []
-    lst.clip(out=out, stream=OTHER)
-    assert released(out) == released(lst) == [("a", OTHER), ("b", OTHER)]
-    lst.accumulate(torch.zeros(5), stream=OTHER)
-    assert released(lst) == [("a", OTHER), ("b", OTHER)]
-
-    class Stub:
-        def __getattr__(self, name):
-            return lambda *args: 0
+    def stub(*args):
+        return 0
 
     opt = B200Adamw.__new__(B200Adamw)
-    opt.P, opt.device, opt._h, opt.lib, opt._check = 5, 0, None, Stub(), lambda status: None
+    opt.P, opt.device, opt._h, opt._check = 5, 0, None, lambda status: None
+    opt.lib = SimpleNamespace(slm_opt_step_list=stub, slm_opt_norm_pass_list=stub,
+                              slm_opt_norm_pass_accumulate_list=stub)
     monkeypatch.setattr("slmopt.optimizer._check_accumulator", lambda acc, n, device: None)
-    for call in (lambda: opt.step(lst, stream=OTHER, wait=False),
-                 lambda: opt.norm_pass(lst, stream=OTHER),
-                 lambda: opt.norm_pass_accumulate(torch.zeros(5), lst, stream=OTHER)):
+    assert released(lst) == []
+    for call in (lambda **on: lst.norm(**on), lambda **on: lst.clip(out=out, **on),
+                 lambda **on: lst.accumulate(torch.zeros(5), **on),
+                 lambda **on: opt.step(lst, wait=False, **on),
+                 lambda **on: opt.norm_pass(lst, **on),
+                 lambda **on: opt.norm_pass_accumulate(torch.zeros(5), lst, **on)):
+        call(stream=CURRENT)  # torch's current stream: in order by itself
+        assert released(lst) == released(out) == []
+        call(stream=Stream)
         call()
-        assert released(lst) == [("a", OTHER), ("b", OTHER)]
+        assert released(lst) == [("a", 0), ("a", OTHER), ("b", 0), ("b", OTHER)]
+        assert released(lst) == []
+        released(out)
+        call(stream=OTHER)  # a handle, whose stream its owner may destroy
+        assert released(lst) == [("synchronize", OTHER)]
+        released(out)
+    lst.clip(out=out, stream=Stream)
+    assert released(out) == released(lst) == [("a", OTHER), ("b", OTHER)]
