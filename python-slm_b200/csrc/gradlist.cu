@@ -1027,18 +1027,16 @@ __device__ __forceinline__ void clip_rows(const GradUnit& u, const GradUnit& o, 
 
 // kRows: kNoRows, kRowVectors, kAnyRows, each with the registers it needs.
 template <uint32_t T, uint32_t O, uint32_t kRows, bool kSame>
-__device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o,
-                                          const GradListView& list, const GradListView& out,
-                                          float scale, ClipState& state) {
+__device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o, float scale,
+                                          ClipState& state) {
   if (kRows == kRowVectors && ((u.flags | o.flags) & kGradPitched))
     clip_row_vectors<T, O, kSame>(u, o, scale, state);
   else if (kRows == kAnyRows && ((u.flags | o.flags) & kGradPitched))
     clip_rows<T, O>(u, o, scale, state);
   else
     clip_flat<T, O, kRows == kRowVectors, kRows != kRowVectors && !kSame>(
-        static_cast<const uint8_t*>(u.ptr),
-                    static_cast<uint8_t*>(const_cast<void*>(o.ptr)), u.count, scale,
-                    state);
+        static_cast<const uint8_t*>(u.ptr), static_cast<uint8_t*>(const_cast<void*>(o.ptr)),
+        u.count, scale, state);
 }
 
 // Unit i in any layout and type on either side, element by element.  The launch
@@ -1083,11 +1081,11 @@ __device__ __forceinline__ void clip_any(const GradListView& list, const GradLis
   }
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
-      return clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows, kSame>(u, o, list, out, scale, state);
+      return clip_unit<kGradF32, kSame ? kGradF32 : kOut, kRows, kSame>(u, o, scale, state);
     case kGradBf16:
-      return clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows, kSame>(u, o, list, out, scale, state);
+      return clip_unit<kGradBf16, kSame ? kGradBf16 : kOut, kRows, kSame>(u, o, scale, state);
     default:
-      return clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows, kSame>(u, o, list, out, scale, state);
+      return clip_unit<kGradF16, kSame ? kGradF16 : kOut, kRows, kSame>(u, o, scale, state);
   }
 }
 
@@ -1358,9 +1356,8 @@ __global__ void __launch_bounds__(kListThreads, 4)
 // its first element, the last one padded with +0.0) and adds the squares of the
 // sums.
 template <uint32_t T, bool kFactor>
-__device__ __forceinline__ double accumulate_squares(const GradUnit& u, const GradListView& list,
-                                                     float* acc, bool overwrite, float factor,
-                                                     uint32_t& top) {
+__device__ __forceinline__ double accumulate_squares(const GradUnit& u, float* acc, bool overwrite,
+                                                     float factor, uint32_t& top) {
   constexpr uint32_t kBatch = 2;
   Rows<T> src(u, unit_thread() * kVec);
   float* dst = acc + u.offset;
@@ -1415,16 +1412,15 @@ __device__ __forceinline__ double accumulate_squares(const GradUnit& u, const Gr
 }
 
 template <bool kFactor>
-__device__ __forceinline__ double accumulate_squares_any(const GradUnit& u,
-                                                         const GradListView& list, float* acc,
+__device__ __forceinline__ double accumulate_squares_any(const GradUnit& u, float* acc,
                                                          bool overwrite, float factor,
                                                          uint32_t& top) {
   switch (u.flags & kGradTypeMask) {
     case kGradF32:
-      return accumulate_squares<kGradF32, kFactor>(u, list, acc, overwrite, factor, top);
+      return accumulate_squares<kGradF32, kFactor>(u, acc, overwrite, factor, top);
     case kGradBf16:
-      return accumulate_squares<kGradBf16, kFactor>(u, list, acc, overwrite, factor, top);
-    default: return accumulate_squares<kGradF16, kFactor>(u, list, acc, overwrite, factor, top);
+      return accumulate_squares<kGradBf16, kFactor>(u, acc, overwrite, factor, top);
+    default: return accumulate_squares<kGradF16, kFactor>(u, acc, overwrite, factor, top);
   }
 }
 
@@ -1439,8 +1435,8 @@ __global__ void __launch_bounds__(kListThreads)
   const float factor = square_factor(scaler ? scaler->scale : scale);
   uint32_t top = 0u;
   const double sum = factor == 1.0f
-                   ? accumulate_squares_any<false>(u, list, acc, overwrite != 0, factor, top)
-                   : accumulate_squares_any<true>(u, list, acc, overwrite != 0, factor, top);
+                   ? accumulate_squares_any<false>(u, acc, overwrite != 0, factor, top)
+                   : accumulate_squares_any<true>(u, acc, overwrite != 0, factor, top);
   fold_unit(sum, top, slot, 1u, partials + blockIdx.x);
 }
 
@@ -1464,8 +1460,7 @@ constexpr uint32_t kUpdateElems = kUpdateBlock * kVec;
 
 // 8 gradients from element e of the unit on, and one.
 template <uint32_t T, bool kRows>
-__device__ __forceinline__ void update_grads(const GradUnit& u, const GradListView& list,
-                                             uint32_t e, float (&x)[8]) {
+__device__ __forceinline__ void update_grads(const GradUnit& u, uint32_t e, float (&x)[8]) {
   Raw<T> raw;
   if (kRows && (u.flags & kGradPitched)) {
     Rows<T>(u, e).load(raw, kVec, inside_unit(u, e), l2_first_out());
@@ -1481,8 +1476,7 @@ __device__ __forceinline__ void update_grads(const GradUnit& u, const GradListVi
   raw.unpack(x);
 }
 template <uint32_t T, bool kRows>
-__device__ __forceinline__ float update_grad(const GradUnit& u, const GradListView& list,
-                                             uint32_t e) {
+__device__ __forceinline__ float update_grad(const GradUnit& u, uint32_t e) {
   if (kRows && (u.flags & kGradPitched))
     return from_bits<T>(elem_bits<T>(Rows<T>(u, e).p, 0));
   return from_bits<T>(elem_bits<T>(u.ptr, e));
@@ -1524,11 +1518,11 @@ __global__ void __launch_bounds__(kUpdateBlock, 8)
     load_acc(mom + at, m);
     load_acc(var + at, v);
     if (type == kGradF32)
-      update_grads<kGradF32, kRows>(u, list, uint32_t(e), g);
+      update_grads<kGradF32, kRows>(u, uint32_t(e), g);
     else if (type == kGradBf16)
-      update_grads<kGradBf16, kRows>(u, list, uint32_t(e), g);
+      update_grads<kGradBf16, kRows>(u, uint32_t(e), g);
     else
-      update_grads<kGradF16, kRows>(u, list, uint32_t(e), g);
+      update_grads<kGradF16, kRows>(u, uint32_t(e), g);
   }
   const float wd = __ldg(decay + u.tensor) ? p.decay_weight : p.no_decay_weight;
   pdl_wait();  // the decision is complete and visible
@@ -1551,9 +1545,9 @@ __global__ void __launch_bounds__(kUpdateBlock, 8)
     const int32_t from = e < 0 ? 0 : e, to = e + int32_t(kVec) < count ? e + int32_t(kVec) : count;
     for (int32_t k = from; k < to; ++k) {
       const float x =
-          type == kGradF32    ? update_grad<kGradF32, kRows>(u, list, uint32_t(k))
-          : type == kGradBf16 ? update_grad<kGradBf16, kRows>(u, list, uint32_t(k))
-                              : update_grad<kGradF16, kRows>(u, list, uint32_t(k));
+          type == kGradF32    ? update_grad<kGradF32, kRows>(u, uint32_t(k))
+          : type == kGradBf16 ? update_grad<kGradBf16, kRows>(u, uint32_t(k))
+                              : update_grad<kGradF16, kRows>(u, uint32_t(k));
       const uint64_t i = u.offset + uint32_t(k);
       const float gv =
           __fmul_rn(sc.mul ? unscale<true>(x, sc) : unscale<false>(x, sc), clip);

@@ -47,7 +47,7 @@ struct slm_grad_list {
 
   GradListView view() const {
     return GradListView{d_units, d_tensors, n_units, uint32_t(tensors.size()), unit_elems, pitched,
-                        at.off_runs, off_vectors, types, cluster, sms, keep, elements};
+                        at.off_runs, off_vectors, types, cluster, sms, keep};
   }
 };
 

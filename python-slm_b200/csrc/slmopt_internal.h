@@ -321,7 +321,6 @@ struct GradListView {
   uint32_t cluster;      // blocks of the cluster for small lists, see list_small_cluster
   uint32_t sms;          // of the device
   uint32_t keep;         // units from here on stay in the L2 for a second pass
-  uint64_t elements;
 };
 struct GradListOut {
   float* result;         // norm, clip scale, largest magnitude, non-finite flag
