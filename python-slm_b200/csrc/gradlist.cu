@@ -853,7 +853,11 @@ __device__ __forceinline__ void clip_raw(const Raw<T>& raw, const ClipFactor& f,
 // What the clip needs of the norm, which may still be on its way: it is waited
 // for once per block, after the first loads have been issued.  Lists of few units
 // have no finalize kernel; every block adds the partials for itself (one launch
-// and one hop less: see kGradOwnNorm).
+// and one hop less: see kGradOwnNorm).  kOwn: whether the kernel can do that.  The
+// forms for contiguous tensors and for rows on the boundaries come without it as well,
+// for larger lists: its registers make them spill (60M bf16 in columns in place
+// 68 us without, 82 with; into bf16 69 against 72).  The form for any rows has it
+// always (60M bf16 in odd columns 135 us, against 138 without).
 struct ClipNorm {
   const float* result;          // of the finalize kernel, or NULL:
   const GradPartial* partials;  // what to form it from
@@ -862,6 +866,7 @@ struct ClipNorm {
   int kind;
   GradListOut out;
 };
+template <bool kOwn>
 struct ClipState {
   const ClipNorm* norm;
   float scale;
@@ -872,7 +877,7 @@ struct ClipState {
   __device__ __forceinline__ bool ready() {
     if (!known) {
       pdl_wait();
-      if (norm->result) {
+      if (!kOwn || norm->result) {
         clip = __ldcg(norm->result + 1);
         bad = __ldcg(norm->result + 3);
       } else {
@@ -901,9 +906,9 @@ struct ClipState {
 // input is shifted where it lies off them.
 // kAligned: both units lie on the boundaries (kGradVector).  kShift: whether the
 // input can lie off them where the output is on them (not in place).
-template <uint32_t T, uint32_t O, bool kAligned, bool kShift>
+template <uint32_t T, uint32_t O, bool kAligned, bool kShift, typename S>
 __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint32_t count,
-                                          float scale, ClipState& state) {
+                                          float scale, S& state) {
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
   constexpr uint32_t kStep = kListThreads * kVecBytes<T>;
   const uint32_t peel = kAligned ? 0u : peel_of<O>(dst, count);
@@ -963,9 +968,9 @@ __device__ __forceinline__ void clip_flat(const uint8_t* src, uint8_t* dst, uint
 }
 
 // Rows on either side where every vector is one aligned run on both.
-template <uint32_t T, uint32_t O, bool kSame>
+template <uint32_t T, uint32_t O, bool kSame, typename S>
 __device__ __forceinline__ void clip_row_vectors(const GradUnit& u, const GradUnit& o, float scale,
-                                                 ClipState& state) {
+                                                 S& state) {
   constexpr uint32_t kBatch = T == kGradF32 ? 2 : 4;
   if (!state.ready()) return;
   const ClipFactor f(state.clip, scale);
@@ -990,9 +995,9 @@ __device__ __forceinline__ void clip_row_vectors(const GradUnit& u, const GradUn
 
 // Any rows.  With rows in and contiguous memory out, vectors start at the
 // output's boundaries.
-template <uint32_t T, uint32_t O>
+template <uint32_t T, uint32_t O, typename S>
 __device__ __forceinline__ void clip_rows(const GradUnit& u, const GradUnit& o, float scale,
-                                          ClipState& state) {
+                                          S& state) {
   if (!state.ready()) return;
   const ClipFactor f(state.clip, scale);
   const uint32_t head = o.flags & kGradPitched ? 0u : peel_of<O>(o.ptr, u.count);
@@ -1026,9 +1031,9 @@ __device__ __forceinline__ void clip_rows(const GradUnit& u, const GradUnit& o, 
 }
 
 // kRows: kNoRows, kRowVectors, kAnyRows, each with the registers it needs.
-template <uint32_t T, uint32_t O, uint32_t kRows, bool kSame>
+template <uint32_t T, uint32_t O, uint32_t kRows, bool kSame, typename S>
 __device__ __forceinline__ void clip_unit(const GradUnit& u, const GradUnit& o, float scale,
-                                          ClipState& state) {
+                                          S& state) {
   if (kRows == kRowVectors && ((u.flags | o.flags) & kGradPitched))
     clip_row_vectors<T, O, kSame>(u, o, scale, state);
   else if (kRows == kAnyRows && ((u.flags | o.flags) & kGradPitched))
@@ -1065,11 +1070,11 @@ __device__ __noinline__ void clip_elements(const GradUnit* units, const GradUnit
 }
 
 // kOut: the output type (units written in another one are left to the launch for
-// theirs), or in place.  All nine pairs of types in one kernel would spill.
+// theirs), or in place: three pairs of types a kernel, not nine, for its registers.
 constexpr uint32_t kOutSame = 3u;
-template <uint32_t kOut, uint32_t kRows>
+template <uint32_t kOut, uint32_t kRows, typename S>
 __device__ __forceinline__ void clip_any(const GradListView& list, const GradListView& out,
-                                         uint32_t i, float scale, ClipState& state) {
+                                         uint32_t i, float scale, S& state) {
   constexpr bool kSame = kOut == kOutSame;
   const GradUnit u = load_unit<kRows != kNoRows>(list.units, i);
   const GradUnit o = kSame ? u : load_unit<kRows != kNoRows>(out.units, i);
@@ -1089,12 +1094,12 @@ __device__ __forceinline__ void clip_any(const GradListView& list, const GradLis
   }
 }
 
-template <uint32_t kOut, uint32_t kRows>
+template <uint32_t kOut, uint32_t kRows, bool kOwn>
 __global__ void __launch_bounds__(kListThreads,
                                   kRows == kAnyRows || (kRows && kOut == kOutSame) ? 3 : 4)
     list_clip_kernel(GradListView list, GradListView out, float scale,
                      const __grid_constant__ ClipNorm norm) {
-  ClipState state{&norm, scale, 0.0f, 0.0f, false};
+  ClipState<kOwn> state{&norm, scale, 0.0f, 0.0f, false};
   // In place with a loss scale of one there may be nothing to do: look before
   // anything is loaded.
   if (kOut == kOutSame && scale == 1.0f && (!state.ready() || state.clip == 1.0f)) return;
@@ -1192,7 +1197,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   }
   if constexpr (kClip) {
     __syncthreads();
-    ClipState state{nullptr, scale, s_clip.x, s_clip.y, true};
+    ClipState<false> state{nullptr, scale, s_clip.x, s_clip.y, true};
     if (!state.ready() || (kMode == kOutSame && scale == 1.0f && state.clip == 1.0f)) return;
     for (uint32_t i = begin; i < list.n_units; i += step)
       clip_any<kMode, kAnyRows>(list, to, i, scale, state);
@@ -1720,9 +1725,14 @@ namespace {
 template <uint32_t kOut>
 cudaError_t launch_clip_to(const GradListView& list, const GradListView& out, float scale,
                            const ClipNorm& norm, cudaStream_t stream) {
-  const auto kernel = !list.rows && !out.rows ? list_clip_kernel<kOut, kNoRows>
-                      : list.off_runs || out.off_runs ? list_clip_kernel<kOut, kAnyRows>
-                                                      : list_clip_kernel<kOut, kRowVectors>;
+  const bool own = norm.result == nullptr;
+  const auto kernel =
+      !list.rows && !out.rows
+          ? (own ? list_clip_kernel<kOut, kNoRows, true> : list_clip_kernel<kOut, kNoRows, false>)
+      : list.off_runs || out.off_runs
+          ? list_clip_kernel<kOut, kAnyRows, true>
+          : (own ? list_clip_kernel<kOut, kRowVectors, true>
+                 : list_clip_kernel<kOut, kRowVectors, false>);
   // Where there may be nothing to do, one wave of blocks that walk the units, so
   // that leaving is quick (135M below the limit: 44.7 us with the norm, against 76
   // for a block per unit); else a block per unit, which the hardware balances.
