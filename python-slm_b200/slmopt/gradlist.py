@@ -65,23 +65,24 @@ class GradientNorm:
     is not finite (the clip scale is then 0.0) else 0.0; and with per_tensor each
     tensor's norm, then each tensor's largest magnitude."""
 
-    __slots__ = ("_buffer", "_count", "_tensors", "_index", "_stream", "_event", "_after")
+    __slots__ = ("_buffer", "_count", "_tensors", "_call", "_after")
 
-    def __init__(self, buffer, count: int, tensors: int, index: int, stream: int, event):
+    def __init__(self, buffer, count: int, tensors: int, call: tuple):
         # f32: the values, the f64 sum of squares, and scratch of the call.
         self._buffer = buffer
         self._count = count
         self._tensors = tensors
-        self._index = index     # of the device
-        self._stream = stream   # the call's
-        self._event = event     # behind the call, if that stream was not the current one
-        self._after = stream    # the last one ordered behind it
+        # The device's index, the call's stream, and an event behind the call if that
+        # was not the current stream.
+        self._call = call
+        self._after = None  # the last stream ordered behind it
 
     def _ready(self):
         """The buffer, with the current stream behind the call."""
-        current = _current_stream(self._index)
-        if current != self._stream and current != self._after and \
-                _order_behind(self._buffer, self._index, self._stream, self._event):
+        index, stream, event = self._call
+        current = _current_stream(index)
+        if current != stream and current != self._after and \
+                _order_behind(self._buffer, index, stream, event):
             self._after = current
         return self._buffer
 
@@ -166,7 +167,7 @@ class GradientList:
         # caller owns (and may destroy) an event behind the last call there.
         self._streams: dict = {}
         self.elements = int(self.lib.slm_grad_list_elements(h))
-        self._work_bytes = int(self.lib.slm_grad_list_workspace_bytes(h))
+        self._lay_out(int(self.lib.slm_grad_list_workspace_bytes(h)))
         # What every call needs, looked up once.
         self._empty, self._f32, self._index = torch.empty, torch.float32, self.device.index
         self._tensor_type, self._strided = torch.Tensor, torch.strided
@@ -196,6 +197,19 @@ class GradientList:
                 t.is_contiguous() and t.numel() == shape[2]:
             return not t.is_neg()
         return self._layout(t) == shape
+
+    def _lay_out(self, work_bytes: int) -> None:
+        """Where a call's results and workspace go: for calls without and with
+        per_tensor the number of values, where the workspace begins in the results'
+        allocation (in f32), and the elements of that allocation.  A small workspace
+        shares it; a large one is freed with the call instead of living as long as
+        the results."""
+        self._work_bytes = work_bytes
+        self._shared = work_bytes <= _SHARED_BYTES
+        counts = (4, 4 + 2 * len(self.tensors))
+        heads = [(count + 5) & ~3 for count in counts]
+        self._plan = [(count, head, head + work_bytes // 4 if self._shared else head)
+                      for count, head in zip(counts, heads)]
 
     def __len__(self) -> int:
         return len(self.tensors)
@@ -268,26 +282,19 @@ class GradientList:
             raise ValueError('kind must be "l2" or "max"')
         h = self._h or self.handle
         n = len(self.tensors)
-        count = 4 + 2 * n if per_tensor else 4
-        # A small workspace shares the results' allocation; a large one is freed
-        # with the call instead of living as long as the results.
-        head = (count + 5) & ~3
-        # Both come from the memory of the stream that the call runs on: another
-        # stream's may still be in use by what is queued there.
-        small = self._work_bytes <= _SHARED_BYTES
+        count, head, room = self._plan[1 if per_tensor else 0]
+        # Results and workspace come from the memory of the stream that the call runs
+        # on: another stream's may still be in use by what is queued there.
         s = None if stream is None else _stream_handle(stream)
         on = s or 0
         away = _current_stream(self._index) != on
         if away:
             with _on_stream(self._index, s):
-                buffer, work = self._room(head, small)
-        elif small:
-            buffer = work = self._empty(head + self._work_bytes // 4, dtype=self._f32,
-                                        device=self.device)
+                buffer, work = self._room(room)
         else:
-            buffer, work = self._room(head, False)
+            buffer, work = self._room(room)
         v = buffer.data_ptr()
-        w = v + 4 * head if small else work.data_ptr()
+        w = v + 4 * head if work is None else work.data_ptr()
         norms, tops = (v + 16, v + 16 + 4 * n) if per_tensor else (None, None)
         if write:
             to = None if out is None else out._h or out.handle
@@ -298,23 +305,18 @@ class GradientList:
                                  self._work_bytes, s)
         if st:
             _lib.check(st)
-        event = None
-        if away:
-            event = _event_on(self._index, on)
-            self._streams[on] = event if isinstance(stream, int) else None
-        else:
-            self._streams[on] = None
+        event = _event_on(self._index, on) if away else None
+        self._streams[on] = owned = event if isinstance(stream, int) else None
         if out is not None:
-            out._streams[on] = self._streams[on]
-        return GradientNorm(buffer, count, n, self._index, on, event)
+            out._streams[on] = owned
+        return GradientNorm(buffer, count, n, (self._index, on, event))
 
-    def _room(self, head: int, small: bool):
-        """Results and workspace of a call, from the current stream's memory."""
-        buffer = self._empty(head + self._work_bytes // 4 if small else head, dtype=self._f32,
-                             device=self.device)
-        if small:
-            return buffer, buffer
-        return buffer, self._empty(self._work_bytes // 4, dtype=self._f32, device=self.device)
+    def _room(self, elements: int):
+        """Results of a call, and its workspace where they do not share, from the
+        current stream's memory."""
+        buffer = self._empty(elements, dtype=self._f32, device=self.device)
+        return buffer, None if self._shared else self._empty(
+            self._work_bytes // 4, dtype=self._f32, device=self.device)
 
     def accumulate(self, acc, overwrite: bool = False, stream=None) -> None:
         """acc (f32, one value per element, tensor after tensor) += the

@@ -53,7 +53,8 @@ def a_list(log, work_bytes=64):
     lst.tensors = (torch.ones(3), torch.ones(2))
     lst.device, lst._index = torch.device("cpu"), 0
     lst._streams = {}
-    lst.elements, lst._work_bytes, lst._f32 = 5, work_bytes, torch.float32
+    lst.elements, lst._f32 = 5, torch.float32
+    lst._lay_out(work_bytes)
 
     def empty(n, dtype, device):
         log.events.append(("allocate", log.now.stream))
