@@ -488,13 +488,15 @@ int slm_grad_list_norm(const slm_grad_list* list, float loss_scale, float max_no
                        slm_list_norm* result_device, float* tensor_norms_device,
                        float* tensor_max_device, double* sum_squares_device,
                        void* workspace_device, uint64_t workspace_bytes, void* stream);
-/* The norm, and every gradient divided by the loss scale and multiplied by the
- * clip scale (each in f32, rounded once more to the output's type, nearest
- * even), written to `out` -- a list of tensors of the same sizes, of any type
+/* The norm, and every gradient times clip_scale / loss_scale, a quotient formed
+ * once in f32 (the product is rounded to f32 and once more to the output's type,
+ * nearest even; with a loss scale that is no power of two it can differ in its last
+ * bit from a division of every element, which the step makes), written to `out` -- a list of tensors of the same sizes, of any type
  * and layout -- or in place when out is NULL or the list itself.  Nothing is
  * written when a gradient is not finite.  Output tensors that share elements
  * with each other, or with a gradient other than the same one in the same
- * layout and type, are refused. */
+ * layout and type, are refused (in rows of pitches with no common divisor wide
+ * enough for both, also where they only might). */
 int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, float loss_scale,
                        float max_norm, int kind, slm_list_norm* result_device,
                        float* tensor_norms_device, float* tensor_max_device,

@@ -11,8 +11,9 @@ evaluation / checkpoint boundary was crossed and whether training is done).
 
 ``UpdateAccounting`` restates that bookkeeping on the host (it is scalar
 integer work; nothing here touches a gradient).  ``B200Trainer`` drives the
-device path with it: micro-batch gradients are summed on the GPU
-(``slm_grad_accumulate``), the last micro-batch of an update goes through the
+device path with it: micro-batch gradients, one flat tensor or a ``GradientList``
+each, are summed on the GPU (``slm_grad_accumulate``,
+``slm_grad_list_accumulate``), the last micro-batch of an update goes through the
 fused accumulate + norm pass, normalised by the update's target count, then
 the update pass and the state hash.  Evaluation and the forward/backward graph
 are not part of this path: ``checkpoint_due`` reports the boundary the
