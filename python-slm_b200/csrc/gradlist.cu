@@ -353,7 +353,7 @@ __device__ __forceinline__ GradUnit load_unit(const GradUnit* units, uint32_t i)
 // first form (unscaling and squaring each value, 66 warp instructions an 8-element
 // vector) was bound by issue at 71 % instead.  Squares by packed fused multiply-adds of the
 // stored values take 40, 32 registers keep 8 blocks of 256 threads a SM resident
-// with 64 bytes a thread on their way: 135M bf16 in 42-43 us with the finalize
+// with 64 bytes a thread on their way: 135M bf16 in 42-44 us with the finalize
 // (6.5 TB/s; a kernel that only reads the same bytes takes 39.4-42.7), 49 us at
 // the start.  Off the vector boundaries a vector costs two loads and a shift:
 // 120M bf16 in odd-sized packed tensors 57.5 us against 37.8 (vectors start at the
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(kLanes)
 // y = round(x * (clip / scale)): a second read and the write behind the norm's
 // read.  DRAM bounds it: 135M bf16 read, mostly read again (the L2 keeps the last
 // 24 MB, see kGradKeepBytes) and written are 790 MB, 120 us at 6.57 TB/s; measured
-// 125-127 us.  Keeping more on chip than the L2 does was not tried: 30 MB of shared
+// 125-129 us.  Keeping more on chip than the L2 does was not tried: 30 MB of shared
 // memory would save 4.6 us.
 constexpr uint32_t kNoRows = 0u, kRowVectors = 1u, kAnyRows = 2u;
 template <uint32_t T>
@@ -1210,7 +1210,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
 // acc = micro or acc + micro, one f32 rounding an element: 10 bytes an element from
 // bf16 (6 to start an update), so DRAM alone bounds it.  32-byte loads and stores
 // of the accumulator, everything first to leave the L2, 8,192 elements a block:
-// 135M from bf16 in 201 us (6.73 TB/s; a plain copy reaches 6.57), 216 us with
+// 135M from bf16 in 201-204 us (6.7 TB/s; a plain copy reaches 6.57), 216 us with
 // 2,048 a block, 204 with 16,384.
 constexpr uint32_t kAccElems = 8192;
 __device__ __forceinline__ void load_acc(const float* p, float (&y)[8]) {
@@ -1361,7 +1361,7 @@ __global__ void __launch_bounds__(kListThreads, 4)
 
 // The last micro-batch: accumulates the unit's vectors in the tree's order (from
 // its first element, the last one padded with +0.0) and adds the squares of the
-// sums.  135M bf16 in 205 us (accumulate alone 201); where the accumulator's vectors are
+// sums.  135M bf16 in 205 us (accumulate alone 201-204); where the accumulator's vectors are
 // off its 32-byte boundaries, as behind odd sizes, it is read and written value by
 // value: 9M in 61 odd-sized tensors 27.9 us against 11.5.
 template <uint32_t T, bool kFactor>
@@ -1459,9 +1459,9 @@ __global__ void __launch_bounds__(kListThreads)
 // boundaries is shifted.
 //
 // 28 bytes an element (bf16 gradients), bound by DRAM: all loads are in flight
-// before the norm is finished (pdl_wait), 64 registers and 128 threads a block keep
+// before the norm is finished (pdl_wait), 62 registers and 128 threads a block keep
 // 112 KB a SM on their way, and the hardware balances the blocks.  135M elements:
-// step 627-642 us, of which the update 585-600 (6.4 TB/s).  The flat step's form
+// step 627-647 us, of which the update 585-605 (6.4 TB/s).  The flat step's form
 // (2,048-element tiles by bulk copies into shared memory, 3 blocks a SM) took
 // 667 us here; 256 / 512 threads a block 663 / 688, two vectors a thread 761.
 constexpr uint32_t kUpdateBlock = 128;

@@ -315,7 +315,10 @@ void slmopt::drop_norm_pass(slm_opt_handle* h, cudaStream_t s) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(s, &status) != cudaSuccess) cudaGetLastError();
   if (status != cudaStreamCaptureStatusNone) {
-    h->parked_lists.push_back(list);
+    try {
+      h->parked_lists.push_back(list);
+    } catch (const std::exception&) {  // without room to note it, it is kept for good
+    }
     return;
   }
   cudaStreamSynchronize(s);

@@ -310,7 +310,9 @@ inline uint32_t grad_unit_elems(uint64_t total) {
   while (u < kGradUnitMax && total / u > kGradUnitsAimed) u *= 2;
   return u;
 }
-struct GradListView {
+// On 16 bytes, as a kernel's first parameter: those behind it then keep the alignment that
+// the compiler loads them by (list_update_kernel: 62 registers, else 64).
+struct __align__(16) GradListView {
   const GradUnit* units;
   const GradTensor* tensors;
   uint32_t n_units, n_tensors;
