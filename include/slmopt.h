@@ -420,11 +420,11 @@ int slm_grad_norm_noalloc(const void* grads, int dtype, uint64_t n, float loss_s
  *
  * A list borrows its tensors: they must stay allocated while the list or work
  * enqueued with it uses them.  A captured call reads the list's tables at every
- * replay, so the list must outlive the graph.  It is immutable but for slm_grad_list_bind, so
- * calls with it may run at the same time on several streams or in several
- * captured graphs, each with its own workspace and results; all but
- * slm_grad_list_create and _destroy may be captured.  Elements are counted in
- * row-major order, tensor after tensor.
+ * replay, so the list must outlive the graph.  It is immutable but for
+ * slm_grad_list_bind, so calls with it may run at the same time on several
+ * streams or in several captured graphs, each with its own workspace and
+ * results; all but slm_grad_list_create and _destroy may be captured.  Elements
+ * are counted in row-major order, tensor after tensor.
  *
  * Norm: each tensor is cut into units of consecutive elements (a power of two
  * between 8,192 and 2^26, so that a list has about 16,384 of them at most).
@@ -464,7 +464,8 @@ int slm_grad_list_create(const slm_grad_view* views, uint32_t n, int device,
                          slm_grad_list** out);
 /* Waits for the device's outstanding work, then frees the list.  Graphs that have
  * captured a call with the list must not be replayed any more.  While a stream
- * is captured it fails (SLM_ERR_CUDA; the list lives on). */
+ * is captured the wait is refused (SLM_ERR_CUDA, the list lives on), and the
+ * capture is lost. */
 int slm_grad_list_destroy(slm_grad_list* list);
 uint64_t slm_grad_list_elements(const slm_grad_list* list);
 /* Bytes of device workspace of one norm or clip call. */
@@ -488,15 +489,16 @@ int slm_grad_list_norm(const slm_grad_list* list, float loss_scale, float max_no
                        slm_list_norm* result_device, float* tensor_norms_device,
                        float* tensor_max_device, double* sum_squares_device,
                        void* workspace_device, uint64_t workspace_bytes, void* stream);
-/* The norm, and every gradient times clip_scale / loss_scale, a quotient formed
- * once in f32 (the product is rounded to f32 and once more to the output's type,
- * nearest even; with a loss scale that is no power of two it can differ in its last
- * bit from a division of every element, which the step makes), written to `out` -- a list of tensors of the same sizes, of any type
- * and layout -- or in place when out is NULL or the list itself.  Nothing is
- * written when a gradient is not finite.  Output tensors that share elements
- * with each other, or with a gradient other than the same one in the same
- * layout and type, are refused (in rows of pitches with no common divisor wide
- * enough for both, also where they only might). */
+/* The norm, and every gradient times clip_scale / loss_scale, written to `out` --
+ * a list of tensors of the same sizes, of any type and layout -- or in place when
+ * out is NULL or the list itself.  The quotient is formed once in f32; the
+ * product is rounded to f32 and once more to the output's type, nearest even.
+ * (With a loss scale that is no power of two it can differ in its last bit from
+ * the division of every element that the step makes.)  Nothing is written when
+ * a gradient is not finite.  Output tensors that share elements with each other,
+ * or with a gradient other than the same one in the same layout and type, are
+ * refused (in rows of pitches with no common divisor wide enough for both, also
+ * where they only might). */
 int slm_grad_list_clip(const slm_grad_list* list, const slm_grad_list* out, float loss_scale,
                        float max_norm, int kind, slm_list_norm* result_device,
                        float* tensor_norms_device, float* tensor_max_device,

@@ -403,7 +403,7 @@ int slm_grad_list_destroy(slm_grad_list* list) {
   // Work enqueued with the list (on any stream) has read its tables, and its
   // tensors, when this returns; an update pass to come may still read them.
   const cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaErrorStreamCaptureUnsupported) {
+  if (e >= cudaErrorStreamCaptureUnsupported && e <= cudaErrorStreamCaptureWrongThread) {
     cudaGetLastError();
     return fail(SLM_ERR_CUDA, "a gradient list cannot be destroyed while a stream is captured");
   }

@@ -244,7 +244,8 @@ class GradientList:
     def bind(self, tensors, stream=None) -> None:
         """Take other tensors of the same types, sizes and strides, in order.  The
         old ones are let go; torch's allocator learns which streams calls of the
-        list have used them on."""
+        list have used them on (calls on a stream given by its handle, other than
+        torch's current one, are waited for)."""
         tensors = tuple(tensors)
         if len(tensors) != len(self._shapes) or \
                 not all(self._is(t, shape) for t, shape in zip(tensors, self._shapes)):

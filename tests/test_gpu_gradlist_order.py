@@ -651,3 +651,21 @@ def test_streams_of_the_callers_own_may_end_before_results_are_read(torch):
             del r
             lst.bind(new)
             lst.bind(tensors)
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2], ids=["global", "thread", "relaxed"])
+def test_a_list_destroyed_through_the_abi_inside_a_capture_lives_on(torch, mode):
+    """The runtime refuses the wait (and ends the capture): an error, nothing runs."""
+    tensors = make(torch, [70_001, 33], seed=110)
+    runtime = ctypes.CDLL("libcudart.so.12")
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    with GradientList(tensors) as lst:
+        torch.cuda.synchronize()
+        assert runtime.cudaStreamCreateWithFlags(ctypes.byref(stream), 1) == 0
+        assert runtime.cudaStreamBeginCapture(stream, mode) == 0
+        got = lst.lib.slm_grad_list_destroy(lst.handle)
+        runtime.cudaStreamEndCapture(stream, ctypes.byref(graph))
+        runtime.cudaGetLastError()
+        assert runtime.cudaStreamDestroy(stream) == 0
+        assert got == _lib.SLM_ERR_CUDA
+        near(lst.norm().read().norm, norm64(tensors), 4 * U, "norm")
